@@ -13,6 +13,7 @@
 #include <unordered_map>
 
 #include "b200norm.h"
+#include "host.h"
 #include "norm_bwd.cuh"
 #include "norm_colreduce.cuh"
 #include "norm_fwd.cuh"
@@ -26,10 +27,26 @@ namespace b200norm {
 namespace {
 
 constexpr int kMaxDevices = 64;
-constexpr int64_t kMaxRowBytes = 65536;  // the reference's limit (layernorm.py:69-72)
 constexpr int kLN = 0, kRMS = 1;
 
 thread_local char g_err[512] = "";
+DeviceState g_dev[kMaxDevices];
+
+// Tuning builds only (-DB200NORM_TUNING, which the shipped library is not built with): an environment
+// variable, read once, that overrides a launch decision -- the index of the table entry to use
+// whenever it can hold the row (B200NORM_FORCE_FWD / _BWD / _SOFTMAX / _PNORM), or B200NORM_PDL=0 to
+// launch without programmatic dependent launch.  Without the flag these return `fallback`.
+int tuning_env(const char* name, int fallback) {
+#ifdef B200NORM_TUNING
+  const char* v = std::getenv(name);
+  return v != nullptr ? std::atoi(v) : fallback;
+#else
+  (void)name;
+  return fallback;
+#endif
+}
+
+}  // namespace
 
 int fail(int code, const char* fmt, ...) {
   va_list ap;
@@ -39,26 +56,6 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-struct DeviceState {
-  // Launch planning: SM count, occupancies, shared-memory allowances.  Set up without allocating
-  // anything, and shared by every entry point -- a kernel's shared-memory allowance is a property
-  // of the device, so there must be exactly one record of it per device.
-  std::once_flag once;
-  cudaError_t init_err = cudaSuccess;
-  int sm_count = 0;
-  std::mutex mu;
-  std::unordered_map<unsigned long long, int> occupancy;  // (kernel, dyn smem) -> CTAs per SM
-  std::unordered_map<const void*, size_t> smem_limit;     // kernel -> dynamic shared memory it has been allowed
-  // Status word: pinned, mapped host memory where kernels report a timed-out wait.  Allocated by the
-  // first call of an entry point that reports through it (never by b200norm_rms_bwd_static).
-  std::once_flag status_once;
-  cudaError_t status_err = cudaSuccess;
-  int* status_host = nullptr;
-  int* status_dev = nullptr;
-};
-DeviceState g_dev[kMaxDevices];
-
-// The launch-planning part of the current device's state; allocates nothing.
 int device_caches(DeviceState** out) {
   int d = -1;
   cudaError_t e = cudaGetDevice(&d);
@@ -74,7 +71,9 @@ int device_caches(DeviceState** out) {
   return B200NORM_OK;
 }
 
-// Per-device set-up, run by the first call on each device: the above plus the status word.
+namespace {
+
+// Per-device set-up, run by the first call on each device: the launch-planning part plus the status word.
 int device_state(DeviceState** out) {
   DeviceState* s = nullptr;
   if (int rc = device_caches(&s)) return rc;
@@ -90,9 +89,9 @@ int device_state(DeviceState** out) {
   return B200NORM_OK;
 }
 
-// Resident CTAs per SM of `fn` at this block size and dynamic shared memory (cluster == 1), or
-// resident clusters on the whole device (cluster > 1); cached.
-int occupancy(DeviceState& s, const void* fn, int threads, size_t smem, int* out, int cluster = 1) {
+}  // namespace
+
+int occupancy(DeviceState& s, const void* fn, int threads, size_t smem, int* out, int cluster) {
   const unsigned long long key =
       (reinterpret_cast<unsigned long long>(fn) * 0x9E3779B97F4A7C15ull) ^ (unsigned long long)smem;
   std::lock_guard<std::mutex> lock(s.mu);
@@ -102,11 +101,11 @@ int occupancy(DeviceState& s, const void* fn, int threads, size_t smem, int* out
     return B200NORM_OK;
   }
   cudaError_t e;
-  // Static shared memory counts toward the 48 KB default limit too, hence 32 KB.  The limit is only
+  // Static shared memory (up to 18 KB beside dynamic) counts toward the 48 KB default limit too.  The limit is only
   // ever raised: one kernel serves a range of row lengths, and a shorter row after a longer one must
   // not take the allowance away from a launch shape whose occupancy is already cached.
   size_t& allowed = s.smem_limit[fn];
-  if (smem > 32 * 1024 && smem > allowed) {
+  if (smem > 28 * 1024 && smem > allowed) {
     e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess)
       return fail(B200NORM_ERR_CUDA, "cudaFuncSetAttribute(%zu B): %s", smem, cudaGetErrorString(e));
@@ -136,6 +135,8 @@ int occupancy(DeviceState& s, const void* fn, int threads, size_t smem, int* out
   return B200NORM_OK;
 }
 
+namespace {
+
 // The kernel table of a storage type and a fused activation (0 none, 1 GeLU erf, 2 GeLU tanh).
 const DTypeKernels* kernels_for(int dtype, int act = 0) {
 #define B200NORM_PICK(name) \
@@ -151,22 +152,6 @@ const DTypeKernels* kernels_for(int dtype, int act = 0) {
 }
 
 bool valid_act(int act) { return act >= B200NORM_ACT_NONE && act <= B200NORM_ACT_GELU_TANH; }
-
-// Tuning builds only (-DB200NORM_TUNING, which the shipped library is not built with): an environment
-// variable, read once, that overrides a launch decision -- the index of the table entry to use
-// whenever it can hold the row (B200NORM_FORCE_FWD / _BWD / _SOFTMAX / _PNORM), or B200NORM_PDL=0 to
-// launch without programmatic dependent launch.  Without the flag these return `fallback`.
-int tuning_env(const char* name, int fallback) {
-#ifdef B200NORM_TUNING
-  const char* v = std::getenv(name);
-  return v != nullptr ? std::atoi(v) : fallback;
-#else
-  (void)name;
-  return fallback;
-#endif
-}
-
-constexpr size_t kMaxSmemPerCta = 227 * 1024;  // opt-in dynamic + static shared memory of one sm_100 CTA
 
 bool valid_dtype(int d) { return d >= B200NORM_F32 && d <= B200NORM_F64; }
 
@@ -199,10 +184,10 @@ const PacketKernel* pick(const PacketKernel* tab, int n, int64_t V, bool bwd = f
   return nullptr;
 }
 
-// `pdl`: launch with programmatic stream serialization (the kernel calls grid_dependency_sync()
-// before its first global access); the any-alignment kernels do not and are launched plainly.
-int launch(const void* fn, dim3 grid, dim3 block, size_t smem, void* params, cudaStream_t stream, bool pdl = true,
-           int cluster = 1) {
+}  // namespace
+
+int launch(const void* fn, dim3 grid, dim3 block, size_t smem, void* params, cudaStream_t stream, bool pdl,
+           int cluster) {
   void* args[1] = {params};
   cudaError_t e;
   static const bool pdl_enabled = tuning_env("B200NORM_PDL", 1) != 0;
@@ -235,6 +220,21 @@ int launch(const void* fn, dim3 grid, dim3 block, size_t smem, void* params, cud
   if (e != cudaSuccess) return fail(B200NORM_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
   return B200NORM_OK;
 }
+
+int launch_colreduce(const float* part, int rows, int64_t N, void* dw, int w_dtype, cudaStream_t stream) {
+  ColReduceParams c;
+  c.part[0] = part; c.part[1] = nullptr;
+  c.out[0] = dw; c.out[1] = nullptr;
+  c.group_sums = nullptr;
+  c.per_shard = rows; c.row_shards = 1; c.slots = 1; c.N = static_cast<int>(N); c.w_dtype = w_dtype;
+  if (N % 4 == 0)
+    return launch(reinterpret_cast<const void*>(&colreduce4_kernel), dim3(static_cast<unsigned>((N + 127) / 128)),
+                  dim3(32, 16), 0, &c, stream);
+  return launch(reinterpret_cast<const void*>(&colreduce_kernel), dim3(static_cast<unsigned>((N + 31) / 32)),
+                dim3(32, 16), 0, &c, stream);
+}
+
+namespace {
 
 // Launches an any-alignment row kernel (forward: one staged row per ring slot, backward dx: two).
 // Shared memory per CTA = (rows_per_slot * slots + 1) row buffers; four slots when that leaves room
