@@ -310,6 +310,81 @@ B200NORM_API int b200norm_finalize_pushed(const b200norm_peers* peers, uint64_t 
                                           int64_t N, int w_dtype, void* stream);
 
 /*
+ * RMSNorm with the residual addition in front of it.  (No counterpart in the reference.)
+ *
+ * b200norm_add_rms_fwd: h = x + residual rounded to the residual's type, rstd = 1/sqrt(sum(h^2)/N + eps),
+ *   y = h*rstd [*w].  x and y are io_dtype, residual and h res_dtype: the same type, or B200NORM_F32
+ *   (io_dtype F32, F16 or BF16).  w may be NULL.  rstd is an (M,) fp32 output saved for backward.
+ * b200norm_add_rms_bwd: with xhat = h*rstd, wdy = w*dy, c1 = sum(xhat*wdy)/N:
+ *   d = (wdy - xhat*c1)*rstd + dh;  dx = d in io_dtype, dres = d in res_dtype;  dw = sum_rows(dy*xhat).
+ *   dh (the gradient of h) and dw may be NULL.  dres is written when res_dtype is not io_dtype; it must be
+ *   NULL when it is (dx is the gradient of both then).  workspace: needed for dw, at least
+ *   b200norm_add_rms_bwd_workspace_bytes bytes, 256-byte aligned; contents undefined on entry and exit.
+ * No output may overlap an input.
+ */
+B200NORM_API int b200norm_add_rms_fwd(const void* x, int64_t x_row_stride, const void* residual,
+                                      int64_t residual_row_stride, const void* w, void* y, int64_t y_row_stride,
+                                      void* h, int64_t h_row_stride, float* rstd, int64_t M, int64_t N, float eps,
+                                      int io_dtype, int res_dtype, int w_dtype, void* stream);
+B200NORM_API size_t b200norm_add_rms_bwd_workspace_bytes(int64_t M, int64_t N, int io_dtype, int res_dtype);
+B200NORM_API int b200norm_add_rms_bwd(const void* h, int64_t h_row_stride, const void* dy, int64_t dy_row_stride,
+                                      const void* dh, int64_t dh_row_stride, const void* w, const float* rstd,
+                                      void* dx, int64_t dx_row_stride, void* dres, int64_t dres_row_stride, void* dw,
+                                      void* workspace, size_t workspace_bytes, int64_t M, int64_t N, int io_dtype,
+                                      int res_dtype, int w_dtype, void* stream);
+
+/*
+ * RMSNorm with an 8-bit output.  As b200norm_add_rms_fwd (residual NULL: h = x, and h must be NULL; with a
+ * residual h may be NULL), but the unrounded y is stored as e4m3 bytes q (M, N) with one scale per `group`
+ * columns -- 32, 64 or 128, the last group of a row may be shorter -- or per row (group 0):
+ *   scale = max(largest |y| of the group, 2^-64) / 448, q = e4m3(y / scale).
+ * scale is (M, ceil(N / group)) or (M,) contiguous: fp32, or with e8m0 != 0 rounded up to a power of two
+ * and stored as its biased exponent in a byte.  A NaN in a group makes its scale NaN.
+ */
+B200NORM_API int b200norm_rms_fp8(const void* x, int64_t x_row_stride, const void* residual,
+                                  int64_t residual_row_stride, const void* w, void* q, int64_t q_row_stride,
+                                  void* scale, void* h, int64_t h_row_stride, int64_t M, int64_t N, float eps,
+                                  int group, int e8m0, int io_dtype, int res_dtype, int w_dtype, void* stream);
+
+/*
+ * Choice of a token per row of logits (M, V), V <= 262144, io_dtype F32, F16 or BF16, with given random
+ * numbers uniform (M,) in [0, 1): temperature, top-k, top-p and min-p, each one number or, where the
+ * *_v pointer is not NULL, one per row.  weight_i = exp((l_i - max l) / temperature); kept are the first
+ * top_k tokens in order of (logit descending, index ascending), of those the shortest prefix that holds
+ * top_p of their weight, of those the ones of weight >= min_p; drawn is the lowest index at which the
+ * running sum of the kept weights, in index order, exceeds uniform * total.  temperature <= 0: the likeliest
+ * token; top_k outside [1, V), top_p >= 1, min_p <= 0: off.  tokens (M,): -1 for a row that holds a NaN or
+ * nothing above -inf.  Needs no workspace.
+ */
+B200NORM_API int b200norm_sample(const void* logits, int64_t row_stride, const float* uniform,
+                                 const float* temperature_v, float temperature, const int* top_k_v, int top_k,
+                                 const float* top_p_v, float top_p, const float* min_p_v, float min_p,
+                                 int64_t* tokens, int64_t M, int64_t V, int io_dtype, void* stream);
+
+/*
+ * Choice of k experts per token from router logits (T, E), E <= 1024, k <= min(32, E), io_dtype F32, F16 or
+ * BF16, with counts and a balance loss.  p = softmax(logits); the k largest logits are chosen, ties to the
+ * lower index; gates (T, k) are their p, divided by the sum of the chosen p when normalize != 0.
+ * counts (E + 1): tokens that chose each expert, then the number n of live tokens.
+ * loss = E * sum_e (counts_e / (n k)) * (sum_t p_te / n), 0 when n = 0.
+ * Not live: tokens whose mask (T,) byte is 0 (mask may be NULL) or whose logits are all -inf; they get
+ * experts -1, gates 0.  Slots left over when fewer than k logits are above -inf get the same.
+ * lse (T,), needed for backward only (else NULL): log-sum-exp of the logits, -inf for tokens not live.
+ * b200norm_route_bwd: gradients dgates (T, k) and dloss (one fp32 value on the device), either NULL, to dlogits (T, E)
+ *   contiguous; counts are taken as constants.
+ * workspace: at least b200norm_route_workspace_bytes bytes, 16-byte aligned.
+ */
+B200NORM_API size_t b200norm_route_workspace_bytes(int64_t T, int E, int k, int io_dtype);
+B200NORM_API int b200norm_route_fwd(const void* logits, int64_t row_stride, const uint8_t* mask, float* gates,
+                                    int* experts, float* lse, int* counts, float* loss, void* workspace,
+                                    size_t workspace_bytes, int64_t T, int E, int k, int normalize, int io_dtype,
+                                    void* stream);
+B200NORM_API int b200norm_route_bwd(const void* logits, int64_t row_stride, const float* gates, const int* experts,
+                                    const float* lse, const int* counts, const float* dgates,
+                                    int64_t dgates_row_stride, const float* dloss, void* dlogits, int64_t T, int E,
+                                    int k, int normalize, int io_dtype, void* stream);
+
+/*
  * RMSNorm backward for callers that cannot allocate device memory.  (No counterpart in the
  * reference, whose wrapper allocates its partial-sum buffers with torch on every call.)
  *

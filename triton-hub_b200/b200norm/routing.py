@@ -1,0 +1,118 @@
+"""Choice of experts from router logits on libb200norm.so: softmax, the k likeliest experts of each token,
+how many tokens chose each expert, and the balance loss, with gradients.
+
+    p = softmax(logits);  gates: p of the chosen, or (normalize) their share of the chosen p
+    f_e = counts_e / (n k),  P_e = mean p_e over the n live tokens,  loss = E * sum_e f_e P_e   (1 when balanced)
+
+The gradient reaches the logits through the gates and through P; f is a count.  Ties go to the lower index.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .functional import _code, _on_device, _ptr, _raw_stream, _require_cuda, _row_stride, _rows
+
+_WS_BYTES = {}  # (device, T, E, k, dtype code) -> workspace bytes; the answer never changes
+
+
+def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True):
+    """Returns (gates fp32 (..., k), experts int32 (..., k), counts int32 (E + 1,) whose last is the number of live
+    tokens, loss fp32 scalar, lse fp32 (T,) or None)."""
+    _require_cuda(logits)
+    if logits.dtype == torch.float64:
+        raise RuntimeError("b200norm: router logits of dtype torch.float64 are not supported (float32, float16, bfloat16)")
+    shape, device = logits.shape[:-1], logits.device
+    code = _code(logits, "router logits")
+    if mask is not None:
+        if mask.shape != shape or mask.device != device or mask.dtype not in (torch.bool, torch.uint8):
+            raise RuntimeError(f"b200norm: mask is bool, one value a token, of shape {tuple(shape)} on {device}; got "
+                               f"{tuple(mask.shape)} of {mask.dtype} on {mask.device}")
+        mask = mask.contiguous()
+    x = _rows(logits)
+    T, E = x.shape
+    gates = torch.empty((*shape, k), dtype=torch.float32, device=device)
+    experts = torch.empty((*shape, k), dtype=torch.int32, device=device)
+    counts = torch.empty((E + 1,), dtype=torch.int32, device=device)
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    lse = torch.empty((T,), dtype=torch.float32, device=device) if need_lse else None
+    lib = _lib.load()
+    index = device.index
+    with _on_device(index):
+        key = (index, T, E, k, code)
+        ws_bytes = _WS_BYTES.get(key)
+        if ws_bytes is None:
+            ws_bytes = lib.b200norm_route_workspace_bytes(T, E, k, code)
+            if ws_bytes == 0:
+                _lib.check(_lib.ERR_ARG)
+            _WS_BYTES[key] = ws_bytes
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=device)
+        _lib.check(lib.b200norm_route_fwd(
+            x.data_ptr(), _row_stride(x), _ptr(mask), gates.data_ptr(), experts.data_ptr(), _ptr(lse), counts.data_ptr(),
+            loss.data_ptr(), ws.data_ptr(), ws_bytes, T, E, k, int(bool(normalize)), code, _raw_stream(index)))
+    return gates, experts, counts, loss, lse
+
+
+def _route_bwd(logits, gates, experts, counts, lse, dgates, dloss, normalize=True):
+    """Gradients of (gates, loss), either of which may be None, with respect to the logits."""
+    _require_cuda(logits)
+    k = experts.shape[-1]
+    x = _rows(logits)
+    T, E = x.shape
+    for t in (dgates, dloss):
+        if t is not None and t.device != logits.device:
+            raise RuntimeError(f"b200norm: gradient on {t.device}, router logits on {logits.device}")
+    if dgates is not None:
+        assert dgates.shape == experts.shape, 'expect input and output shape to be the same'
+        dgates = _rows(dgates.to(torch.float32))
+    if dloss is not None:
+        dloss = dloss.to(torch.float32)
+    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    lib = _lib.load()
+    index = logits.device.index
+    with _on_device(index):
+        _lib.check(lib.b200norm_route_bwd(
+            x.data_ptr(), _row_stride(x), gates.data_ptr(), experts.data_ptr(), lse.data_ptr(), counts.data_ptr(),
+            _ptr(dgates), _row_stride(dgates) if dgates is not None else k, _ptr(dloss), dlogits.data_ptr(), T, E, k,
+            int(bool(normalize)), _code(x, "router logits"), _raw_stream(index)))
+    return dlogits
+
+
+class route(torch.autograd.Function):
+    """(logits (..., E), k, normalize, mask or None) -> (gates (..., k) fp32, experts (..., k) int32, counts (E,) int32,
+    loss fp32 scalar).  E up to 1024, k up to 32.  mask: bool, one value a token; tokens whose mask is False, and
+    tokens all of whose logits are -inf, choose nothing: experts -1, gates 0, no count, no gradient.  So do the slots
+    left over when fewer than k logits of a token are above -inf.  A NaN among a live token's logits makes its gates
+    and the loss NaN."""
+
+    @staticmethod
+    def forward(ctx, logits, k, normalize=True, mask=None):
+        gates, experts, counts, loss, lse = _route_fwd(logits, k, normalize, mask, need_lse=ctx.needs_input_grad[0])
+        chosen = counts[:-1]
+        ctx.mark_non_differentiable(experts, chosen)
+        ctx.set_materialize_grads(False)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(logits, gates, experts, counts, lse)
+            ctx.normalize = normalize
+        return gates, experts, chosen, loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dgates, _dexperts, _dcounts, dloss):
+        if dgates is None and dloss is None:
+            return None, None, None, None
+        logits, gates, experts, counts, lse = ctx.saved_tensors
+        return _route_bwd(logits, gates, experts, counts, lse, dgates, dloss, ctx.normalize), None, None, None
+
+
+class Router:
+    """Callable with fixed settings: Router(top_k, normalize)(logits, mask=None) -> (gates, experts, counts, loss),
+    see `route`."""
+
+    def __init__(self, top_k, normalize=True):
+        self.top_k, self.normalize = top_k, normalize
+        self.route_fn = route.apply
+
+    def __call__(self, logits, mask=None):
+        return self.route_fn(logits, self.top_k, self.normalize, mask)

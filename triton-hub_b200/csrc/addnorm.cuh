@@ -1,0 +1,731 @@
+// Residual addition + RMSNorm, forward and backward, and RMSNorm (with or without the residual
+// addition) with an 8-bit output and scales.
+//
+//   forward    h = round_R(x + r);  rstd = 1 / sqrt(sum(h^2)/N + eps);  y = h * rstd * w
+//   backward   xhat = h * rstd;  wdy = w * dy;  c1 = sum(xhat * wdy) / N
+//              d = (wdy - xhat * c1) * rstd + dh;  dx = round_T(d), dr = round_R(d);  dw = sum_rows(dy * xhat)
+//   8 bits     a_g = max |y| over a group of columns;  s_g = max(a_g, 2^-64) / 448 (or the next power of two
+//              up);  q = e4m3(y / s_g), from the unrounded y
+//
+// T is the storage type of x, y, dy and dx; R that of the residual stream (r, h, dh, dr): T or fp32.  h is
+// rounded to R before the statistics are taken, so that y is the norm of the h that is returned and that
+// the backward reads; everything else stays fp32 until its one rounding on store.
+//
+// All of it is bound by memory: the forward reads x, r and writes h, y, the backward reads h, dy, dh and
+// writes one gradient (two when R is not T), so the aim is only to touch each byte once and to keep
+// enough of them in flight.  A row lives in the registers of TPR threads, LD 16-byte packets each.
+#pragma once
+
+#include "norm_common.cuh"
+#include "norm_stage.cuh"
+
+namespace b200norm {
+
+struct AddNormParams {
+  // forward: x, r (null without a residual), w -> y (or q), h, rstd, scale
+  // backward: h, dy (as x), dh (as r; null for none), w, rstd -> dx (as y), dr, part
+  const void* x;
+  const void* r;
+  const void* w;  // may be null
+  void* y;
+  void* h;      // forward: may be null in the 8-bit form
+  float* rstd;  // forward: may be null in the 8-bit form
+  void* scale;  // 8-bit form
+  float* part;  // backward: (gridDim.x, N) partial rows of dw, or null
+  void* dr;     // backward: the gradient in R, null when R is T (it is dx then)
+  int64_t x_stride, r_stride, y_stride, h_stride, dr_stride;  // elements
+  int64_t M;
+  int N;
+  int w_dtype;
+  float eps;
+  int group;  // 8-bit form: columns per scale, 0 for one scale a row
+  int groups_per_row;
+  int e8m0;  // 8-bit form: scales are powers of two, stored as their biased exponent
+};
+
+constexpr float kE4m3Max = 448.f;
+constexpr float kAmaxFloor = 5.421010862427522e-20f;  // 2^-64: a group of zeros still gets a finite scale
+
+// VEC consecutive elements of E as raw registers.  The streams are read once, hence past L1.
+template <typename E, int VEC>
+struct RawVec {
+  static constexpr int kWords = VEC * static_cast<int>(sizeof(E)) / 4;
+  static_assert(kWords == 4 || kWords == 8, "16 or 32 bytes");
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void load(const E* p) {
+    if constexpr (kWords == 4) {
+      const uint4 v = ld_stream(reinterpret_cast<const uint4*>(p));
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
+      asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                   : "l"(p));
+    }
+  }
+  __device__ __forceinline__ void store(E* p) const {
+    if constexpr (kWords == 4) {
+      st_stream(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
+    } else {
+      asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                   "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                   : "memory");
+    }
+  }
+  // Columns c0 .. c0 + VEC - 1 of a row of n, some of them outside it: element by element.
+  __device__ __forceinline__ void load_part(const E* row, int c0, int n) {
+    E v[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      v[e] = from_f32<E>(0.f);
+      if (c0 + e >= 0 && c0 + e < n) v[e] = row[c0 + e];
+    }
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(E) == 4) w[i] = reinterpret_cast<const uint32_t&>(v[i]);
+      else
+        w[i] = static_cast<uint32_t>(reinterpret_cast<const uint16_t&>(v[2 * i])) |
+               (static_cast<uint32_t>(reinterpret_cast<const uint16_t&>(v[2 * i + 1])) << 16);
+    }
+  }
+  __device__ __forceinline__ void store_part(E* row, int c0, int n) const {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      if (c0 + e < 0 || c0 + e >= n) continue;
+      if constexpr (sizeof(E) == 4) {
+        row[c0 + e] = __uint_as_float(w[e]);
+      } else {
+        const uint16_t b = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+        row[c0 + e] = reinterpret_cast<const E&>(b);
+      }
+    }
+  }
+  __device__ __forceinline__ void unpack(float2* f) const {
+    if constexpr (sizeof(E) == 4) {
+#pragma unroll
+      for (int i = 0; i < kWords / 2; ++i) f[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    } else {
+      Pack16<E>::unpack2(make_uint4(w[0], w[1], w[2], w[3]), f);
+    }
+  }
+  __device__ __forceinline__ void pack(const float2* f) {
+    if constexpr (sizeof(E) == 4) {
+#pragma unroll
+      for (int i = 0; i < kWords / 2; ++i) {
+        w[2 * i] = __float_as_uint(f[i].x);
+        w[2 * i + 1] = __float_as_uint(f[i].y);
+      }
+    } else {
+      const uint4 v = Pack16<E>::pack2(f);
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    }
+  }
+};
+
+// VEC parameter values from column c0; ALIGNED: c0 is a multiple of VEC and the vector's base 16-byte
+// aligned.  The parameters are re-read by every row a CTA handles: L1 serves them.
+template <int VEC, bool ALIGNED>
+__device__ __forceinline__ void load_w(const void* p, int dtype, int c0, int n, float2* f) {
+  float v[VEC];
+  if (p == nullptr) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = 1.f;
+  } else if (ALIGNED && dtype == kF32) {
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      const float4 q = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c0) + i);
+      v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+    }
+  } else if (ALIGNED && (dtype == kF16 || dtype == kBF16)) {
+    uint32_t q[VEC / 2];
+    const uint16_t* src = static_cast<const uint16_t*>(p) + c0;
+    if constexpr (VEC == 8) {
+      const uint4 t = __ldg(reinterpret_cast<const uint4*>(src));
+      q[0] = t.x; q[1] = t.y; q[2] = t.z; q[3] = t.w;
+    } else {
+      const uint2 t = __ldg(reinterpret_cast<const uint2*>(src));
+      q[0] = t.x; q[1] = t.y;
+    }
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      if (dtype == kBF16) {
+        v[2 * i] = __uint_as_float(q[i] << 16);
+        v[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
+      } else {
+        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&q[i]));
+        v[2 * i] = h.x;
+        v[2 * i + 1] = h.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = (c0 + e >= 0 && c0 + e < n) ? load_param(p, dtype, c0 + e) : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i) f[i] = make_float2(v[2 * i], v[2 * i + 1]);
+}
+
+// Maximum that keeps a NaN, so that a poisoned group shows in its scale.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// The scale of a group whose largest magnitude is `amax`, and the byte a power-of-two scale is stored as.
+__device__ __forceinline__ float fp8_scale(float amax, bool e8m0, uint8_t* code) {
+  float s = max_nan(amax, kAmaxFloor) / kE4m3Max;
+  if (e8m0) {
+    // the next power of two: the exponent field, one more where the fraction is not zero
+    const uint32_t bits = __float_as_uint(s);
+    const uint32_t e = (s != s) ? 255u : (bits + 0x7fffffu) >> 23;
+    *code = static_cast<uint8_t>(e);
+    s = __uint_as_float(e == 255u ? 0x7fffffffu : e << 23);
+  }
+  return s;
+}
+
+__device__ __forceinline__ uint32_t fp8x2(float lo, float hi) {  // saturating, NaN stays NaN
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+__host__ __device__ constexpr int addnorm_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
+
+// Whether a backward thread's LD * VEC dweight sums go to shared memory: they would not fit in the
+// registers beside the row.
+__host__ __device__ constexpr bool addnorm_wide(int ld, int vec, int tpr) { return ld * vec > 24 || tpr > 512; }
+
+// Sum over the TPR threads that share a row.
+template <int TPR, int FIRST>
+__device__ __forceinline__ float row_sum(float v, float* scratch, int& phase, int group, int warp_n, int lane) {
+  if constexpr (TPR <= 32) {
+#pragma unroll
+    for (int o = TPR / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  } else {
+    float s[1] = {v};
+    group_sum<TPR / 32, 1, FIRST>(s, scratch, phase, group, warp_n, lane);
+    return s[0];
+  }
+}
+
+// Forward.  OFF: the rows of all buffers start at one common offset within a packet that need not be
+// zero (contiguous tensors of an odd row length); packets are then laid on the buffers' own alignment,
+// the first and the last of a row are partial, and the launch gives every row group rows of one offset
+// only (row_step is a multiple of the offsets' period), so that a thread's columns stay the same.
+// FP8: the 8-bit form.  Thread t of a row group holds packets t, t + TPR, ...: neighbouring lanes hold
+// neighbouring columns, so a scale's 32, 64 or 128 columns are 4 to 32 adjacent lanes of one warp.
+template <typename T, typename R, int LD, int TPR, bool OFF, bool FP8>
+__global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_fwd_kernel(const AddNormParams p) {
+  static_assert(!(OFF && FP8), "scale groups lie on packet boundaries");
+  constexpr int VEC = Pack16<T>::kElems, H = VEC / 2;
+  constexpr int GROUPS = addnorm_threads(TPR) / TPR;
+  constexpr int WARPS_N = TPR >= 32 ? TPR / 32 : 1;
+  constexpr bool WREG = LD * VEC <= 16;  // the weights fit in registers next to the row
+  __shared__ float scratch[GROUPS][2 * WARPS_N];
+  __shared__ float max_scratch[FP8 ? GROUPS : 1][2 * WARPS_N];
+
+  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  const int lane = threadIdx.x & 31, warp_n = TPR >= 32 ? t / 32 : 0;
+  int phase = 0, max_phase = 0;
+  grid_dependency_sync();
+  trigger_dependents();
+
+  const int64_t first = (int64_t)blockIdx.x * GROUPS + group;
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  const int off = OFF ? static_cast<int>((reinterpret_cast<uintptr_t>(p.x) / sizeof(T) + first * p.x_stride) % VEC) : 0;
+  const int packets = (off + p.N + VEC - 1) / VEC;
+  const float inv_n = 1.f / static_cast<float>(p.N);
+
+  float2 wr[WREG ? LD : 1][H];
+  if constexpr (WREG) {
+#pragma unroll
+    for (int j = 0; j < LD; ++j) {
+      const int pk = j * TPR + t;
+      if (pk < packets) load_w<VEC, !OFF>(p.w, p.w_dtype, pk * VEC - off, p.N, wr[j]);
+    }
+  }
+
+  // Rows of fewer than 32 threads share a warp: the loop runs while the warp's first row is a row.
+  const int64_t lead = TPR < 32 ? (int64_t)blockIdx.x * GROUPS + (threadIdx.x & ~31) / TPR : first;
+  for (int64_t i = 0; lead + i < p.M; i += step) {
+    const int64_t row = first + i;
+    const bool valid = TPR >= 32 || row < p.M;
+    const T* xrow = static_cast<const T*>(p.x) + row * p.x_stride;
+    const R* rrow = static_cast<const R*>(p.r) + row * p.r_stride;
+    R* hrow = static_cast<R*>(p.h) + row * p.h_stride;
+
+    float2 hf[LD][H];
+    {
+      RawVec<T, VEC> xv[LD];
+      RawVec<R, VEC> rv[LD];
+#pragma unroll
+      for (int j = 0; j < LD; ++j) {
+        const int pk = j * TPR + t, c0 = pk * VEC - off;
+        xv[j].zero();
+        rv[j].zero();
+        if (!valid || pk >= packets) continue;
+        if (!OFF || (c0 >= 0 && c0 + VEC <= p.N)) {
+          xv[j].load(xrow + c0);
+          if (p.r != nullptr) rv[j].load(rrow + c0);
+        } else {
+          xv[j].load_part(xrow, c0, p.N);
+          if (p.r != nullptr) rv[j].load_part(rrow, c0, p.N);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < LD; ++j) {
+        const int pk = j * TPR + t, c0 = pk * VEC - off;
+        xv[j].unpack(hf[j]);
+        if (p.r != nullptr) {
+          float2 rf[H];
+          rv[j].unpack(rf);
+#pragma unroll
+          for (int k = 0; k < H; ++k) hf[j][k] = add2(hf[j][k], rf[k]);
+          rv[j].pack(hf[j]);
+          if (sizeof(R) < 4) rv[j].unpack(hf[j]);  // the norm is that of h as stored
+        } else if constexpr (sizeof(R) == sizeof(T)) {
+#pragma unroll
+          for (int k = 0; k < RawVec<R, VEC>::kWords; ++k) rv[j].w[k] = xv[j].w[k];
+        }
+        if (p.h != nullptr && valid && pk < packets) {
+          if (!OFF || (c0 >= 0 && c0 + VEC <= p.N)) rv[j].store(hrow + c0);
+          else rv[j].store_part(hrow, c0, p.N);
+        }
+      }
+    }
+
+    float2 q2 = splat2(0.f);
+#pragma unroll
+    for (int j = 0; j < LD; ++j)
+#pragma unroll
+      for (int k = 0; k < H; ++k) q2 = fma2(hf[j][k], hf[j][k], q2);
+    const float q = row_sum<TPR, 0>(q2.x + q2.y, scratch[group], phase, group, warp_n, lane);
+    const float rstd = 1.f / sqrtf(q * inv_n + p.eps);
+    if (t == 0 && valid && p.rstd != nullptr) p.rstd[row] = rstd;
+    const float2 r2 = splat2(rstd);
+
+    float amax = 0.f;  // FP8, one scale a row
+    float amax_j[FP8 ? LD : 1];
+#pragma unroll
+    for (int j = 0; j < LD; ++j) {
+      const int pk = j * TPR + t, c0 = pk * VEC - off;
+      float2 wf[H];
+      if constexpr (WREG) {
+#pragma unroll
+        for (int k = 0; k < H; ++k) wf[k] = wr[j][k];
+      } else if (pk < packets) {
+        load_w<VEC, !OFF>(p.w, p.w_dtype, c0, p.N, wf);
+      }
+      if constexpr (!FP8) {
+        if (valid && pk < packets) {
+#pragma unroll
+          for (int k = 0; k < H; ++k) hf[j][k] = mul2(mul2(hf[j][k], r2), wf[k]);
+          T* yrow = static_cast<T*>(p.y) + row * p.y_stride;
+          RawVec<T, VEC> o;
+          o.pack(hf[j]);
+          if (!OFF || (c0 >= 0 && c0 + VEC <= p.N)) o.store(yrow + c0);
+          else o.store_part(yrow, c0, p.N);
+        }
+      } else {
+        float a = 0.f;
+        if (pk < packets) {
+#pragma unroll
+          for (int k = 0; k < H; ++k) {
+            hf[j][k] = mul2(mul2(hf[j][k], r2), wf[k]);
+            a = max_nan(a, max_nan(fabsf(hf[j][k].x), fabsf(hf[j][k].y)));
+          }
+        }
+        amax_j[j] = a;
+        amax = max_nan(amax, a);
+      }
+    }
+
+    if constexpr (FP8) {
+      uint8_t* qrow = static_cast<uint8_t*>(p.y) + row * p.y_stride;
+      float scale = 0.f, inv = 0.f;
+      uint8_t code = 0;
+      const int lanes = p.group == 0 ? (TPR < 32 ? TPR : 32) : min(p.group / VEC, TPR);  // adjacent lanes to merge
+      if (p.group == 0) {
+#pragma unroll
+        for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if constexpr (TPR > 32) {
+          float* buf = max_scratch[group] + max_phase * WARPS_N;
+          if (lane == 0) buf[warp_n] = amax;
+          group_sync<WARPS_N, 0>(group);
+#pragma unroll
+          for (int k = 0; k < WARPS_N; ++k) amax = max_nan(amax, buf[k]);
+          max_phase ^= 1;
+        }
+        scale = fp8_scale(amax, p.e8m0 != 0, &code);
+        inv = 1.f / scale;
+        if (t == 0 && valid) {
+          if (p.e8m0) static_cast<uint8_t*>(p.scale)[row] = code;
+          else static_cast<float*>(p.scale)[row] = scale;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < LD; ++j) {
+        const int pk = j * TPR + t;
+        if (p.group != 0) {
+          float a = amax_j[j];
+          for (int o = 1; o < lanes; o <<= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+          scale = fp8_scale(a, p.e8m0 != 0, &code);
+          inv = 1.f / scale;
+          if (valid && pk < packets && (t & (lanes - 1)) == 0) {
+            const int64_t at = row * p.groups_per_row + pk * VEC / p.group;
+            if (p.e8m0) static_cast<uint8_t*>(p.scale)[at] = code;
+            else static_cast<float*>(p.scale)[at] = scale;
+          }
+        }
+        if (valid && pk < packets) {
+          uint32_t word[VEC / 4];
+#pragma unroll
+          for (int k = 0; k < VEC / 4; ++k) {
+            const float2 lo = hf[j][2 * k], hi = hf[j][2 * k + 1];
+            word[k] = fp8x2(lo.x * inv, lo.y * inv) | (fp8x2(hi.x * inv, hi.y * inv) << 16);
+          }
+          if constexpr (VEC == 8) __stcs(reinterpret_cast<uint2*>(qrow + pk * VEC), make_uint2(word[0], word[1]));
+          else __stcs(reinterpret_cast<uint32_t*>(qrow + pk * VEC), word[0]);
+        }
+      }
+    }
+  }
+}
+
+// Backward.  A thread owns fixed columns of every row its group visits and carries their dweight sums:
+// in registers, or (WIDE: more than 16 of them) in shared memory, laid out so that lane t touches word t.
+// The row groups of a CTA are added in order at the end: one partial row per CTA.
+template <typename T, typename R, int LD, int TPR, bool OFF>
+__global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_bwd_kernel(const AddNormParams p) {
+  constexpr int VEC = Pack16<T>::kElems, H = VEC / 2;
+  constexpr int GROUPS = addnorm_threads(TPR) / TPR;
+  constexpr int WARPS_N = TPR >= 32 ? TPR / 32 : 1;
+  constexpr bool WREG = LD * VEC <= 16;
+  constexpr bool WIDE = addnorm_wide(LD, VEC, TPR);
+  extern __shared__ __align__(16) float acc[];  // WIDE: [LD * VEC][TPR]; GROUPS > 1: [GROUPS][N]
+  __shared__ float scratch[GROUPS][2 * WARPS_N];
+
+  const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  const int lane = threadIdx.x & 31, warp_n = TPR >= 32 ? t / 32 : 0;
+  int phase = 0;
+  grid_dependency_sync();
+  trigger_dependents();
+
+  const int64_t first = (int64_t)blockIdx.x * GROUPS + group;
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  const int off = OFF ? static_cast<int>((reinterpret_cast<uintptr_t>(p.x) / sizeof(T) + first * p.x_stride) % VEC) : 0;
+  const int packets = (off + p.N + VEC - 1) / VEC;
+  const float inv_n = 1.f / static_cast<float>(p.N);
+
+  float2 wr[WREG ? LD : 1][H];
+  float2 dw[WIDE ? 1 : LD][H];
+  if constexpr (WREG) {
+#pragma unroll
+    for (int j = 0; j < LD; ++j) {
+      const int pk = j * TPR + t;
+      if (pk < packets) load_w<VEC, !OFF>(p.w, p.w_dtype, pk * VEC - off, p.N, wr[j]);
+    }
+  }
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int k = 0; k < LD * VEC; ++k) acc[k * TPR + t] = 0.f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < LD; ++j)
+#pragma unroll
+      for (int k = 0; k < H; ++k) dw[j][k] = splat2(0.f);
+  }
+
+  const int64_t lead = TPR < 32 ? (int64_t)blockIdx.x * GROUPS + (threadIdx.x & ~31) / TPR : first;
+  for (int64_t i = 0; lead + i < p.M; i += step) {
+    const int64_t row = first + i;
+    const bool valid = TPR >= 32 || row < p.M;
+    const T* grow = static_cast<const T*>(p.x) + row * p.x_stride;  // dy
+    const R* hrow = static_cast<const R*>(p.h) + row * p.h_stride;
+    const R* drow = static_cast<const R*>(p.r) + row * p.r_stride;  // dh
+    const float rs = valid ? __ldg(p.rstd + row) : 0.f;
+
+    RawVec<T, VEC> gv[LD];
+    RawVec<R, VEC> hv[LD], dv[LD];
+#pragma unroll
+    for (int j = 0; j < LD; ++j) {
+      const int pk = j * TPR + t, c0 = pk * VEC - off;
+      gv[j].zero();
+      hv[j].zero();
+      dv[j].zero();
+      if (!valid || pk >= packets) continue;
+      if (!OFF || (c0 >= 0 && c0 + VEC <= p.N)) {
+        gv[j].load(grow + c0);
+        hv[j].load(hrow + c0);
+        if (p.r != nullptr) dv[j].load(drow + c0);
+      } else {
+        gv[j].load_part(grow, c0, p.N);
+        hv[j].load_part(hrow, c0, p.N);
+        if (p.r != nullptr) dv[j].load_part(drow, c0, p.N);
+      }
+    }
+    float2 s2 = splat2(0.f);
+    const float2 rs2 = splat2(rs);
+#pragma unroll
+    for (int j = 0; j < LD; ++j) {
+      const int pk = j * TPR + t;
+      if (pk >= packets) continue;
+      float2 gf[H], hf[H], wf[H];
+      gv[j].unpack(gf);
+      hv[j].unpack(hf);
+      if constexpr (WREG) {
+#pragma unroll
+        for (int k = 0; k < H; ++k) wf[k] = wr[j][k];
+      } else {
+        load_w<VEC, !OFF>(p.w, p.w_dtype, pk * VEC - off, p.N, wf);
+      }
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        const float2 a = mul2(gf[k], mul2(hf[k], rs2));  // dy * xhat
+        s2 = fma2(wf[k], a, s2);
+        if constexpr (WIDE) {
+          acc[(j * VEC + 2 * k) * TPR + t] += a.x;
+          acc[(j * VEC + 2 * k + 1) * TPR + t] += a.y;
+        } else {
+          dw[j][k] = add2(dw[j][k], a);
+        }
+      }
+    }
+    const float c1 = row_sum<TPR, (GROUPS == 1 ? 0 : 1)>(s2.x + s2.y, scratch[group], phase, group, warp_n, lane) * inv_n;
+    // d = w * dy * rstd - h * (c1 * rstd^2) + dh
+    const float2 kh = splat2(-c1 * rs * rs);
+    T* dxrow = static_cast<T*>(p.y) + row * p.y_stride;
+    R* drrow = static_cast<R*>(p.dr) + row * p.dr_stride;
+#pragma unroll
+    for (int j = 0; j < LD; ++j) {
+      const int pk = j * TPR + t, c0 = pk * VEC - off;
+      if (!valid || pk >= packets) continue;
+      float2 gf[H], hf[H], wf[H], df[H];
+      gv[j].unpack(gf);
+      hv[j].unpack(hf);
+      dv[j].unpack(df);
+      if constexpr (WREG) {
+#pragma unroll
+        for (int k = 0; k < H; ++k) wf[k] = wr[j][k];
+      } else {
+        load_w<VEC, !OFF>(p.w, p.w_dtype, c0, p.N, wf);
+      }
+#pragma unroll
+      for (int k = 0; k < H; ++k) df[k] = fma2(mul2(wf[k], rs2), gf[k], fma2(hf[k], kh, df[k]));
+      const bool full = !OFF || (c0 >= 0 && c0 + VEC <= p.N);
+      RawVec<T, VEC> o;
+      o.pack(df);
+      if (full) o.store(dxrow + c0);
+      else o.store_part(dxrow, c0, p.N);
+      if constexpr (sizeof(R) != sizeof(T)) {
+        RawVec<R, VEC> od;
+        od.pack(df);
+        if (full) od.store(drrow + c0);
+        else od.store_part(drrow, c0, p.N);
+      }
+    }
+  }
+
+  if (p.part == nullptr) return;
+  float* out = p.part + (size_t)blockIdx.x * p.N;
+  if constexpr (GROUPS > 1) {
+    static_assert(GROUPS == 1 || !WIDE, "several row groups keep their sums in registers");
+    float* mine = acc + (size_t)group * p.N;
+#pragma unroll
+    for (int j = 0; j < LD; ++j) {
+      const int pk = j * TPR + t, c0 = pk * VEC - off;
+      if (pk >= packets) continue;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (c0 + k >= 0 && c0 + k < p.N) mine[c0 + k] = (k & 1) ? dw[j][k / 2].y : dw[j][k / 2].x;
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.N; c += GROUPS * TPR) {
+      float s = 0.f;
+      for (int g = 0; g < GROUPS; ++g) s += acc[(size_t)g * p.N + c];
+      out[c] = s;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < LD; ++j) {
+      const int pk = j * TPR + t, c0 = pk * VEC - off;
+      if (pk >= packets) continue;
+      float2 a[H];
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        if constexpr (WIDE) a[k] = make_float2(acc[(j * VEC + 2 * k) * TPR + t], acc[(j * VEC + 2 * k + 1) * TPR + t]);
+        else a[k] = dw[j][k];
+      }
+      if constexpr (!OFF) {
+        st_f32_pairs<H>(out + c0, a);
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          if (c0 + k >= 0 && c0 + k < p.N) out[c0 + k] = (k & 1) ? a[k / 2].y : a[k / 2].x;
+      }
+    }
+  }
+}
+
+// Buffers whose rows are aligned differently (views, odd strides): one CTA per row, element by element,
+// the row kept in shared memory as fp32 between the two passes.  In the 8-bit form a warp takes a scale's
+// columns at a time.
+template <typename T, typename R, bool FP8>
+__global__ void __launch_bounds__(512) addnorm_fwd_any_kernel(const AddNormParams p) {
+  extern __shared__ float hs[];  // [N]
+  __shared__ float scratch[2 * 16];
+  __shared__ float max_scratch[16];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int phase = 0;
+  grid_dependency_sync();
+  trigger_dependents();
+  for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
+    const T* xrow = static_cast<const T*>(p.x) + row * p.x_stride;
+    const R* rrow = static_cast<const R*>(p.r) + row * p.r_stride;
+    R* hrow = static_cast<R*>(p.h) + row * p.h_stride;
+    float q = 0.f;
+#pragma unroll 4
+    for (int c = threadIdx.x; c < p.N; c += 512) {
+      float v = to_f32(xrow[c]);
+      if (p.r != nullptr) v = to_f32(from_f32<R>(v + to_f32(rrow[c])));
+      if (p.h != nullptr) hrow[c] = from_f32<R>(v);
+      hs[c] = v;
+      q = fmaf(v, v, q);
+    }
+    float s[1] = {q};
+    group_sum<16, 1, 0>(s, scratch, phase, 0, warp, lane);  // a barrier: the row is in shared memory after it
+    const float rstd = 1.f / sqrtf(s[0] / static_cast<float>(p.N) + p.eps);
+    if (threadIdx.x == 0 && p.rstd != nullptr) p.rstd[row] = rstd;
+    if constexpr (!FP8) {
+      T* yrow = static_cast<T*>(p.y) + row * p.y_stride;
+      for (int c = threadIdx.x; c < p.N; c += 512) {
+        const float w = p.w != nullptr ? load_param(p.w, p.w_dtype, c) : 1.f;
+        yrow[c] = from_f32<T>(hs[c] * rstd * w);
+      }
+    } else {
+      uint8_t* qrow = static_cast<uint8_t*>(p.y) + row * p.y_stride;
+      const bool whole = p.group == 0;
+      float amax = 0.f;
+      for (int c = threadIdx.x; c < p.N; c += 512) {
+        const float w = p.w != nullptr ? load_param(p.w, p.w_dtype, c) : 1.f;
+        const float v = hs[c] * rstd * w;
+        hs[c] = v;
+        amax = max_nan(amax, fabsf(v));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (lane == 0) max_scratch[warp] = amax;
+      __syncthreads();
+      if (whole) {
+        for (int k = 0; k < 16; ++k) amax = max_nan(amax, max_scratch[k]);
+        uint8_t code = 0;
+        const float scale = fp8_scale(amax, p.e8m0 != 0, &code), inv = 1.f / scale;
+        if (threadIdx.x == 0) {
+          if (p.e8m0) static_cast<uint8_t*>(p.scale)[row] = code;
+          else static_cast<float*>(p.scale)[row] = scale;
+        }
+        for (int c = threadIdx.x; c < p.N; c += 512) qrow[c] = static_cast<uint8_t>(fp8x2(hs[c] * inv, 0.f));
+      } else {
+        for (int g = warp; g < p.groups_per_row; g += 16) {
+          const int c0 = g * p.group;
+          float v[4], a = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int c = c0 + k * 32 + lane;
+            v[k] = (k * 32 < p.group && c < p.N) ? hs[c] : 0.f;
+            a = max_nan(a, fabsf(v[k]));
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+          uint8_t code = 0;
+          const float scale = fp8_scale(a, p.e8m0 != 0, &code), inv = 1.f / scale;
+          if (lane == 0) {
+            const int64_t at = row * p.groups_per_row + g;
+            if (p.e8m0) static_cast<uint8_t*>(p.scale)[at] = code;
+            else static_cast<float*>(p.scale)[at] = scale;
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int c = c0 + k * 32 + lane;
+            if (k * 32 < p.group && c < p.N) qrow[c] = static_cast<uint8_t>(fp8x2(v[k] * inv, 0.f));
+          }
+        }
+      }
+    }
+    __syncthreads();  // the next row overwrites hs
+  }
+}
+
+template <typename T, typename R>
+__global__ void __launch_bounds__(512) addnorm_bwd_any_kernel(const AddNormParams p) {
+  extern __shared__ float acc[];  // [N]: column c belongs to thread c % 512
+  __shared__ float scratch[2 * 16];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int phase = 0;
+  grid_dependency_sync();
+  trigger_dependents();
+  for (int c = threadIdx.x; c < p.N; c += 512) acc[c] = 0.f;
+  const float inv_n = 1.f / static_cast<float>(p.N);
+  for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) {
+    const T* grow = static_cast<const T*>(p.x) + row * p.x_stride;
+    const R* hrow = static_cast<const R*>(p.h) + row * p.h_stride;
+    const R* drow = static_cast<const R*>(p.r) + row * p.r_stride;
+    T* dxrow = static_cast<T*>(p.y) + row * p.y_stride;
+    R* drrow = static_cast<R*>(p.dr) + row * p.dr_stride;
+    const float rs = p.rstd[row];
+    float s[1] = {0.f};
+#pragma unroll 4
+    for (int c = threadIdx.x; c < p.N; c += 512) {
+      const float w = p.w != nullptr ? load_param(p.w, p.w_dtype, c) : 1.f;
+      const float a = to_f32(grow[c]) * (to_f32(hrow[c]) * rs);
+      acc[c] += a;
+      s[0] = fmaf(w, a, s[0]);
+    }
+    group_sum<16, 1, 0>(s, scratch, phase, 0, warp, lane);
+    const float kh = -s[0] * inv_n * rs * rs;
+#pragma unroll 4
+    for (int c = threadIdx.x; c < p.N; c += 512) {
+      const float w = p.w != nullptr ? load_param(p.w, p.w_dtype, c) : 1.f;
+      const float dh = p.r != nullptr ? to_f32(drow[c]) : 0.f;
+      const float d = fmaf(w * rs, to_f32(grow[c]), fmaf(to_f32(hrow[c]), kh, dh));
+      dxrow[c] = from_f32<T>(d);
+      if constexpr (sizeof(R) != sizeof(T)) drrow[c] = from_f32<R>(d);
+    }
+  }
+  if (p.part == nullptr) return;
+  for (int c = threadIdx.x; c < p.N; c += 512) p.part[(size_t)blockIdx.x * p.N + c] = acc[c];
+}
+
+// ---------------------------------------------------------------------------------------
+// What the launch code needs to know of the compiled kernels, one table per (T, R).
+// ---------------------------------------------------------------------------------------
+struct AddNormShape {
+  int ld, tpr;
+  const void* fwd[2];  // [rows at a common offset]
+  const void* fp8;
+  const void* bwd[2];
+  int capacity() const { return ld * tpr; }  // packets per row
+  int threads() const { return addnorm_threads(tpr); }
+  int groups() const { return threads() / tpr; }
+};
+struct AddNormTable {
+  int size_t_, size_r;  // bytes per element
+  const AddNormShape* shapes;  // ascending capacity
+  int n;
+  const void *fwd_any, *fp8_any, *bwd_any;
+};
+
+const AddNormTable* addnorm_table_f32();
+const AddNormTable* addnorm_table_f16();
+const AddNormTable* addnorm_table_bf16();
+const AddNormTable* addnorm_table_f16_f32();
+const AddNormTable* addnorm_table_bf16_f32();
+
+}  // namespace b200norm

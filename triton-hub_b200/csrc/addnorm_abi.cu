@@ -1,0 +1,201 @@
+// Entry points of the residual + RMSNorm operators: argument checks, launch planning, launches.
+#include <algorithm>
+#include <numeric>
+
+#include "addnorm.cuh"
+#include "host.h"
+
+namespace b200norm {
+namespace {
+
+// How the rows of a call's buffers lie: on packet boundaries, at one common offset from them, or neither.
+enum Layout { kAligned = 0, kOffset = 1, kAny = 2 };
+enum Which { kFwd, kFp8, kBwd };
+
+struct Buffer {
+  const void* p;
+  int64_t stride;
+  int size;  // bytes per element
+};
+
+const AddNormTable* table_for(int io, int res) {
+  if (io == B200NORM_F32 && res == B200NORM_F32) return addnorm_table_f32();
+  if (io == B200NORM_F16 && res == B200NORM_F16) return addnorm_table_f16();
+  if (io == B200NORM_BF16 && res == B200NORM_BF16) return addnorm_table_bf16();
+  if (io == B200NORM_F16 && res == B200NORM_F32) return addnorm_table_f16_f32();
+  if (io == B200NORM_BF16 && res == B200NORM_F32) return addnorm_table_bf16_f32();
+  return nullptr;
+}
+
+int check(int64_t M, int64_t N, int io, int res, int w_dtype) {
+  if (table_for(io, res) == nullptr)
+    return fail(B200NORM_ERR_ARG, "residual + RMSNorm runs on fp32, fp16 and bf16 rows with a residual of the same type or "
+                "fp32 (io code %d, residual code %d)", io, res);
+  if (w_dtype < B200NORM_F32 || w_dtype > B200NORM_F64) return fail(B200NORM_ERR_ARG, "unknown weight dtype code %d", w_dtype);
+  if (M < 0 || N < 1) return fail(B200NORM_ERR_ARG, "bad shape M=%lld N=%lld", (long long)M, (long long)N);
+  if (N * table_for(io, res)->size_t_ > kMaxRowBytes)
+    return fail(B200NORM_ERR_UNSUPPORTED, "This layer norm doesn't support feature dim >= 64KB.");
+  return B200NORM_OK;
+}
+
+// The common layout of the buffers (null ones are skipped) in packets of `vec` elements; *period: after how
+// many rows the offset repeats.
+Layout layout_of(const Buffer* b, int n, int64_t N, int vec, const void* w, int* period) {
+  *period = 1;
+  int64_t phase = -1, stride = -1;
+  for (int i = 0; i < n; ++i) {
+    if (b[i].p == nullptr) continue;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(b[i].p);
+    if (a % b[i].size != 0) return kAny;
+    const int64_t ph = static_cast<int64_t>((a / b[i].size) % vec), st = b[i].stride % vec;
+    if (phase >= 0 && (ph != phase || st != stride)) return kAny;
+    phase = ph;
+    stride = st;
+  }
+  if (phase == 0 && stride == 0 && N % vec == 0 && (reinterpret_cast<uintptr_t>(w) & 15u) == 0) return kAligned;
+  if (stride > 0) *period = static_cast<int>(vec / std::gcd<int64_t>(vec, stride));
+  return kOffset;
+}
+
+struct Plan {
+  const void* fn;
+  int threads, grid;
+  size_t smem;
+};
+
+int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, int period, int64_t M, int64_t N, Plan* out) {
+  const int vec = 16 / t->size_t_;
+  // packets a row can span: up to one more at either end when it starts inside one
+  const int64_t need = layout == kOffset ? (N + 2 * vec - 2) / vec : (N + vec - 1) / vec;
+  const AddNormShape* s = nullptr;
+  if (layout == kAligned || (layout == kOffset && which != kFp8))
+    for (int i = 0; i < t->n && s == nullptr; ++i)
+      if (t->shapes[i].capacity() >= need) s = &t->shapes[i];
+  int groups = 1;
+  if (s == nullptr) {
+    out->fn = which == kFwd ? t->fwd_any : which == kFp8 ? t->fp8_any : t->bwd_any;
+    out->threads = 512;
+    out->smem = static_cast<size_t>(N) * sizeof(float);
+  } else {
+    out->fn = which == kFwd ? s->fwd[layout] : which == kFp8 ? s->fp8 : s->bwd[layout];
+    out->threads = s->threads();
+    groups = s->groups();
+    out->smem = 0;
+    if (which == kBwd) {
+      if (groups > 1) out->smem = static_cast<size_t>(groups) * N * sizeof(float);
+      else if (addnorm_wide(s->ld, vec, s->tpr)) out->smem = static_cast<size_t>(s->ld) * vec * s->tpr * sizeof(float);
+    }
+  }
+  int occ;
+  if (int rc = occupancy(dev, out->fn, out->threads, out->smem, &occ)) return rc;
+  const int64_t want = std::max<int64_t>(1, (M + groups - 1) / groups), resident = (int64_t)dev.sm_count * occ;
+  int64_t grid = std::min(want, resident);
+  // a row group's rows have to share one offset (see the kernels): a step that is a multiple of the period
+  if (s != nullptr && layout == kOffset && grid < want) {
+    const int64_t unit = period / std::gcd<int64_t>(period, groups);
+    grid = std::max<int64_t>(unit, grid / unit * unit);
+  }
+  out->grid = static_cast<int>(grid);
+  return B200NORM_OK;
+}
+
+int forward(bool fp8, const void* x, int64_t xs, const void* r, int64_t rs, const void* w, void* y, int64_t ys, void* scale,
+            void* h, int64_t hs, float* rstd, int64_t M, int64_t N, float eps, int group, int e8m0, int io, int res,
+            int w_dtype, void* stream) {
+  if (int rc = check(M, N, io, res, w_dtype)) return rc;
+  if (group != 0 && group != 32 && group != 64 && group != 128)
+    return fail(B200NORM_ERR_ARG, "a scale covers 32, 64 or 128 columns, or (0) a row; got %d", group);
+  if (M == 0) return B200NORM_OK;
+  if (!x || !y || (fp8 && !scale) || (!fp8 && (!r || !h || !rstd))) return fail(B200NORM_ERR_ARG, "null buffer");
+  if (r == nullptr && h != nullptr) return fail(B200NORM_ERR_ARG, "h is the sum with a residual: there is none");
+  if (xs < N || ys < N || (r && rs < N) || (h && hs < N)) return fail(B200NORM_ERR_ARG, "row stride smaller than N");
+  DeviceState* dev = nullptr;
+  if (int rc = device_caches(&dev)) return rc;
+  const AddNormTable* t = table_for(io, res);
+  const Buffer bufs[4] = {{x, xs, t->size_t_}, {r, rs, t->size_r}, {y, ys, fp8 ? 1 : t->size_t_}, {h, hs, t->size_r}};
+  int period;
+  const Layout layout = layout_of(bufs, 4, N, 16 / t->size_t_, w, &period);
+  Plan pl;
+  if (int rc = plan(*dev, t, fp8 ? kFp8 : kFwd, layout, period, M, N, &pl)) return rc;
+  AddNormParams p = {};
+  p.x = x; p.r = r; p.w = w; p.y = y; p.h = h; p.rstd = rstd; p.scale = scale;
+  p.x_stride = xs; p.r_stride = rs; p.y_stride = ys; p.h_stride = hs;
+  p.M = M; p.N = static_cast<int>(N); p.w_dtype = w_dtype; p.eps = eps;
+  p.group = group; p.groups_per_row = group ? static_cast<int>((N + group - 1) / group) : 1; p.e8m0 = e8m0 != 0;
+  return launch(pl.fn, dim3(pl.grid), dim3(pl.threads), pl.smem, &p, static_cast<cudaStream_t>(stream));
+}
+
+}  // namespace
+}  // namespace b200norm
+
+using namespace b200norm;
+
+extern "C" {
+
+int b200norm_add_rms_fwd(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride, const void* w,
+                         void* y, int64_t y_row_stride, void* h, int64_t h_row_stride, float* rstd, int64_t M, int64_t N,
+                         float eps, int io_dtype, int res_dtype, int w_dtype, void* stream) {
+  return forward(false, x, x_row_stride, residual, residual_row_stride, w, y, y_row_stride, nullptr, h, h_row_stride, rstd, M,
+                 N, eps, 0, 0, io_dtype, res_dtype, w_dtype, stream);
+}
+
+int b200norm_rms_fp8(const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride, const void* w,
+                     void* q, int64_t q_row_stride, void* scale, void* h, int64_t h_row_stride, int64_t M, int64_t N,
+                     float eps, int group, int e8m0, int io_dtype, int res_dtype, int w_dtype, void* stream) {
+  return forward(true, x, x_row_stride, residual, residual_row_stride, w, q, q_row_stride, scale, h, h_row_stride, nullptr, M,
+                 N, eps, group, e8m0, io_dtype, res_dtype, w_dtype, stream);
+}
+
+size_t b200norm_add_rms_bwd_workspace_bytes(int64_t M, int64_t N, int io_dtype, int res_dtype) {
+  if (check(M, N, io_dtype, res_dtype, B200NORM_F32)) return 0;
+  DeviceState* dev = nullptr;
+  if (device_caches(&dev)) return 0;
+  const AddNormTable* t = table_for(io_dtype, res_dtype);
+  int64_t rows = 0;
+  for (Layout layout : {kAligned, kOffset, kAny}) {  // whichever the buffers turn out to have
+    Plan pl;
+    if (plan(*dev, t, kBwd, layout, 1, M, N, &pl)) return 0;
+    rows = std::max<int64_t>(rows, pl.grid);
+  }
+  return (static_cast<size_t>(rows) * N * sizeof(float) + 255) & ~static_cast<size_t>(255);
+}
+
+int b200norm_add_rms_bwd(const void* h, int64_t h_row_stride, const void* dy, int64_t dy_row_stride, const void* dh,
+                         int64_t dh_row_stride, const void* w, const float* rstd, void* dx, int64_t dx_row_stride, void* dres,
+                         int64_t dres_row_stride, void* dw, void* workspace, size_t workspace_bytes, int64_t M, int64_t N,
+                         int io_dtype, int res_dtype, int w_dtype, void* stream_v) {
+  if (int rc = check(M, N, io_dtype, res_dtype, w_dtype)) return rc;
+  if (M == 0 && dw == nullptr) return B200NORM_OK;
+  const bool split = io_dtype != res_dtype;
+  if (M > 0 && (!h || !dy || !rstd || !dx || (split && !dres))) return fail(B200NORM_ERR_ARG, "null h / dy / rstd / dx / dres");
+  if (!split && dres != nullptr)
+    return fail(B200NORM_ERR_ARG, "dres is written only when the residual's type is not that of the rows: it equals dx");
+  if (h_row_stride < N || dy_row_stride < N || dx_row_stride < N || (dh && dh_row_stride < N) || (dres && dres_row_stride < N))
+    return fail(B200NORM_ERR_ARG, "row stride smaller than N");
+  DeviceState* dev = nullptr;
+  if (int rc = device_caches(&dev)) return rc;
+  const AddNormTable* t = table_for(io_dtype, res_dtype);
+  const Buffer bufs[5] = {{dy, dy_row_stride, t->size_t_}, {h, h_row_stride, t->size_r}, {dh, dh_row_stride, t->size_r},
+                          {dx, dx_row_stride, t->size_t_}, {dres, dres_row_stride, t->size_r}};
+  int period;
+  const Layout layout = layout_of(bufs, 5, N, 16 / t->size_t_, w, &period);
+  Plan pl;
+  if (int rc = plan(*dev, t, kBwd, layout, period, M, N, &pl)) return rc;
+  AddNormParams p = {};
+  p.x = dy; p.r = dh; p.w = w; p.y = dx; p.h = const_cast<void*>(h); p.rstd = const_cast<float*>(rstd); p.dr = dres;
+  p.x_stride = dy_row_stride; p.r_stride = dh_row_stride; p.y_stride = dx_row_stride; p.h_stride = h_row_stride;
+  p.dr_stride = dres_row_stride;
+  p.M = M; p.N = static_cast<int>(N); p.w_dtype = w_dtype;
+  if (dw != nullptr) {
+    const size_t need = static_cast<size_t>(pl.grid) * N * sizeof(float);
+    if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u))
+      return fail(B200NORM_ERR_ARG, "workspace needs %zu bytes, 256-byte aligned (got %zu)", need, workspace_bytes);
+    p.part = static_cast<float*>(workspace);
+  }
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  if (int rc = launch(pl.fn, dim3(pl.grid), dim3(pl.threads), pl.smem, &p, stream)) return rc;
+  if (dw == nullptr) return B200NORM_OK;
+  return launch_colreduce(p.part, pl.grid, N, dw, w_dtype, stream);
+}
+
+}  // extern "C"

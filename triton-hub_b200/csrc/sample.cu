@@ -1,0 +1,62 @@
+// Entry point of the token choice (sample.cuh): argument checks, launch planning, launch.
+#include <algorithm>
+
+#include "host.h"
+#include "sample.cuh"
+
+namespace b200norm {
+namespace {
+
+template <typename T>
+const void* sample_fn(int cluster) {
+  switch (cluster) {
+    case 1: return reinterpret_cast<const void*>(&sample_kernel<T, 1>);
+    case 2: return reinterpret_cast<const void*>(&sample_kernel<T, 2>);
+    case 4: return reinterpret_cast<const void*>(&sample_kernel<T, 4>);
+    default: return reinterpret_cast<const void*>(&sample_kernel<T, 8>);
+  }
+}
+
+}  // namespace
+}  // namespace b200norm
+
+using namespace b200norm;
+
+extern "C" int b200norm_sample(const void* logits, int64_t row_stride, const float* uniform, const float* temperature_v,
+                               float temperature, const int* top_k_v, int top_k, const float* top_p_v, float top_p,
+                               const float* min_p_v, float min_p, int64_t* tokens, int64_t M, int64_t V, int dtype,
+                               void* stream) {
+  if (dtype != B200NORM_F32 && dtype != B200NORM_F16 && dtype != B200NORM_BF16)
+    return fail(B200NORM_ERR_ARG, "logits are fp32, fp16 or bf16 (dtype code %d)", dtype);
+  if (M < 0 || V < 1) return fail(B200NORM_ERR_ARG, "bad shape M=%lld V=%lld", (long long)M, (long long)V);
+  if (V > kSampleMaxVocab)
+    return fail(B200NORM_ERR_UNSUPPORTED, "a vocabulary of up to %d tokens, got %lld", kSampleMaxVocab, (long long)V);
+  if (M == 0) return B200NORM_OK;
+  if (M > INT32_MAX / kSampleMaxCluster) return fail(B200NORM_ERR_ARG, "too many rows: %lld", (long long)M);
+  if (!logits || !uniform || !tokens) return fail(B200NORM_ERR_ARG, "null logits / uniform / tokens");
+  if (row_stride < V) return fail(B200NORM_ERR_ARG, "row stride smaller than the vocabulary");
+  DeviceState* dev = nullptr;
+  if (int rc = device_caches(&dev)) return rc;
+  const int es = dtype == B200NORM_F32 ? 4 : 2, vec = 16 / es;
+  // CTAs per row: parts of at most 64 KB, so that two or three CTAs share an SM and one's barriers hide behind
+  // another's arithmetic; and with few rows as many as there are SMs, while a part keeps 4096 tokens.
+  int cluster = 1;
+  while (cluster < kSampleMaxCluster && V * es > (int64_t)cluster * 65536) cluster *= 2;
+  while (cluster < kSampleMaxCluster && M * cluster * 2 <= dev->sm_count && V >= (int64_t)cluster * 2 * 4096) cluster *= 2;
+  SampleParams p = {};
+  p.logits = logits; p.stride = row_stride; p.uniform = uniform;
+  p.temperature_v = temperature_v; p.temperature = temperature;
+  p.top_k_v = top_k_v; p.top_k = top_k;
+  p.top_p_v = top_p_v; p.top_p = top_p;
+  p.min_p_v = min_p_v; p.min_p = min_p;
+  p.tokens = tokens; p.M = M; p.V = static_cast<int>(V);
+  const int64_t per = (V + cluster - 1) / cluster;
+  p.chunk = static_cast<int>((per + vec - 1) / vec * vec);
+  const size_t smem = static_cast<size_t>(p.chunk) * es;
+  const void* fn = dtype == B200NORM_F32 ? sample_fn<float>(cluster)
+                   : dtype == B200NORM_F16 ? sample_fn<__half>(cluster) : sample_fn<__nv_bfloat16>(cluster);
+  int occ;  // also raises the kernel's shared-memory allowance
+  if (int rc = occupancy(*dev, fn, kSampleThreads, smem, &occ, cluster)) return rc;
+  return launch(fn, dim3(static_cast<unsigned>(M * cluster)), dim3(kSampleThreads), smem, &p,
+                static_cast<cudaStream_t>(stream), true, cluster);
+}
