@@ -314,7 +314,8 @@ B200NORM_API int b200norm_finalize_pushed(const b200norm_peers* peers, uint64_t 
  *
  * b200norm_add_rms_fwd: h = x + residual rounded to the residual's type, rstd = 1/sqrt(sum(h^2)/N + eps),
  *   y = h*rstd [*w].  x and y are io_dtype, residual and h res_dtype: the same type, or B200NORM_F32
- *   (io_dtype F32, F16 or BF16).  w may be NULL.  rstd is an (M,) fp32 output saved for backward.
+ *   (io_dtype F32, F16 or BF16).  w may be NULL.  rstd is an (M,) fp32 output saved for backward (NULL: not
+ *   wanted).
  * b200norm_add_rms_bwd: with xhat = h*rstd, wdy = w*dy, c1 = sum(xhat*wdy)/N:
  *   d = (wdy - xhat*c1)*rstd + dh;  dx = d in io_dtype, dres = d in res_dtype;  dw = sum_rows(dy*xhat).
  *   dh (the gradient of h) and dw may be NULL.  dres is written when res_dtype is not io_dtype; it must be
@@ -372,7 +373,8 @@ B200NORM_API int b200norm_sample(const void* logits, int64_t row_stride, const f
  * lse (T,), needed for backward only (else NULL): log-sum-exp of the logits, -inf for tokens not live.
  * b200norm_route_bwd: gradients dgates (T, k) and dloss (one fp32 value on the device), either NULL, to dlogits (T, E)
  *   contiguous; counts are taken as constants.
- * workspace: at least b200norm_route_workspace_bytes bytes, 16-byte aligned.
+ * workspace: at least b200norm_route_workspace_bytes bytes, 16-byte aligned; where that is 1 none is needed, and
+ *   workspace may be NULL.
  */
 B200NORM_API size_t b200norm_route_workspace_bytes(int64_t T, int E, int k, int io_dtype);
 B200NORM_API int b200norm_route_fwd(const void* logits, int64_t row_stride, const uint8_t* mask, float* gates,

@@ -14,13 +14,13 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import functional as Fn
-from .functional import _code, _on_device, _params, _ptr, _raw_stream, _require_cuda, _row_stride, _rows
+from .functional import _code, _flat, _on_device, _params, _ptr, _raw_stream, _require_cuda
 
 _ADD_WS = {}  # (device, M, N, dtype codes) -> workspace bytes; the answer never changes
 
 
-def _residual_rows(x, residual):
-    """`residual` as rows, checked against x (its rows' shape, device and type)."""
+def _check_residual(x, residual):
+    """`residual` goes with x: the same shape and device, a type that is taken."""
     if residual.shape != x.shape:
         raise RuntimeError(f"b200norm: residual of shape {tuple(residual.shape)}, input of shape {tuple(x.shape)}")
     if residual.device != x.device:
@@ -28,27 +28,30 @@ def _residual_rows(x, residual):
     if x.dtype == torch.float64 or residual.dtype not in (x.dtype, torch.float32):
         raise RuntimeError(f"b200norm: input of dtype {x.dtype} with a residual of dtype {residual.dtype}; it takes float32, "
                            "float16 and bfloat16 with a residual of the same dtype or float32")
-    return _rows(residual)
 
 
-def _add_rmsnorm_fwd(x, residual, weight, eps):
-    """Returns (y shaped and typed like x, h typed like residual, rstd (M,) fp32)."""
+def _like(t, rows):
+    """An uninitialised contiguous tensor shaped like t; `rows` is what _flat made of t."""
+    return torch.empty_like(t) if rows is t else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _add_rmsnorm_fwd(x, residual, weight, eps, *, need_rstd=True):
+    """Returns (y shaped and typed like x, h typed like residual, rstd (M,) fp32 or None)."""
     _require_cuda(x)
-    shape, N = x.shape, x.shape[-1]
+    _check_residual(x, residual)
+    device = x.device
+    xr, M, N, xs = _flat(x)
+    r, _, _, rs = _flat(residual)
     Fn._check_dim(x, N)
-    r = _residual_rows(x, residual)
-    x = _rows(x)
-    M = x.shape[0]
-    weight, _, wcode = _params(weight, None, N, x.device)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(shape, dtype=r.dtype, device=x.device)
-    rstd = torch.empty((M,), dtype=torch.float32, device=x.device)
+    weight, _, wcode = _params(weight, None, N, device)
+    y, h = _like(x, xr), _like(residual, r)
+    rstd = torch.empty((M,), dtype=torch.float32, device=device) if need_rstd else None
     lib = _lib.load()
-    with _on_device(x.device.index):
+    index = device.index
+    with _on_device(index):
         _lib.check(lib.b200norm_add_rms_fwd(
-            x.data_ptr(), _row_stride(x), r.data_ptr(), _row_stride(r), _ptr(weight), y.data_ptr(), N, h.data_ptr(), N,
-            rstd.data_ptr(), M, N, float(eps), _code(x, "input"), _code(r, "residual"), wcode,
-            _raw_stream(x.device.index)))
+            xr.data_ptr(), xs, r.data_ptr(), rs, _ptr(weight), y.data_ptr(), N, h.data_ptr(), N, _ptr(rstd), M, N, eps,
+            _code(x, "input"), _code(r, "residual"), wcode, _raw_stream(index)))
     return y, h, rstd
 
 
@@ -56,25 +59,24 @@ def _add_rmsnorm_bwd(h, dy, dh, weight, rstd, *, need_dw=True):
     """Gradients of (y, h) -> (x, residual, weight).  `dy` decides x's type; `dh` may be None.  When the two
     types are one, dx and dresidual are the same tensor."""
     _require_cuda(h)
-    shape, N = h.shape, h.shape[-1]
+    device, shape = h.device, h.shape
     assert dy.shape == shape and (dh is None or dh.shape == shape), 'expect input and output shape to be the same'
     for t in (dy, dh, rstd):
-        if t is not None and t.device != h.device:
-            raise RuntimeError(f"b200norm: gradient on {t.device}, input on {h.device}")
-    Fn._check_dim(dy, N)
+        if t is not None and t.device != device:
+            raise RuntimeError(f"b200norm: gradient on {t.device}, input on {device}")
     if dh is not None and dh.dtype != h.dtype:
         dh = dh.to(h.dtype)
-    hr, dyr = _rows(h), _rows(dy)
-    dhr = _rows(dh) if dh is not None else None
-    M = hr.shape[0]
-    weight, _, wcode = _params(weight, None, N, h.device)
-    split = h.dtype != dy.dtype
-    dx = torch.empty(shape, dtype=dy.dtype, device=h.device)
-    dres = torch.empty(shape, dtype=h.dtype, device=h.device) if split else None
-    dw = torch.empty((N,), dtype=weight.dtype, device=h.device) if (weight is not None and need_dw) else None
+    hr, M, N, hs = _flat(h)
+    dyr, _, _, dys = _flat(dy)
+    dhr, _, _, dhs = _flat(dh) if dh is not None else (None, M, N, N)
+    Fn._check_dim(dy, N)
+    weight, _, wcode = _params(weight, None, N, device)
+    dx = _like(dy, dyr)
+    dres = _like(h, hr) if h.dtype != dy.dtype else None
+    dw = torch.empty_like(weight) if (weight is not None and need_dw) else None
     io, res = _code(dyr, "input"), _code(hr, "residual")
     lib = _lib.load()
-    index = h.device.index
+    index = device.index
     with _on_device(index):
         ws, ws_bytes = None, 0
         if dw is not None:
@@ -85,16 +87,21 @@ def _add_rmsnorm_bwd(h, dy, dh, weight, rstd, *, need_dw=True):
                 if ws_bytes == 0:
                     _lib.check(_lib.ERR_ARG)
                 _ADD_WS[key] = ws_bytes
-            ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=h.device)
+            ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=device)
         _lib.check(lib.b200norm_add_rms_bwd(
-            hr.data_ptr(), _row_stride(hr), dyr.data_ptr(), _row_stride(dyr), _ptr(dhr),
-            _row_stride(dhr) if dhr is not None else N, _ptr(weight), rstd.data_ptr(), dx.data_ptr(), N, _ptr(dres), N,
-            _ptr(dw), _ptr(ws), ws_bytes, M, N, io, res, wcode, _raw_stream(index)))
-    return dx, (dres if split else dx), dw
+            hr.data_ptr(), hs, dyr.data_ptr(), dys, _ptr(dhr), dhs, _ptr(weight), rstd.data_ptr(), dx.data_ptr(), N, _ptr(dres),
+            N, _ptr(dw), _ptr(ws), ws_bytes, M, N, io, res, wcode, _raw_stream(index)))
+    return dx, (dx if dres is None else dres), dw
 
 
 class add_rmsnorm(torch.autograd.Function):
     """(x, residual, weight or None, eps) -> (y, h).  Saves (h, weight, rstd)."""
+
+    @classmethod
+    def apply(cls, x, residual, weight, eps):
+        if not torch.is_grad_enabled():  # nothing to record: a decode step's call is spared autograd's bookkeeping
+            return _add_rmsnorm_fwd(x, residual, weight, eps, need_rstd=False)[:2]
+        return super().apply(x, residual, weight, eps)
 
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
@@ -133,22 +140,25 @@ def rmsnorm_fp8(x, weight=None, eps=1e-5, *, residual=None, group=0, scale_dtype
         raise RuntimeError(f"b200norm: scales are float32 or float8_e8m0fnu, not {scale_dtype}")
     if x.dtype == torch.float64:
         raise RuntimeError("b200norm: input dtype torch.float64 is not supported (float32, float16, bfloat16)")
-    shape, N = x.shape, x.shape[-1]
+    shape, device = x.shape, x.device
+    if residual is not None:
+        _check_residual(x, residual)
+    x, M, N, xs = _flat(x)
     Fn._check_dim(x, N)
-    r = _residual_rows(x, residual) if residual is not None else None
-    x = _rows(x)
-    M = x.shape[0]
-    weight, _, wcode = _params(weight, None, N, x.device)
-    q = torch.empty(shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty((*shape[:-1], -(-N // group) if group else 1), dtype=scale_dtype, device=x.device)
-    h = torch.empty(shape, dtype=r.dtype, device=x.device) if r is not None else None
-    code = _code(x, "input")
+    code = rcode = _code(x, "input")
+    r, rs, h = None, N, None
+    if residual is not None:
+        r, _, _, rs = _flat(residual)
+        h, rcode = _like(residual, r), _code(r, "residual")
+    weight, _, wcode = _params(weight, None, N, device)
+    q = torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)
+    scale = torch.empty((*shape[:-1], -(-N // group) if group else 1), dtype=scale_dtype, device=device)
     lib = _lib.load()
-    with _on_device(x.device.index):
+    index = device.index
+    with _on_device(index):
         _lib.check(lib.b200norm_rms_fp8(
-            x.data_ptr(), _row_stride(x), _ptr(r), _row_stride(r) if r is not None else N, _ptr(weight), q.data_ptr(), N,
-            scale.data_ptr(), _ptr(h), N, M, N, float(eps), group, int(scale_dtype != torch.float32), code,
-            _code(r, "residual") if r is not None else code, wcode, _raw_stream(x.device.index)))
+            x.data_ptr(), xs, _ptr(r), rs, _ptr(weight), q.data_ptr(), N, scale.data_ptr(), _ptr(h), N, M, N, eps, group,
+            0 if scale_dtype == torch.float32 else 1, code, rcode, wcode, _raw_stream(index)))
     return (q, scale) if h is None else (q, scale, h)
 
 

@@ -82,6 +82,16 @@ def _row_stride(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
+def _flat(x: torch.Tensor):
+    """-> (x as rows the kernels accept, M, N, row stride).  A contiguous tensor is its own rows: the usual case
+    costs no view."""
+    N = x.shape[-1]
+    if N > 0 and x.is_contiguous():
+        return x, x.numel() // N, N, N
+    x = _rows(x)
+    return x, x.shape[0], N, _row_stride(x)
+
+
 def _params(weight, bias, N, device):
     """Contiguous parameter vectors of one storage type, or None."""
     if weight is not None:

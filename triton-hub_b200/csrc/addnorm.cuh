@@ -41,7 +41,10 @@ struct AddNormParams {
   int group;  // 8-bit form: columns per scale, 0 for one scale a row
   int groups_per_row;
   int e8m0;  // 8-bit form: scales are powers of two, stored as their biased exponent
+  int stages;   // backward with a ring: slots per row group
+  int* status;  // device status word for bounded waits that ran out
 };
+constexpr int kAddNormStages = 4;
 
 constexpr float kE4m3Max = 448.f;
 constexpr float kAmaxFloor = 5.421010862427522e-20f;  // 2^-64: a group of zeros still gets a finite scale
@@ -67,6 +70,13 @@ struct RawVec {
                    : "l"(p));
     }
   }
+  __device__ __forceinline__ void load_shared(const void* p) {
+#pragma unroll
+    for (int i = 0; i < kWords / 4; ++i) {
+      const uint4 v = ld_shared16(static_cast<const unsigned char*>(p) + 16 * i);
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  }
   __device__ __forceinline__ void store(E* p) const {
     if constexpr (kWords == 4) {
       st_stream(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
@@ -76,32 +86,13 @@ struct RawVec {
                    : "memory");
     }
   }
-  // Columns c0 .. c0 + VEC - 1 of a row of n, some of them outside it: element by element.
-  __device__ __forceinline__ void load_part(const E* row, int c0, int n) {
-    E v[VEC];
+  // Zeroes the elements whose column is outside a row of n.
+  __device__ __forceinline__ void mask(int c0, int n) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      v[e] = from_f32<E>(0.f);
-      if (c0 + e >= 0 && c0 + e < n) v[e] = row[c0 + e];
-    }
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-      if constexpr (sizeof(E) == 4) w[i] = reinterpret_cast<const uint32_t&>(v[i]);
-      else
-        w[i] = static_cast<uint32_t>(reinterpret_cast<const uint16_t&>(v[2 * i])) |
-               (static_cast<uint32_t>(reinterpret_cast<const uint16_t&>(v[2 * i + 1])) << 16);
-    }
-  }
-  __device__ __forceinline__ void store_part(E* row, int c0, int n) const {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      if (c0 + e < 0 || c0 + e >= n) continue;
-      if constexpr (sizeof(E) == 4) {
-        row[c0 + e] = __uint_as_float(w[e]);
-      } else {
-        const uint16_t b = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
-        row[c0 + e] = reinterpret_cast<const E&>(b);
-      }
+      if (c0 + e >= 0 && c0 + e < n) continue;
+      if constexpr (sizeof(E) == 4) w[e] = 0u;
+      else w[e / 2] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
     }
   }
   __device__ __forceinline__ void unpack(float2* f) const {
@@ -126,21 +117,78 @@ struct RawVec {
   }
 };
 
-// VEC parameter values from column c0; ALIGNED: c0 is a multiple of VEC and the vector's base 16-byte
-// aligned.  The parameters are re-read by every row a CTA handles: L1 serves them.
-template <int VEC, bool ALIGNED>
-__device__ __forceinline__ void load_w(const void* p, int dtype, int c0, int n, float2* f) {
+// A packet of which part lies outside its row, element by element.  Kept out of line: few packets come here.
+template <typename E, int VEC>
+__device__ __noinline__ RawVec<E, VEC> load_elements(const E* row, int c0, int n) {
+  RawVec<E, VEC> r;
+  r.zero();
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    if (c0 + e < 0 || c0 + e >= n) continue;
+    if constexpr (sizeof(E) == 4) r.w[e] = reinterpret_cast<const uint32_t*>(row)[c0 + e];
+    else r.w[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[c0 + e]) << (16 * (e & 1));
+  }
+  return r;
+}
+template <typename E, int VEC>
+__device__ __noinline__ void store_elements(E* row, int c0, int n, RawVec<E, VEC> r) {
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    if (c0 + e < 0 || c0 + e >= n) continue;
+    if constexpr (sizeof(E) == 4) reinterpret_cast<uint32_t*>(row)[c0 + e] = r.w[e];
+    else reinterpret_cast<uint16_t*>(row)[c0 + e] = static_cast<uint16_t>(r.w[e / 2] >> (16 * (e & 1)));
+  }
+}
+
+// Rows of one buffer.  OFF: a row's first and last packet may lie partly outside it.  A load then takes the
+// whole packet and masks it -- its other elements belong to the neighbouring row or to the gap before it -- unless
+// the packet leaves the buffer, which the first packet of the first row and the last of the last row may do.
+template <typename E, int VEC, bool OFF>
+struct Rows {
+  E* base;
+  int64_t stride;
+  int64_t size;  // elements from the first row's start to the last row's end
+  int n;
+
+  __device__ __forceinline__ Rows(const void* p, int64_t stride, int64_t m, int n)
+      : base(static_cast<E*>(const_cast<void*>(p))), stride(stride), size((m - 1) * stride + n), n(n) {}
+  __device__ __forceinline__ RawVec<E, VEC> load(int64_t row, int c0) const {
+    RawVec<E, VEC> r;
+    const int64_t at = row * stride + c0;
+    if constexpr (!OFF) {
+      r.load(base + at);
+    } else if (at >= 0 && at + VEC <= size) {
+      r.load(base + at);
+      if (c0 < 0 || c0 + VEC > n) r.mask(c0, n);
+    } else {
+      r = load_elements<E, VEC>(base + row * stride, c0, n);
+    }
+    return r;
+  }
+  __device__ __forceinline__ void store(int64_t row, int c0, const RawVec<E, VEC>& r) const {
+    if (!OFF || (c0 >= 0 && c0 + VEC <= n)) r.store(base + row * stride + c0);
+    else store_elements<E, VEC>(base + row * stride, c0, n, r);
+  }
+};
+
+// VEC parameter values from column c0, a multiple of VEC, of a 16-byte aligned vector.  The parameters are
+// re-read by every row a CTA handles: L1 serves them.
+template <int VEC>
+__device__ __forceinline__ void load_w(const void* p, int dtype, int c0, float2* f) {
   float v[VEC];
   if (p == nullptr) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = 1.f;
-  } else if (ALIGNED && dtype == kF32) {
+  } else if (dtype == kF32) {
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i) {
       const float4 q = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + c0) + i);
       v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
     }
-  } else if (ALIGNED && (dtype == kF16 || dtype == kBF16)) {
+  } else if (dtype == kF64) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = static_cast<float>(static_cast<const double*>(p)[c0 + e]);
+  } else {
     uint32_t q[VEC / 2];
     const uint16_t* src = static_cast<const uint16_t*>(p) + c0;
     if constexpr (VEC == 8) {
@@ -161,32 +209,76 @@ __device__ __forceinline__ void load_w(const void* p, int dtype, int c0, int n, 
         v[2 * i + 1] = h.y;
       }
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) v[e] = (c0 + e >= 0 && c0 + e < n) ? load_param(p, dtype, c0 + e) : 0.f;
   }
 #pragma unroll
   for (int i = 0; i < VEC / 2; ++i) f[i] = make_float2(v[2 * i], v[2 * i + 1]);
 }
 
-// Maximum that keeps a NaN, so that a poisoned group shows in its scale.
-__device__ __forceinline__ float max_nan(float a, float b) {
+// Rows off the packet boundaries: the parameters wait in shared memory as fp32, with a word left free after every
+// VEC of them so that the lanes' reads, VEC words apart, fall into different banks.
+template <int VEC>
+__host__ __device__ constexpr int w_slots(int n) { return (n + n / VEC + 4) / 4 * 4; }
+template <int VEC>
+__device__ __forceinline__ void stage_w(const void* p, int dtype, int n, float* ws) {
+#pragma unroll 1
+  for (int c = threadIdx.x; c < n; c += blockDim.x) ws[c + c / VEC] = p != nullptr ? load_param(p, dtype, c) : 1.f;
+}
+template <int VEC>
+__device__ __forceinline__ void staged_w(const float* ws, int c0, int n, float2* f) {
+  float v[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const int c = c0 + e;
+    v[e] = c >= 0 && c < n ? ws[c + c / VEC] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i) f[i] = make_float2(v[2 * i], v[2 * i + 1]);
+}
+
+// Maxima of magnitudes that keep a NaN, so that a poisoned group shows in its scale.
+__device__ __forceinline__ float max_abs(float a, float b) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return fabsf(r);
+}
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float warp_max_abs(float v) {
+  float r;
+  asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
 
-// The scale of a group whose largest magnitude is `amax`, and the byte a power-of-two scale is stored as.
-__device__ __forceinline__ float fp8_scale(float amax, bool e8m0, uint8_t* code) {
-  float s = max_nan(amax, kAmaxFloor) / kE4m3Max;
+// A group's scale from its largest magnitude, the byte that a power-of-two scale is stored as, and 1 / scale
+// (one instruction good to an ulp: it moves a value only where that lies within an ulp of a border between two
+// e4m3 values; the reciprocal of a power of two is exact).
+struct Fp8Scale {
+  float scale, inv;
+  uint8_t code;
+};
+__device__ __forceinline__ Fp8Scale fp8_scale(float amax, bool e8m0) {
+  Fp8Scale r;
+  amax = max_abs(amax, kAmaxFloor);
+  r.code = 0;
   if (e8m0) {
+    r.scale = amax / kE4m3Max;  // correctly rounded: a power of two must not look like a little more
     // the next power of two: the exponent field, one more where the fraction is not zero
-    const uint32_t bits = __float_as_uint(s);
-    const uint32_t e = (s != s) ? 255u : (bits + 0x7fffffu) >> 23;
-    *code = static_cast<uint8_t>(e);
-    s = __uint_as_float(e == 255u ? 0x7fffffffu : e << 23);
+    const uint32_t e = r.scale != r.scale ? 255u : (__float_as_uint(r.scale) + 0x7fffffu) >> 23;
+    r.code = static_cast<uint8_t>(e);
+    r.scale = __uint_as_float(e == 255u ? 0x7fffffffu : e << 23);
+    r.inv = __uint_as_float(e == 255u ? 0x7fffffffu : (254u - e) << 23);
+  } else {
+    r.scale = amax * (1.f / kE4m3Max);
+    r.inv = rcp_fast(r.scale);
   }
-  return s;
+  return r;
+}
+__device__ __forceinline__ void store_scale(void* p, int64_t at, const Fp8Scale& s, bool e8m0) {
+  if (e8m0) static_cast<uint8_t*>(p)[at] = s.code;
+  else static_cast<float*>(p)[at] = s.scale;
 }
 
 __device__ __forceinline__ uint32_t fp8x2(float lo, float hi) {  // saturating, NaN stays NaN
@@ -195,11 +287,22 @@ __device__ __forceinline__ uint32_t fp8x2(float lo, float hi) {  // saturating, 
   return r;
 }
 
-__host__ __device__ constexpr int addnorm_threads(int tpr) { return tpr < 256 ? 256 : tpr; }
+// Threads of a CTA: row groups of fewer than 160 threads share one.
+__host__ __device__ constexpr int addnorm_threads(int tpr) { return tpr < 160 ? 256 / tpr * tpr : tpr; }
 
 // Whether a backward thread's LD * VEC dweight sums go to shared memory: they would not fit in the
 // registers beside the row.
 __host__ __device__ constexpr bool addnorm_wide(int ld, int vec, int tpr) { return ld * vec > 24 || tpr > 512; }
+
+// CTAs per SM that the register allocation leaves room for: as many threads as run without spills.
+__host__ __device__ constexpr int addnorm_fwd_ctas(int ld, int tpr, bool lean) {
+  const int n = (ld > 2 ? 512 : lean ? 1024 : 768) / addnorm_threads(tpr);
+  return n < 1 ? 1 : n;
+}
+__host__ __device__ constexpr int addnorm_bwd_ctas(int ld, int tpr, bool lean) {
+  const int n = (ld > 2 ? 512 : lean ? 768 : 512) / addnorm_threads(tpr);
+  return n < 1 ? 1 : n;
+}
 
 // Sum over the TPR threads that share a row.
 template <int TPR, int FIRST>
@@ -218,16 +321,18 @@ __device__ __forceinline__ float row_sum(float v, float* scratch, int& phase, in
 // Forward.  OFF: the rows of all buffers start at one common offset within a packet that need not be
 // zero (contiguous tensors of an odd row length); packets are then laid on the buffers' own alignment,
 // the first and the last of a row are partial, and the launch gives every row group rows of one offset
-// only (row_step is a multiple of the offsets' period), so that a thread's columns stay the same.
+// only (its step is a multiple of the offsets' period), so that a thread's columns stay the same.
 // FP8: the 8-bit form.  Thread t of a row group holds packets t, t + TPR, ...: neighbouring lanes hold
 // neighbouring columns, so a scale's 32, 64 or 128 columns are 4 to 32 adjacent lanes of one warp.
 template <typename T, typename R, int LD, int TPR, bool OFF, bool FP8>
-__global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_fwd_kernel(const AddNormParams p) {
+__global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR, !OFF && !(FP8 && TPR <= 128)))
+    addnorm_fwd_kernel(const AddNormParams p) {
   static_assert(!(OFF && FP8), "scale groups lie on packet boundaries");
   constexpr int VEC = Pack16<T>::kElems, H = VEC / 2;
   constexpr int GROUPS = addnorm_threads(TPR) / TPR;
   constexpr int WARPS_N = TPR >= 32 ? TPR / 32 : 1;
   constexpr bool WREG = LD * VEC <= 16;  // the weights fit in registers next to the row
+  extern __shared__ __align__(16) float ws[];  // OFF: the weights
   __shared__ float scratch[GROUPS][2 * WARPS_N];
   __shared__ float max_scratch[FP8 ? GROUPS : 1][2 * WARPS_N];
 
@@ -237,18 +342,28 @@ __global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_fwd_kernel(const
   grid_dependency_sync();
   trigger_dependents();
 
+  const Rows<T, VEC, OFF> xs(p.x, p.x_stride, p.M, p.N), ys(p.y, p.y_stride, p.M, p.N);
+  const Rows<R, VEC, OFF> rs(p.r, p.r_stride, p.M, p.N), hs(p.h, p.h_stride, p.M, p.N);
   const int64_t first = (int64_t)blockIdx.x * GROUPS + group;
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   const int off = OFF ? static_cast<int>((reinterpret_cast<uintptr_t>(p.x) / sizeof(T) + first * p.x_stride) % VEC) : 0;
   const int packets = (off + p.N + VEC - 1) / VEC;
   const float inv_n = 1.f / static_cast<float>(p.N);
 
+  if constexpr (OFF) {
+    stage_w<VEC>(p.w, p.w_dtype, p.N, ws);
+    __syncthreads();
+  }
+  auto weights = [&](int c0, float2* f) {
+    if constexpr (OFF) staged_w<VEC>(ws, c0, p.N, f);
+    else load_w<VEC>(p.w, p.w_dtype, c0, f);
+  };
   float2 wr[WREG ? LD : 1][H];
   if constexpr (WREG) {
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
       const int pk = j * TPR + t;
-      if (pk < packets) load_w<VEC, !OFF>(p.w, p.w_dtype, pk * VEC - off, p.N, wr[j]);
+      if (pk < packets) weights(pk * VEC - off, wr[j]);
     }
   }
 
@@ -257,9 +372,6 @@ __global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_fwd_kernel(const
   for (int64_t i = 0; lead + i < p.M; i += step) {
     const int64_t row = first + i;
     const bool valid = TPR >= 32 || row < p.M;
-    const T* xrow = static_cast<const T*>(p.x) + row * p.x_stride;
-    const R* rrow = static_cast<const R*>(p.r) + row * p.r_stride;
-    R* hrow = static_cast<R*>(p.h) + row * p.h_stride;
 
     float2 hf[LD][H];
     {
@@ -267,21 +379,16 @@ __global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_fwd_kernel(const
       RawVec<R, VEC> rv[LD];
 #pragma unroll
       for (int j = 0; j < LD; ++j) {
-        const int pk = j * TPR + t, c0 = pk * VEC - off;
+        const int pk = j * TPR + t;
         xv[j].zero();
         rv[j].zero();
         if (!valid || pk >= packets) continue;
-        if (!OFF || (c0 >= 0 && c0 + VEC <= p.N)) {
-          xv[j].load(xrow + c0);
-          if (p.r != nullptr) rv[j].load(rrow + c0);
-        } else {
-          xv[j].load_part(xrow, c0, p.N);
-          if (p.r != nullptr) rv[j].load_part(rrow, c0, p.N);
-        }
+        xv[j] = xs.load(row, pk * VEC - off);
+        if (p.r != nullptr) rv[j] = rs.load(row, pk * VEC - off);
       }
 #pragma unroll
       for (int j = 0; j < LD; ++j) {
-        const int pk = j * TPR + t, c0 = pk * VEC - off;
+        const int pk = j * TPR + t;
         xv[j].unpack(hf[j]);
         if (p.r != nullptr) {
           float2 rf[H];
@@ -290,13 +397,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_fwd_kernel(const
           for (int k = 0; k < H; ++k) hf[j][k] = add2(hf[j][k], rf[k]);
           rv[j].pack(hf[j]);
           if (sizeof(R) < 4) rv[j].unpack(hf[j]);  // the norm is that of h as stored
-        } else if constexpr (sizeof(R) == sizeof(T)) {
-#pragma unroll
-          for (int k = 0; k < RawVec<R, VEC>::kWords; ++k) rv[j].w[k] = xv[j].w[k];
-        }
-        if (p.h != nullptr && valid && pk < packets) {
-          if (!OFF || (c0 >= 0 && c0 + VEC <= p.N)) rv[j].store(hrow + c0);
-          else rv[j].store_part(hrow, c0, p.N);
+          if (p.h != nullptr && valid && pk < packets) hs.store(row, pk * VEC - off, rv[j]);
         }
       }
     }
@@ -311,85 +412,76 @@ __global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_fwd_kernel(const
     if (t == 0 && valid && p.rstd != nullptr) p.rstd[row] = rstd;
     const float2 r2 = splat2(rstd);
 
-    float amax = 0.f;  // FP8, one scale a row
+    float amax = 0.f;  // one scale a row
     float amax_j[FP8 ? LD : 1];
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
-      const int pk = j * TPR + t, c0 = pk * VEC - off;
+      const int pk = j * TPR + t;
+      if constexpr (FP8) amax_j[j] = 0.f;
+      if (pk >= packets) continue;
       float2 wf[H];
       if constexpr (WREG) {
 #pragma unroll
         for (int k = 0; k < H; ++k) wf[k] = wr[j][k];
-      } else if (pk < packets) {
-        load_w<VEC, !OFF>(p.w, p.w_dtype, c0, p.N, wf);
+      } else {
+        weights(pk * VEC - off, wf);
       }
-      if constexpr (!FP8) {
-        if (valid && pk < packets) {
 #pragma unroll
-          for (int k = 0; k < H; ++k) hf[j][k] = mul2(mul2(hf[j][k], r2), wf[k]);
-          T* yrow = static_cast<T*>(p.y) + row * p.y_stride;
-          RawVec<T, VEC> o;
-          o.pack(hf[j]);
-          if (!OFF || (c0 >= 0 && c0 + VEC <= p.N)) o.store(yrow + c0);
-          else o.store_part(yrow, c0, p.N);
-        }
+      for (int k = 0; k < H; ++k) hf[j][k] = mul2(mul2(hf[j][k], r2), wf[k]);
+      if constexpr (!FP8) {
+        RawVec<T, VEC> o;
+        o.pack(hf[j]);
+        if (valid) ys.store(row, pk * VEC - off, o);
       } else {
         float a = 0.f;
-        if (pk < packets) {
 #pragma unroll
-          for (int k = 0; k < H; ++k) {
-            hf[j][k] = mul2(mul2(hf[j][k], r2), wf[k]);
-            a = max_nan(a, max_nan(fabsf(hf[j][k].x), fabsf(hf[j][k].y)));
-          }
-        }
+        for (int k = 0; k < H; ++k) a = max_abs3(a, hf[j][k].x, hf[j][k].y);
         amax_j[j] = a;
-        amax = max_nan(amax, a);
+        amax = max_abs(amax, a);
       }
     }
 
     if constexpr (FP8) {
       uint8_t* qrow = static_cast<uint8_t*>(p.y) + row * p.y_stride;
-      float scale = 0.f, inv = 0.f;
-      uint8_t code = 0;
-      const int lanes = p.group == 0 ? (TPR < 32 ? TPR : 32) : min(p.group / VEC, TPR);  // adjacent lanes to merge
+      Fp8Scale sc;
       if (p.group == 0) {
+        if constexpr (TPR >= 32) {
+          amax = warp_max_abs(amax);
+        } else {
 #pragma unroll
-        for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+          for (int o = TPR / 2; o > 0; o >>= 1) amax = max_abs(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        }
         if constexpr (TPR > 32) {
           float* buf = max_scratch[group] + max_phase * WARPS_N;
           if (lane == 0) buf[warp_n] = amax;
           group_sync<WARPS_N, 0>(group);
 #pragma unroll
-          for (int k = 0; k < WARPS_N; ++k) amax = max_nan(amax, buf[k]);
+          for (int k = 0; k < WARPS_N; ++k) amax = max_abs(amax, buf[k]);
           max_phase ^= 1;
         }
-        scale = fp8_scale(amax, p.e8m0 != 0, &code);
-        inv = 1.f / scale;
-        if (t == 0 && valid) {
-          if (p.e8m0) static_cast<uint8_t*>(p.scale)[row] = code;
-          else static_cast<float*>(p.scale)[row] = scale;
-        }
+        sc = fp8_scale(amax, p.e8m0 != 0);
+        if (t == 0 && valid) store_scale(p.scale, row, sc, p.e8m0 != 0);
       }
+      const int lanes = p.group == 0 ? 1 : min(p.group / VEC, TPR);  // adjacent lanes that share a scale
 #pragma unroll
       for (int j = 0; j < LD; ++j) {
         const int pk = j * TPR + t;
         if (p.group != 0) {
           float a = amax_j[j];
-          for (int o = 1; o < lanes; o <<= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-          scale = fp8_scale(a, p.e8m0 != 0, &code);
-          inv = 1.f / scale;
-          if (valid && pk < packets && (t & (lanes - 1)) == 0) {
-            const int64_t at = row * p.groups_per_row + pk * VEC / p.group;
-            if (p.e8m0) static_cast<uint8_t*>(p.scale)[at] = code;
-            else static_cast<float*>(p.scale)[at] = scale;
-          }
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1)
+            if (o < lanes) a = max_abs(a, __shfl_xor_sync(0xffffffffu, a, o));
+          sc = fp8_scale(a, p.e8m0 != 0);
+          if (valid && pk < packets && (t & (lanes - 1)) == 0)
+            store_scale(p.scale, row * p.groups_per_row + pk * VEC / p.group, sc, p.e8m0 != 0);
         }
         if (valid && pk < packets) {
+          const float2 inv2 = splat2(sc.inv);
           uint32_t word[VEC / 4];
 #pragma unroll
           for (int k = 0; k < VEC / 4; ++k) {
-            const float2 lo = hf[j][2 * k], hi = hf[j][2 * k + 1];
-            word[k] = fp8x2(lo.x * inv, lo.y * inv) | (fp8x2(hi.x * inv, hi.y * inv) << 16);
+            const float2 lo = mul2(hf[j][2 * k], inv2), hi = mul2(hf[j][2 * k + 1], inv2);
+            word[k] = fp8x2(lo.x, lo.y) | (fp8x2(hi.x, hi.y) << 16);
           }
           if constexpr (VEC == 8) __stcs(reinterpret_cast<uint2*>(qrow + pk * VEC), make_uint2(word[0], word[1]));
           else __stcs(reinterpret_cast<uint32_t*>(qrow + pk * VEC), word[0]);
@@ -400,37 +492,83 @@ __global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_fwd_kernel(const
 }
 
 // Backward.  A thread owns fixed columns of every row its group visits and carries their dweight sums:
-// in registers, or (WIDE: more than 16 of them) in shared memory, laid out so that lane t touches word t.
-// The row groups of a CTA are added in order at the end: one partial row per CTA.
-template <typename T, typename R, int LD, int TPR, bool OFF>
-__global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_bwd_kernel(const AddNormParams p) {
+// in registers, or (WIDE) in shared memory, laid out so that lane t touches word t.  The row groups of a
+// CTA are added in order at the end: one partial row per CTA.
+//
+// RING: the rows of h, dy and dh reach the registers through a ring of p.stages shared-memory slots per row
+// group, filled by bulk asynchronous copies, so that whole rows stay in flight while others are reduced.
+// A slot is refilled behind the row's reduction, a barrier that every thread passes with its packets read.
+template <typename T, typename R, int LD, int TPR, bool OFF, bool RING>
+__global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_bwd_ctas(LD, TPR, sizeof(R) == sizeof(T) && TPR >= 160)) addnorm_bwd_kernel(const AddNormParams p) {
+  static_assert(!(OFF && RING) && !(RING && TPR < 32), "bulk copies take whole packets; a ring belongs to whole warps");
   constexpr int VEC = Pack16<T>::kElems, H = VEC / 2;
   constexpr int GROUPS = addnorm_threads(TPR) / TPR;
   constexpr int WARPS_N = TPR >= 32 ? TPR / 32 : 1;
   constexpr bool WREG = LD * VEC <= 16;
   constexpr bool WIDE = addnorm_wide(LD, VEC, TPR);
-  extern __shared__ __align__(16) float acc[];  // WIDE: [LD * VEC][TPR]; GROUPS > 1: [GROUPS][N]
+  // OFF: the weights; then the sums, WIDE [LD * VEC][TPR] or, of several groups, [GROUPS][N]; RING: the slots, which
+  // the sums of several groups reuse
+  extern __shared__ __align__(128) unsigned char dyn[];
+  float* ws = reinterpret_cast<float*>(dyn);
+  float* acc = ws + (OFF ? w_slots<VEC>(p.N) : 0);
   __shared__ float scratch[GROUPS][2 * WARPS_N];
+  __shared__ __align__(8) uint64_t bars[RING ? GROUPS : 1][kAddNormStages];
+  __shared__ int cta_abort;
 
   const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
   const int lane = threadIdx.x & 31, warp_n = TPR >= 32 ? t / 32 : 0;
   int phase = 0;
+  if constexpr (RING) {
+    if (threadIdx.x == 0) {
+      for (int g = 0; g < GROUPS; ++g)
+        for (int i = 0; i < p.stages; ++i) mbar_init(&bars[g][i], 1);
+      cta_abort = 0;
+      mbar_init_fence();
+    }
+    __syncthreads();
+  }
   grid_dependency_sync();
   trigger_dependents();
 
+  const Rows<T, VEC, OFF> gs(p.x, p.x_stride, p.M, p.N), dxs(p.y, p.y_stride, p.M, p.N);
+  const Rows<R, VEC, OFF> hs(p.h, p.h_stride, p.M, p.N), ds(p.r, p.r_stride, p.M, p.N), drs(p.dr, p.dr_stride, p.M, p.N);
   const int64_t first = (int64_t)blockIdx.x * GROUPS + group;
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   const int off = OFF ? static_cast<int>((reinterpret_cast<uintptr_t>(p.x) / sizeof(T) + first * p.x_stride) % VEC) : 0;
   const int packets = (off + p.N + VEC - 1) / VEC;
   const float inv_n = 1.f / static_cast<float>(p.N);
 
+  const uint32_t t_bytes = p.N * sizeof(T), r_bytes = p.N * sizeof(R);
+  const uint32_t slot_bytes = t_bytes + r_bytes * (p.r != nullptr ? 2 : 1);
+  unsigned char* slots = dyn + (WIDE ? sizeof(float) * LD * VEC * TPR : 0) + (size_t)group * p.stages * slot_bytes;
+  auto fill = [&](int s, int64_t row) {  // the group's first thread: dy, h, dh of a row into slot s
+    unsigned char* dst = slots + (size_t)s * slot_bytes;
+    uint64_t* bar = &bars[group][s];
+    mbar_expect_tx(bar, slot_bytes);
+    bulk_load(dst, gs.base + row * gs.stride, t_bytes, bar);
+    bulk_load(dst + t_bytes, hs.base + row * hs.stride, r_bytes, bar);
+    if (p.r != nullptr) bulk_load(dst + t_bytes + r_bytes, ds.base + row * ds.stride, r_bytes, bar);
+  };
+  if constexpr (RING) {
+    if (t == 0)
+      for (int s = 0; s < p.stages; ++s)
+        if (first + s * step < p.M) fill(s, first + s * step);
+  }
+  if constexpr (OFF) {
+    stage_w<VEC>(p.w, p.w_dtype, p.N, ws);
+    __syncthreads();
+  }
+  auto weights = [&](int c0, float2* f) {
+    if constexpr (OFF) staged_w<VEC>(ws, c0, p.N, f);
+    else load_w<VEC>(p.w, p.w_dtype, c0, f);
+  };
   float2 wr[WREG ? LD : 1][H];
   float2 dw[WIDE ? 1 : LD][H];
   if constexpr (WREG) {
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
       const int pk = j * TPR + t;
-      if (pk < packets) load_w<VEC, !OFF>(p.w, p.w_dtype, pk * VEC - off, p.N, wr[j]);
+      if (pk < packets) weights(pk * VEC - off, wr[j]);
     }
   }
   if constexpr (WIDE) {
@@ -443,36 +581,37 @@ __global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_bwd_kernel(const
       for (int k = 0; k < H; ++k) dw[j][k] = splat2(0.f);
   }
 
+  int slot = 0;
+  uint32_t parity = 0;
   const int64_t lead = TPR < 32 ? (int64_t)blockIdx.x * GROUPS + (threadIdx.x & ~31) / TPR : first;
   for (int64_t i = 0; lead + i < p.M; i += step) {
     const int64_t row = first + i;
     const bool valid = TPR >= 32 || row < p.M;
-    const T* grow = static_cast<const T*>(p.x) + row * p.x_stride;  // dy
-    const R* hrow = static_cast<const R*>(p.h) + row * p.h_stride;
-    const R* drow = static_cast<const R*>(p.r) + row * p.r_stride;  // dh
-    const float rs = valid ? __ldg(p.rstd + row) : 0.f;
+    const float rstd = valid ? __ldg(p.rstd + row) : 0.f;
 
     RawVec<T, VEC> gv[LD];
     RawVec<R, VEC> hv[LD], dv[LD];
+    const unsigned char* src = slots + (size_t)slot * slot_bytes;
+    if constexpr (RING) mbar_wait(&bars[group][slot], parity, &cta_abort, p.status);
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
-      const int pk = j * TPR + t, c0 = pk * VEC - off;
+      const int pk = j * TPR + t;
       gv[j].zero();
       hv[j].zero();
       dv[j].zero();
       if (!valid || pk >= packets) continue;
-      if (!OFF || (c0 >= 0 && c0 + VEC <= p.N)) {
-        gv[j].load(grow + c0);
-        hv[j].load(hrow + c0);
-        if (p.r != nullptr) dv[j].load(drow + c0);
+      if constexpr (RING) {
+        gv[j].load_shared(src + (size_t)pk * VEC * sizeof(T));
+        hv[j].load_shared(src + t_bytes + (size_t)pk * VEC * sizeof(R));
+        if (p.r != nullptr) dv[j].load_shared(src + t_bytes + r_bytes + (size_t)pk * VEC * sizeof(R));
       } else {
-        gv[j].load_part(grow, c0, p.N);
-        hv[j].load_part(hrow, c0, p.N);
-        if (p.r != nullptr) dv[j].load_part(drow, c0, p.N);
+        gv[j] = gs.load(row, pk * VEC - off);
+        hv[j] = hs.load(row, pk * VEC - off);
+        if (p.r != nullptr) dv[j] = ds.load(row, pk * VEC - off);
       }
     }
     float2 s2 = splat2(0.f);
-    const float2 rs2 = splat2(rs);
+    const float2 rs2 = splat2(rstd);
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
       const int pk = j * TPR + t;
@@ -484,7 +623,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_bwd_kernel(const
 #pragma unroll
         for (int k = 0; k < H; ++k) wf[k] = wr[j][k];
       } else {
-        load_w<VEC, !OFF>(p.w, p.w_dtype, pk * VEC - off, p.N, wf);
+        weights(pk * VEC - off, wf);
       }
 #pragma unroll
       for (int k = 0; k < H; ++k) {
@@ -499,13 +638,19 @@ __global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_bwd_kernel(const
       }
     }
     const float c1 = row_sum<TPR, (GROUPS == 1 ? 0 : 1)>(s2.x + s2.y, scratch[group], phase, group, warp_n, lane) * inv_n;
+    if constexpr (RING) {
+      if (TPR == 32) __syncwarp();
+      if (t == 0 && row + p.stages * step < p.M) fill(slot, row + p.stages * step);
+      if (++slot == p.stages) {
+        slot = 0;
+        parity ^= 1u;
+      }
+    }
     // d = w * dy * rstd - h * (c1 * rstd^2) + dh
-    const float2 kh = splat2(-c1 * rs * rs);
-    T* dxrow = static_cast<T*>(p.y) + row * p.y_stride;
-    R* drrow = static_cast<R*>(p.dr) + row * p.dr_stride;
+    const float2 kh = splat2(-c1 * rstd * rstd);
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
-      const int pk = j * TPR + t, c0 = pk * VEC - off;
+      const int pk = j * TPR + t;
       if (!valid || pk >= packets) continue;
       float2 gf[H], hf[H], wf[H], df[H];
       gv[j].unpack(gf);
@@ -515,20 +660,28 @@ __global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_bwd_kernel(const
 #pragma unroll
         for (int k = 0; k < H; ++k) wf[k] = wr[j][k];
       } else {
-        load_w<VEC, !OFF>(p.w, p.w_dtype, c0, p.N, wf);
+        weights(pk * VEC - off, wf);
       }
 #pragma unroll
       for (int k = 0; k < H; ++k) df[k] = fma2(mul2(wf[k], rs2), gf[k], fma2(hf[k], kh, df[k]));
-      const bool full = !OFF || (c0 >= 0 && c0 + VEC <= p.N);
       RawVec<T, VEC> o;
       o.pack(df);
-      if (full) o.store(dxrow + c0);
-      else o.store_part(dxrow, c0, p.N);
+      dxs.store(row, pk * VEC - off, o);
       if constexpr (sizeof(R) != sizeof(T)) {
         RawVec<R, VEC> od;
         od.pack(df);
-        if (full) od.store(drrow + c0);
-        else od.store_part(drrow, c0, p.N);
+        drs.store(row, pk * VEC - off, od);
+      }
+    }
+  }
+  if constexpr (RING) {
+    if (t == 0 && cta_abort) {  // a wait ran out: what is still in flight gets a bounded chance to land
+      const int64_t rows = first < p.M ? (p.M - first + step - 1) / step : 0;
+      const unsigned long long t0 = global_ns();
+      for (int s = 0; s < p.stages && s < rows; ++s) {
+        const int64_t fills = (rows - s + p.stages - 1) / p.stages;
+        while (!mbar_try_wait(&bars[group][s], static_cast<uint32_t>((fills - 1) & 1)))
+          if (global_ns() - t0 > 10000000ull) break;
       }
     }
   }
@@ -537,6 +690,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_bwd_kernel(const
   float* out = p.part + (size_t)blockIdx.x * p.N;
   if constexpr (GROUPS > 1) {
     static_assert(GROUPS == 1 || !WIDE, "several row groups keep their sums in registers");
+    if constexpr (RING) __syncthreads();  // every group has read its slots: the sums go there
     float* mine = acc + (size_t)group * p.N;
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
@@ -544,7 +698,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_bwd_kernel(const
       if (pk >= packets) continue;
 #pragma unroll
       for (int k = 0; k < VEC; ++k)
-        if (c0 + k >= 0 && c0 + k < p.N) mine[c0 + k] = (k & 1) ? dw[j][k / 2].y : dw[j][k / 2].x;
+        if (!OFF || (c0 + k >= 0 && c0 + k < p.N)) mine[c0 + k] = (k & 1) ? dw[j][k / 2].y : dw[j][k / 2].x;
     }
     __syncthreads();
     for (int c = threadIdx.x; c < p.N; c += GROUPS * TPR) {
@@ -572,6 +726,35 @@ __global__ void __launch_bounds__(addnorm_threads(TPR)) addnorm_bwd_kernel(const
       }
     }
   }
+}
+
+// dweight from the CTAs' partial rows: a CTA takes 32 columns, its warps every 32nd row each, eight loads in flight
+// per thread; then a warp adds a column's 32 sums.  The order depends on the number of rows alone.
+struct AddNormReduceParams {
+  const float* part;
+  void* dw;
+  int rows, N, w_dtype;
+};
+static __global__ void __launch_bounds__(1024) addnorm_reduce_kernel(const AddNormReduceParams p) {
+  __shared__ float tile[32][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + tx;
+  grid_dependency_sync();
+  trigger_dependents();
+  float s = 0.f;
+  if (col < p.N) {
+    for (int r = ty; r < p.rows; r += 256) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = r + 32 * k < p.rows ? p.part[(size_t)(r + 32 * k) * p.N + col] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += v[k];
+    }
+  }
+  tile[ty][tx] = s;
+  __syncthreads();
+  s = warp_sum(tile[tx][ty]);
+  if (tx == 0 && blockIdx.x * 32 + ty < p.N) store_param(p.dw, p.w_dtype, blockIdx.x * 32 + ty, s);
 }
 
 // Buffers whose rows are aligned differently (views, odd strides): one CTA per row, element by element,
@@ -617,21 +800,16 @@ __global__ void __launch_bounds__(512) addnorm_fwd_any_kernel(const AddNormParam
         const float w = p.w != nullptr ? load_param(p.w, p.w_dtype, c) : 1.f;
         const float v = hs[c] * rstd * w;
         hs[c] = v;
-        amax = max_nan(amax, fabsf(v));
+        amax = max_abs(amax, v);
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      amax = warp_max_abs(amax);
       if (lane == 0) max_scratch[warp] = amax;
       __syncthreads();
       if (whole) {
-        for (int k = 0; k < 16; ++k) amax = max_nan(amax, max_scratch[k]);
-        uint8_t code = 0;
-        const float scale = fp8_scale(amax, p.e8m0 != 0, &code), inv = 1.f / scale;
-        if (threadIdx.x == 0) {
-          if (p.e8m0) static_cast<uint8_t*>(p.scale)[row] = code;
-          else static_cast<float*>(p.scale)[row] = scale;
-        }
-        for (int c = threadIdx.x; c < p.N; c += 512) qrow[c] = static_cast<uint8_t>(fp8x2(hs[c] * inv, 0.f));
+        for (int k = 0; k < 16; ++k) amax = max_abs(amax, max_scratch[k]);
+        const Fp8Scale sc = fp8_scale(amax, p.e8m0 != 0);
+        if (threadIdx.x == 0) store_scale(p.scale, row, sc, p.e8m0 != 0);
+        for (int c = threadIdx.x; c < p.N; c += 512) qrow[c] = static_cast<uint8_t>(fp8x2(hs[c] * sc.inv, 0.f));
       } else {
         for (int g = warp; g < p.groups_per_row; g += 16) {
           const int c0 = g * p.group;
@@ -640,21 +818,14 @@ __global__ void __launch_bounds__(512) addnorm_fwd_any_kernel(const AddNormParam
           for (int k = 0; k < 4; ++k) {
             const int c = c0 + k * 32 + lane;
             v[k] = (k * 32 < p.group && c < p.N) ? hs[c] : 0.f;
-            a = max_nan(a, fabsf(v[k]));
+            a = max_abs(a, v[k]);
           }
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-          uint8_t code = 0;
-          const float scale = fp8_scale(a, p.e8m0 != 0, &code), inv = 1.f / scale;
-          if (lane == 0) {
-            const int64_t at = row * p.groups_per_row + g;
-            if (p.e8m0) static_cast<uint8_t*>(p.scale)[at] = code;
-            else static_cast<float*>(p.scale)[at] = scale;
-          }
+          const Fp8Scale sc = fp8_scale(warp_max_abs(a), p.e8m0 != 0);
+          if (lane == 0) store_scale(p.scale, row * p.groups_per_row + g, sc, p.e8m0 != 0);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int c = c0 + k * 32 + lane;
-            if (k * 32 < p.group && c < p.N) qrow[c] = static_cast<uint8_t>(fp8x2(v[k] * inv, 0.f));
+            if (k * 32 < p.group && c < p.N) qrow[c] = static_cast<uint8_t>(fp8x2(v[k] * sc.inv, 0.f));
           }
         }
       }
@@ -711,6 +882,7 @@ struct AddNormShape {
   const void* fwd[2];  // [rows at a common offset]
   const void* fp8;
   const void* bwd[2];
+  const void* bwd_ring;  // null: none
   int capacity() const { return ld * tpr; }  // packets per row
   int threads() const { return addnorm_threads(tpr); }
   int groups() const { return threads() / tpr; }

@@ -59,32 +59,60 @@ Layout layout_of(const Buffer* b, int n, int64_t N, int vec, const void* w, int*
 
 struct Plan {
   const void* fn;
-  int threads, grid;
+  int threads, grid, stages;
   size_t smem;
 };
 
-int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, int period, int64_t M, int64_t N, Plan* out) {
+// Slots of a backward ring: as many, up to four, as leave room for three, two or one CTA per SM (228 KB, 1 KB of it
+// reserved per CTA, and a little static shared memory), at least two; 0 when two do not fit.
+int ring_stages(size_t slot, size_t fixed, int groups, size_t* smem) {
+  for (size_t cap : {74 * 1024, 112 * 1024, 224 * 1024})
+    for (int stages = kAddNormStages; stages >= 2; --stages)
+      if (fixed + slot * stages * groups <= cap) {
+        *smem = fixed + slot * stages * groups;
+        return stages;
+      }
+  return 0;
+}
+
+int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, int period, int64_t M, int64_t N, bool has_dh,
+         Plan* out) {
   const int vec = 16 / t->size_t_;
   // packets a row can span: up to one more at either end when it starts inside one
   const int64_t need = layout == kOffset ? (N + 2 * vec - 2) / vec : (N + vec - 1) / vec;
   const AddNormShape* s = nullptr;
+  out->stages = 0;
   if (layout == kAligned || (layout == kOffset && which != kFp8))
     for (int i = 0; i < t->n && s == nullptr; ++i)
       if (t->shapes[i].capacity() >= need) s = &t->shapes[i];
   int groups = 1;
+  out->smem = 0;
+  if (s != nullptr) {
+    groups = s->groups();
+    out->fn = which == kFwd ? s->fwd[layout] : which == kFp8 ? s->fp8 : s->bwd[layout];
+    out->threads = s->threads();
+    if (layout == kOffset) out->smem = sizeof(float) * (vec == 8 ? w_slots<8>(static_cast<int>(N)) : w_slots<4>(static_cast<int>(N)));
+    if (which == kBwd) {
+      const size_t wide = addnorm_wide(s->ld, vec, s->tpr) ? sizeof(float) * s->ld * vec * s->tpr : 0;
+      const size_t sums = groups > 1 ? sizeof(float) * groups * N : wide;
+      const size_t slot = static_cast<size_t>(N) * (t->size_t_ + t->size_r * (has_dh ? 2 : 1));
+      size_t ring = 0;
+      if (layout == kAligned && s->bwd_ring != nullptr) out->stages = ring_stages(slot, wide, groups, &ring);
+      if (out->stages > 0) {
+        out->fn = s->bwd_ring;
+        out->smem = std::max(ring, sums);
+      } else {
+        out->smem += sums;
+      }
+    }
+    // the widest rows off the packet boundaries: their weights and sums do not fit beside one another
+    if (out->smem > kMaxSmemPerCta - 4096) s = nullptr;
+  }
   if (s == nullptr) {
     out->fn = which == kFwd ? t->fwd_any : which == kFp8 ? t->fp8_any : t->bwd_any;
     out->threads = 512;
     out->smem = static_cast<size_t>(N) * sizeof(float);
-  } else {
-    out->fn = which == kFwd ? s->fwd[layout] : which == kFp8 ? s->fp8 : s->bwd[layout];
-    out->threads = s->threads();
-    groups = s->groups();
-    out->smem = 0;
-    if (which == kBwd) {
-      if (groups > 1) out->smem = static_cast<size_t>(groups) * N * sizeof(float);
-      else if (addnorm_wide(s->ld, vec, s->tpr)) out->smem = static_cast<size_t>(s->ld) * vec * s->tpr * sizeof(float);
-    }
+    groups = 1;
   }
   int occ;
   if (int rc = occupancy(dev, out->fn, out->threads, out->smem, &occ)) return rc;
@@ -106,7 +134,7 @@ int forward(bool fp8, const void* x, int64_t xs, const void* r, int64_t rs, cons
   if (group != 0 && group != 32 && group != 64 && group != 128)
     return fail(B200NORM_ERR_ARG, "a scale covers 32, 64 or 128 columns, or (0) a row; got %d", group);
   if (M == 0) return B200NORM_OK;
-  if (!x || !y || (fp8 && !scale) || (!fp8 && (!r || !h || !rstd))) return fail(B200NORM_ERR_ARG, "null buffer");
+  if (!x || !y || (fp8 && !scale) || (!fp8 && (!r || !h))) return fail(B200NORM_ERR_ARG, "null buffer");
   if (r == nullptr && h != nullptr) return fail(B200NORM_ERR_ARG, "h is the sum with a residual: there is none");
   if (xs < N || ys < N || (r && rs < N) || (h && hs < N)) return fail(B200NORM_ERR_ARG, "row stride smaller than N");
   DeviceState* dev = nullptr;
@@ -116,7 +144,7 @@ int forward(bool fp8, const void* x, int64_t xs, const void* r, int64_t rs, cons
   int period;
   const Layout layout = layout_of(bufs, 4, N, 16 / t->size_t_, w, &period);
   Plan pl;
-  if (int rc = plan(*dev, t, fp8 ? kFp8 : kFwd, layout, period, M, N, &pl)) return rc;
+  if (int rc = plan(*dev, t, fp8 ? kFp8 : kFwd, layout, period, M, N, r != nullptr, &pl)) return rc;
   AddNormParams p = {};
   p.x = x; p.r = r; p.w = w; p.y = y; p.h = h; p.rstd = rstd; p.scale = scale;
   p.x_stride = xs; p.r_stride = rs; p.y_stride = ys; p.h_stride = hs;
@@ -152,11 +180,12 @@ size_t b200norm_add_rms_bwd_workspace_bytes(int64_t M, int64_t N, int io_dtype, 
   if (device_caches(&dev)) return 0;
   const AddNormTable* t = table_for(io_dtype, res_dtype);
   int64_t rows = 0;
-  for (Layout layout : {kAligned, kOffset, kAny}) {  // whichever the buffers turn out to have
-    Plan pl;
-    if (plan(*dev, t, kBwd, layout, 1, M, N, &pl)) return 0;
-    rows = std::max<int64_t>(rows, pl.grid);
-  }
+  for (Layout layout : {kAligned, kOffset, kAny})  // whichever the buffers turn out to have
+    for (bool has_dh : {false, true}) {
+      Plan pl;
+      if (plan(*dev, t, kBwd, layout, 1, M, N, has_dh, &pl)) return 0;
+      rows = std::max<int64_t>(rows, pl.grid);
+    }
   return (static_cast<size_t>(rows) * N * sizeof(float) + 255) & ~static_cast<size_t>(255);
 }
 
@@ -173,19 +202,20 @@ int b200norm_add_rms_bwd(const void* h, int64_t h_row_stride, const void* dy, in
   if (h_row_stride < N || dy_row_stride < N || dx_row_stride < N || (dh && dh_row_stride < N) || (dres && dres_row_stride < N))
     return fail(B200NORM_ERR_ARG, "row stride smaller than N");
   DeviceState* dev = nullptr;
-  if (int rc = device_caches(&dev)) return rc;
+  if (int rc = device_state(&dev)) return rc;
   const AddNormTable* t = table_for(io_dtype, res_dtype);
   const Buffer bufs[5] = {{dy, dy_row_stride, t->size_t_}, {h, h_row_stride, t->size_r}, {dh, dh_row_stride, t->size_r},
                           {dx, dx_row_stride, t->size_t_}, {dres, dres_row_stride, t->size_r}};
   int period;
   const Layout layout = layout_of(bufs, 5, N, 16 / t->size_t_, w, &period);
   Plan pl;
-  if (int rc = plan(*dev, t, kBwd, layout, period, M, N, &pl)) return rc;
+  if (int rc = plan(*dev, t, kBwd, layout, period, M, N, dh != nullptr, &pl)) return rc;
   AddNormParams p = {};
   p.x = dy; p.r = dh; p.w = w; p.y = dx; p.h = const_cast<void*>(h); p.rstd = const_cast<float*>(rstd); p.dr = dres;
   p.x_stride = dy_row_stride; p.r_stride = dh_row_stride; p.y_stride = dx_row_stride; p.h_stride = h_row_stride;
   p.dr_stride = dres_row_stride;
   p.M = M; p.N = static_cast<int>(N); p.w_dtype = w_dtype;
+  p.stages = pl.stages; p.status = dev->status_dev;
   if (dw != nullptr) {
     const size_t need = static_cast<size_t>(pl.grid) * N * sizeof(float);
     if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u))
@@ -195,7 +225,9 @@ int b200norm_add_rms_bwd(const void* h, int64_t h_row_stride, const void* dy, in
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   if (int rc = launch(pl.fn, dim3(pl.grid), dim3(pl.threads), pl.smem, &p, stream)) return rc;
   if (dw == nullptr) return B200NORM_OK;
-  return launch_colreduce(p.part, pl.grid, N, dw, w_dtype, stream);
+  AddNormReduceParams c = {p.part, dw, pl.grid, static_cast<int>(N), w_dtype};
+  return launch(reinterpret_cast<const void*>(&addnorm_reduce_kernel), dim3(static_cast<unsigned>((N + 31) / 32)), dim3(1024), 0,
+                &c, stream);
 }
 
 }  // extern "C"

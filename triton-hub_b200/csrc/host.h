@@ -39,6 +39,9 @@ struct DeviceState {
 // The launch-planning part of the current device's state; allocates nothing.
 int device_caches(DeviceState** out);
 
+// The same with the device's status word for bounded waits; the first call on a device allocates it.
+int device_state(DeviceState** out);
+
 // Resident CTAs per SM of `fn` at this block size and dynamic shared memory (cluster == 1), or
 // resident clusters on the whole device (cluster > 1); cached.
 int occupancy(DeviceState& s, const void* fn, int threads, size_t smem, int* out, int cluster = 1);
@@ -47,8 +50,5 @@ int occupancy(DeviceState& s, const void* fn, int threads, size_t smem, int* out
 // before its first global access).
 int launch(const void* fn, dim3 grid, dim3 block, size_t smem, void* params, cudaStream_t stream, bool pdl = true,
            int cluster = 1);
-
-// dweight from `rows` fp32 partial rows of N columns: added in a fixed order, cast to w_dtype.
-int launch_colreduce(const float* part, int rows, int64_t N, void* dw, int w_dtype, cudaStream_t stream);
 
 }  // namespace b200norm

@@ -71,8 +71,6 @@ int device_caches(DeviceState** out) {
   return B200NORM_OK;
 }
 
-namespace {
-
 // Per-device set-up, run by the first call on each device: the launch-planning part plus the status word.
 int device_state(DeviceState** out) {
   DeviceState* s = nullptr;
@@ -89,8 +87,6 @@ int device_state(DeviceState** out) {
   return B200NORM_OK;
 }
 
-}  // namespace
-
 int occupancy(DeviceState& s, const void* fn, int threads, size_t smem, int* out, int cluster) {
   const unsigned long long key =
       (reinterpret_cast<unsigned long long>(fn) * 0x9E3779B97F4A7C15ull) ^ (unsigned long long)smem;
@@ -101,11 +97,11 @@ int occupancy(DeviceState& s, const void* fn, int threads, size_t smem, int* out
     return B200NORM_OK;
   }
   cudaError_t e;
-  // Static shared memory (up to 18 KB beside dynamic) counts toward the 48 KB default limit too.  The limit is only
+  // Static shared memory (up to 35 KB) counts toward the 48 KB default limit too.  The limit is only
   // ever raised: one kernel serves a range of row lengths, and a shorter row after a longer one must
   // not take the allowance away from a launch shape whose occupancy is already cached.
   size_t& allowed = s.smem_limit[fn];
-  if (smem > 28 * 1024 && smem > allowed) {
+  if (smem > 12 * 1024 && smem > allowed) {
     e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess)
       return fail(B200NORM_ERR_CUDA, "cudaFuncSetAttribute(%zu B): %s", smem, cudaGetErrorString(e));
@@ -219,19 +215,6 @@ int launch(const void* fn, dim3 grid, dim3 block, size_t smem, void* params, cud
   }
   if (e != cudaSuccess) return fail(B200NORM_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
   return B200NORM_OK;
-}
-
-int launch_colreduce(const float* part, int rows, int64_t N, void* dw, int w_dtype, cudaStream_t stream) {
-  ColReduceParams c;
-  c.part[0] = part; c.part[1] = nullptr;
-  c.out[0] = dw; c.out[1] = nullptr;
-  c.group_sums = nullptr;
-  c.per_shard = rows; c.row_shards = 1; c.slots = 1; c.N = static_cast<int>(N); c.w_dtype = w_dtype;
-  if (N % 4 == 0)
-    return launch(reinterpret_cast<const void*>(&colreduce4_kernel), dim3(static_cast<unsigned>((N + 127) / 128)),
-                  dim3(32, 16), 0, &c, stream);
-  return launch(reinterpret_cast<const void*>(&colreduce_kernel), dim3(static_cast<unsigned>((N + 31) / 32)),
-                dim3(32, 16), 0, &c, stream);
 }
 
 namespace {
