@@ -12,7 +12,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .functional import _code, _on_device, _ptr, _raw_stream, _require_cuda, _row_stride, _rows
+from .functional import _code, _flat, _on_device, _ptr, _raw_stream, _require_cuda
 
 _WS_BYTES = {}  # (device, T, E, k, dtype code) -> workspace bytes; the answer never changes
 
@@ -30,8 +30,7 @@ def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True):
             raise RuntimeError(f"b200norm: mask is bool, one value a token, of shape {tuple(shape)} on {device}; got "
                                f"{tuple(mask.shape)} of {mask.dtype} on {mask.device}")
         mask = mask.contiguous()
-    x = _rows(logits)
-    T, E = x.shape
+    x, T, E, xs = _flat(logits)
     gates = torch.empty((*shape, k), dtype=torch.float32, device=device)
     experts = torch.empty((*shape, k), dtype=torch.int32, device=device)
     counts = torch.empty((E + 1,), dtype=torch.int32, device=device)
@@ -47,10 +46,10 @@ def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True):
             if ws_bytes == 0:
                 _lib.check(_lib.ERR_ARG)
             _WS_BYTES[key] = ws_bytes
-        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=device)
+        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=device) if ws_bytes > 1 else None
         _lib.check(lib.b200norm_route_fwd(
-            x.data_ptr(), _row_stride(x), _ptr(mask), gates.data_ptr(), experts.data_ptr(), _ptr(lse), counts.data_ptr(),
-            loss.data_ptr(), ws.data_ptr(), ws_bytes, T, E, k, int(bool(normalize)), code, _raw_stream(index)))
+            x.data_ptr(), xs, _ptr(mask), gates.data_ptr(), experts.data_ptr(), _ptr(lse), counts.data_ptr(),
+            loss.data_ptr(), _ptr(ws), ws_bytes, T, E, k, int(bool(normalize)), code, _raw_stream(index)))
     return gates, experts, counts, loss, lse
 
 
@@ -58,23 +57,23 @@ def _route_bwd(logits, gates, experts, counts, lse, dgates, dloss, normalize=Tru
     """Gradients of (gates, loss), either of which may be None, with respect to the logits."""
     _require_cuda(logits)
     k = experts.shape[-1]
-    x = _rows(logits)
-    T, E = x.shape
+    x, T, E, xs = _flat(logits)
+    dgs = k
     for t in (dgates, dloss):
         if t is not None and t.device != logits.device:
             raise RuntimeError(f"b200norm: gradient on {t.device}, router logits on {logits.device}")
     if dgates is not None:
         assert dgates.shape == experts.shape, 'expect input and output shape to be the same'
-        dgates = _rows(dgates.to(torch.float32))
-    if dloss is not None:
+        dgates, _, _, dgs = _flat(dgates if dgates.dtype == torch.float32 else dgates.to(torch.float32))
+    if dloss is not None and dloss.dtype != torch.float32:
         dloss = dloss.to(torch.float32)
-    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    dlogits = torch.empty_like(logits) if x is logits else torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     lib = _lib.load()
     index = logits.device.index
     with _on_device(index):
         _lib.check(lib.b200norm_route_bwd(
-            x.data_ptr(), _row_stride(x), gates.data_ptr(), experts.data_ptr(), lse.data_ptr(), counts.data_ptr(),
-            _ptr(dgates), _row_stride(dgates) if dgates is not None else k, _ptr(dloss), dlogits.data_ptr(), T, E, k,
+            x.data_ptr(), xs, gates.data_ptr(), experts.data_ptr(), lse.data_ptr(), counts.data_ptr(),
+            _ptr(dgates), dgs, _ptr(dloss), dlogits.data_ptr(), T, E, k,
             int(bool(normalize)), _code(x, "router logits"), _raw_stream(index)))
     return dlogits
 
@@ -85,6 +84,13 @@ class route(torch.autograd.Function):
     tokens all of whose logits are -inf, choose nothing: experts -1, gates 0, no count, no gradient.  So do the slots
     left over when fewer than k logits of a token are above -inf.  A NaN among a live token's logits makes its gates
     and the loss NaN."""
+
+    @classmethod
+    def apply(cls, logits, k, normalize=True, mask=None):
+        if not torch.is_grad_enabled():  # nothing to record: a decode step's call is spared autograd's bookkeeping
+            gates, experts, counts, loss, _ = _route_fwd(logits, k, normalize, mask, need_lse=False)
+            return gates, experts, counts[:-1], loss
+        return super().apply(logits, k, normalize, mask)
 
     @staticmethod
     def forward(ctx, logits, k, normalize=True, mask=None):

@@ -41,7 +41,12 @@ int check(int64_t T, int E, int k, int dtype) {
   return B200NORM_OK;
 }
 
-size_t fwd_smem(int E) { return (static_cast<size_t>(kRouteWarps) * E + E + 1) * 4; }
+int columns_of(int E) { return (E + 3) / 4 * 4; }
+
+size_t fwd_smem(int E) { return (static_cast<size_t>(kRouteWarps + 1) * columns_of(E) + 1) * 4; }
+
+// Partial rows of the sums and of the counts, and the live tokens, of every CTA; 1 for the CTA that is alone.
+size_t workspace_need(int grid, int E) { return grid == 1 ? 1 : static_cast<size_t>(grid) * (2 * columns_of(E) + 1) * 4; }
 
 int fwd_grid(DeviceState& dev, const void* fn, int64_t T, int E, int* grid) {
   int occ;
@@ -64,7 +69,7 @@ size_t b200norm_route_workspace_bytes(int64_t T, int E, int k, int dtype) {
   if (device_caches(&dev)) return 0;
   int grid;
   if (fwd_grid(*dev, route_fn(dtype, E, false), T, E, &grid)) return 0;
-  return static_cast<size_t>(grid) * (2 * E + 1) * 4 + 256;
+  return workspace_need(grid, E);
 }
 
 int b200norm_route_fwd(const void* logits, int64_t row_stride, const uint8_t* mask, float* gates, int* experts, float* lse,
@@ -78,19 +83,21 @@ int b200norm_route_fwd(const void* logits, int64_t row_stride, const uint8_t* ma
   const void* fn = route_fn(dtype, E, false);
   int grid;
   if (int rc = fwd_grid(*dev, fn, T, E, &grid)) return rc;
-  const size_t need = static_cast<size_t>(grid) * (2 * E + 1) * 4;
-  if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u))
+  const size_t need = workspace_need(grid, E);
+  if (grid > 1 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
     return fail(B200NORM_ERR_ARG, "workspace needs %zu bytes, 16-byte aligned (got %zu)", need, workspace_bytes);
   RouteParams p = {};
   p.logits = logits; p.stride = row_stride; p.mask = mask; p.gates = gates; p.experts = experts; p.lse = lse;
   p.counts = counts; p.loss = loss;
   p.part_p = static_cast<float*>(workspace);
-  p.part_n = reinterpret_cast<int*>(p.part_p + static_cast<size_t>(grid) * E);
+  p.columns = columns_of(E);
+  p.part_n = reinterpret_cast<int*>(p.part_p + static_cast<size_t>(grid) * p.columns);
+  p.part_live = p.part_n + static_cast<size_t>(grid) * p.columns;
   p.T = T; p.E = E; p.k = k; p.normalize = normalize != 0; p.parts = grid;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   if (int rc = launch(fn, dim3(grid), dim3(kRouteThreads), fwd_smem(E), &p, stream)) return rc;
   if (grid == 1) return B200NORM_OK;
-  return launch(reinterpret_cast<const void*>(&route_finish_kernel), dim3(1), dim3(kRouteThreads), 0, &p, stream);
+  return launch(reinterpret_cast<const void*>(&route_finish_kernel), dim3(1), dim3(kRouteFinishThreads), 0, &p, stream);
 }
 
 int b200norm_route_bwd(const void* logits, int64_t row_stride, const float* gates, const int* experts, const float* lse,

@@ -12,8 +12,7 @@
 // fewer than k others exist, the slots left over hold -1 and gate 0.
 //
 // A warp takes a token; lane i holds the EPL neighbouring experts from i * EPL on, so the lowest of several
-// lanes with one maximum also has the lowest index.  Reading the logits is 6 us at 65536 x 128 fp32; the k
-// rounds of "maximum over the warp" are what the instructions go to.
+// lanes with one maximum also has the lowest index.
 #pragma once
 
 #include "norm_common.cuh"
@@ -36,8 +35,10 @@ struct RouteParams {
   float* lse;           // (T,) log of the softmax's denominator; -inf marks a token that is not live
   int* counts;          // (E + 1): per expert, then the number of live tokens
   float* loss;
-  float* part_p;  // (gridDim.x, E) partial sums of p
-  int* part_n;    // (gridDim.x, E + 1) partial counts
+  float* part_p;  // (gridDim.x, columns) partial sums of p
+  int* part_n;    // (gridDim.x, columns) partial counts
+  int* part_live; // (gridDim.x,) partial numbers of live tokens
+  int columns;    // E rounded up to whole 16-byte packets
   // backward
   const float* dgates;  // (T, k) or null
   int64_t dgates_stride;
@@ -87,58 +88,126 @@ __device__ __forceinline__ void load_logits(const T* row, int E, int lane, bool 
   }
 }
 
-// Sums the partial rows of all CTAs and forms counts, the number of live tokens and the loss.  Runs in one CTA of
-// `threads` threads; every column is added in CTA order.
-__device__ __forceinline__ void route_finish(const RouteParams& p, int parts, const float* part_p, const int* part_n,
-                                             double* red, int threads) {
-  const int tid = threadIdx.x;
-  __shared__ int live_s;
-  if (tid < 32) {
-    int n = 0;
-    for (int g = tid; g < parts; g += 32) n += part_n[(size_t)g * (p.E + 1) + p.E];
+// The k rounds of "maximum over the warp".  After it lane r < c holds the r-th choice (its expert in `chosen`, its
+// logit in `chosen_x`), c = the number of choices returned: fewer than k when only -inf is left.
+//
+// Up to 8 experts a lane are sorted once, descending, by exchanges of neighbours, which keep equal ones in their order;
+// a round then looks at the lanes' first keys only, and the lane that held the maximum moves its list up.  Which
+// expert it was is worked out once, after the rounds: the owner's list of indices and how often it was chosen before.
+// A round is a dozen instructions, most of them on the half-rate integer pipe, which is what bounds the kernel:
+// scanning all of a lane's keys in every round made 65536 x 128 fp32, k = 8, 56 us instead of 27.
+template <int EPL>
+__device__ __forceinline__ int route_choose(const float (&x)[EPL], int k, int lane, float& top, int& chosen, float& chosen_x) {
+  uint32_t key[EPL];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    if (tid == 0) live_s = n;
-  }
-  double share = 0.;
-  for (int e = tid; e < p.E; e += threads) {
-    float s = 0.f;
-    int n = 0;
-    for (int g = 0; g < parts; ++g) {
-      s += part_p[(size_t)g * p.E + e];
-      n += part_n[(size_t)g * (p.E + 1) + e];
+  for (int i = 0; i < EPL; ++i) key[i] = order_key(x[i]);
+  uint32_t mine = 0;
+  int r = 0;
+  if constexpr (EPL <= 8) {
+    uint32_t id[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) id[i] = i;
+#pragma unroll
+    for (int n = EPL - 1; n > 0; --n)
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const bool swap = key[i + 1] > key[i];
+        const uint32_t a = key[i], b = key[i + 1], c = id[i], d = id[i + 1];
+        key[i] = swap ? b : a;
+        key[i + 1] = swap ? a : b;
+        id[i] = swap ? d : c;
+        id[i + 1] = swap ? c : d;
+      }
+    uint32_t order = 0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) order |= id[i] << (4 * i);
+    int owner_of_mine = 64 + lane;  // lanes without a choice match nobody
+    for (; r < k; ++r) {
+      const uint32_t most = __reduce_max_sync(0xffffffffu, key[0]);
+      if (r == 0) top = key_value(most);
+      if (most <= kKeyNegInf) break;
+      const int owner = __ffs(__ballot_sync(0xffffffffu, key[0] == most)) - 1;
+      if (lane == r) {
+        mine = most;
+        owner_of_mine = owner;
+      }
+      if (lane == owner) {
+#pragma unroll
+        for (int i = 0; i + 1 < EPL; ++i) key[i] = key[i + 1];
+        key[EPL - 1] = 0u;
+      }
     }
-    p.counts[e] = n;
-    share += static_cast<double>(s) * n;
-  }
-  red[tid] = share;
-  __syncthreads();
-  if (tid >= 32) return;
-  double total = 0.;
-  for (int i = tid; i < threads; i += 32) total += red[i];
+    const int before = __popc(__match_any_sync(0xffffffffu, owner_of_mine) & ((1u << lane) - 1u));
+    const uint32_t list = __shfl_sync(0xffffffffu, order, owner_of_mine & 31);
+    if (lane < r) chosen = owner_of_mine * EPL + static_cast<int>((list >> (4 * before)) & 15u);
+  } else {
+    for (; r < k; ++r) {
+      uint32_t best = key[0];
+      int at = 0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (tid == 0) {
-    const int n = live_s;
+      for (int i = 1; i < EPL; ++i)
+        if (key[i] > best) {
+          best = key[i];
+          at = i;
+        }
+      const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+      if (r == 0) top = key_value(most);
+      if (most <= kKeyNegInf) break;
+      const int owner = __ffs(__ballot_sync(0xffffffffu, best == most)) - 1;
+      const int e = __shfl_sync(0xffffffffu, lane * EPL + at, owner);
+      if (lane == r) {
+        chosen = e;
+        mine = most;
+      }
+      if (lane == owner) {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i)
+          if (i == at) key[i] = 0u;
+      }
+    }
+  }
+  if (lane < r) chosen_x = key_value(mine);
+  return r;
+}
+
+// Counts, the number of live tokens and the loss from the sums of p and the counts of every expert: `sum(e)`, `count(e)`.
+template <int THREADS, typename Sum, typename Count>
+__device__ __forceinline__ void route_loss(const RouteParams& p, int n, Sum sum, Count count) {
+  __shared__ double red[THREADS / 32];
+  double share = 0.;
+  for (int e = threadIdx.x; e < p.E; e += THREADS) {
+    const int c = count(e);
+    p.counts[e] = c;
+    share += static_cast<double>(sum(e)) * c;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) share += __shfl_xor_sync(0xffffffffu, share, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = share;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double total = 0.;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) total += red[w];
     p.counts[p.E] = n;
     *p.loss = n > 0 ? static_cast<float>(total * p.E / (static_cast<double>(n) * n * p.k)) : 0.f;
   }
 }
 
 template <typename T, int EPL>
-__global__ void __launch_bounds__(kRouteThreads) route_fwd_kernel(const RouteParams p) {
-  extern __shared__ __align__(16) unsigned char dyn[];  // float sums[warps][E]; the counts of the CTA: int [E + 1]
+__global__ void __launch_bounds__(kRouteThreads, EPL <= 8 ? 2 : 1) route_fwd_kernel(const RouteParams p) {
+  extern __shared__ __align__(16) unsigned char dyn[];  // float sums[warps][columns]; int counts[columns + 1]
   float* sums = reinterpret_cast<float*>(dyn);
-  int* counts = reinterpret_cast<int*>(sums + (size_t)kRouteWarps * p.E);
-  __shared__ double red[kRouteThreads];
+  int* counts = reinterpret_cast<int*>(sums + (size_t)kRouteWarps * p.columns);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int e = threadIdx.x; e <= p.E; e += kRouteThreads) counts[e] = 0;
+  for (int e = threadIdx.x; e <= p.columns; e += kRouteThreads) counts[e] = 0;
   __syncthreads();
   grid_dependency_sync();
   trigger_dependents();
 
   const T* logits = static_cast<const T*>(p.logits);
   const bool packed = p.E % EPL == 0 && (reinterpret_cast<uintptr_t>(logits) & 15u) == 0 && (p.stride * sizeof(T)) % 16 == 0;
+  int group = 1;  // lanes over which the gates are summed: a power of two, at least k
+  while (group < p.k) group *= 2;
   float acc[EPL];
 #pragma unroll
   for (int i = 0; i < EPL; ++i) acc[i] = 0.f;
@@ -154,40 +223,9 @@ __global__ void __launch_bounds__(kRouteThreads) route_fwd_kernel(const RoutePar
     if (tok + step < p.T) load_logits<T, EPL>(logits + (tok + step) * p.stride, p.E, lane, packed, nx);
     const bool masked = p.mask != nullptr && p.mask[tok] == 0;
 
-    uint32_t key[EPL];
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) key[i] = order_key(x[i]);
-    float top = 0.f;
+    float top = 0.f, chosen_x = 0.f;
     int chosen = -1;
-    float chosen_x = 0.f;
-    bool live = !masked;
-    for (int r = 0; r < p.k; ++r) {
-      uint32_t best = key[0];
-      int at = 0;
-#pragma unroll
-      for (int i = 1; i < EPL; ++i)
-        if (key[i] > best) {
-          best = key[i];
-          at = i;
-        }
-      const uint32_t most = __reduce_max_sync(0xffffffffu, best);
-      if (r == 0) {
-        top = key_value(most);
-        live = live && most > kKeyNegInf;
-      }
-      if (most <= kKeyNegInf) break;  // only -inf is left
-      const int owner = __ffs(__ballot_sync(0xffffffffu, best == most)) - 1;
-      const int e = __shfl_sync(0xffffffffu, lane * EPL + at, owner);
-      if (lane == r) {
-        chosen = e;
-        chosen_x = key_value(most);
-      }
-      if (lane == owner) {
-#pragma unroll
-        for (int i = 0; i < EPL; ++i)
-          if (i == at) key[i] = 0u;
-      }
-    }
+    const bool live = route_choose<EPL>(x, p.k, lane, top, chosen, chosen_x) > 0 && !masked;
 
     float s = 0.f;
 #pragma unroll
@@ -197,12 +235,16 @@ __global__ void __launch_bounds__(kRouteThreads) route_fwd_kernel(const RoutePar
     }
     s = warp_sum(s);
     float gate = chosen >= 0 ? expf(chosen_x - top) : 0.f;
-    const float total = p.normalize ? warp_sum(gate) : s;
-    gate = live && chosen >= 0 ? gate / total : 0.f;
+    float total = s;
+    if (p.normalize) {
+      total = gate;
+      for (int o = 1; o < group; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
     if (lane < p.k) {
-      p.gates[tok * p.k + lane] = gate;
-      p.experts[tok * p.k + lane] = live ? chosen : -1;
-      if (live && chosen >= 0) atomicAdd(&counts[chosen], 1);
+      const bool choice = live && chosen >= 0;
+      p.gates[tok * p.k + lane] = choice ? gate / total : 0.f;
+      p.experts[tok * p.k + lane] = choice ? chosen : -1;
+      if (choice) atomicAdd(&counts[chosen], 1);
     }
     if (p.lse != nullptr && lane == 0) p.lse[tok] = live ? top + logf(s) : -INFINITY;
     if (live) {
@@ -212,33 +254,73 @@ __global__ void __launch_bounds__(kRouteThreads) route_fwd_kernel(const RoutePar
       for (int i = 0; i < EPL; ++i) acc[i] = fmaf(x[i], inv, acc[i]);
     }
   }
-  if (lane == 0) atomicAdd(&counts[p.E], live_tokens);
+  if (lane == 0) atomicAdd(&counts[p.columns], live_tokens);
 #pragma unroll
   for (int i = 0; i < EPL; ++i)
-    if (lane * EPL + i < p.E) sums[(size_t)warp * p.E + lane * EPL + i] = acc[i];
+    if (lane * EPL + i < p.columns) sums[(size_t)warp * p.columns + lane * EPL + i] = acc[i];
   __syncthreads();
-  float* out_p = p.part_p + (size_t)blockIdx.x * p.E;
-  int* out_n = p.part_n + (size_t)blockIdx.x * (p.E + 1);
-  const bool alone = gridDim.x == 1;  // a single CTA finishes by itself: no second launch
-  for (int e = threadIdx.x; e < p.E; e += kRouteThreads) {
+  auto cta_sum = [&](int e) {
     float s = 0.f;
-    for (int w = 0; w < kRouteWarps; ++w) s += sums[(size_t)w * p.E + e];
-    if (alone) sums[e] = s;  // row 0 of a column is read and written by one thread only
-    else out_p[e] = s;
+#pragma unroll
+    for (int w = 0; w < kRouteWarps; ++w) s += sums[(size_t)w * p.columns + e];
+    return s;
+  };
+  if (gridDim.x == 1) {  // a single CTA finishes by itself: no second launch
+    route_loss<kRouteThreads>(p, counts[p.columns], cta_sum, [&](int e) { return counts[e]; });
+    return;
   }
-  if (alone) {
-    __syncthreads();
-    route_finish(p, 1, sums, counts, red, kRouteThreads);
-  } else {
-    for (int e = threadIdx.x; e <= p.E; e += kRouteThreads) out_n[e] = counts[e];
+  for (int e = threadIdx.x; e < p.columns; e += kRouteThreads) {
+    p.part_p[(size_t)blockIdx.x * p.columns + e] = e < p.E ? cta_sum(e) : 0.f;
+    p.part_n[(size_t)blockIdx.x * p.columns + e] = counts[e];
   }
+  if (threadIdx.x == 0) p.part_live[blockIdx.x] = counts[p.columns];
 }
 
-__global__ void __launch_bounds__(kRouteThreads) route_finish_kernel(const RouteParams p) {
-  __shared__ double red[kRouteThreads];
+// Adds the CTAs' partial rows, 16 bytes a thread and up to 32 rows side by side, every column in one fixed order.
+constexpr int kRouteFinishThreads = 1024;
+__global__ void __launch_bounds__(kRouteFinishThreads) route_finish_kernel(const RouteParams p) {
+  __shared__ float4 sum_s[kRouteFinishThreads];
+  __shared__ int4 count_s[kRouteFinishThreads];
+  __shared__ int live_s;
+  const int tid = threadIdx.x;
+  const int quads = p.columns / 4, groups = min(32, kRouteFinishThreads / quads);
+  const int q = tid % quads, g = tid / quads;
   grid_dependency_sync();
   trigger_dependents();
-  route_finish(p, p.parts, p.part_p, p.part_n, red, kRouteThreads);
+  if (g < groups) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    int4 n = make_int4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int r = g; r < p.parts; r += groups) {
+      const float4 a = *reinterpret_cast<const float4*>(p.part_p + (size_t)r * p.columns + 4 * q);
+      const int4 b = *reinterpret_cast<const int4*>(p.part_n + (size_t)r * p.columns + 4 * q);
+      s.x += a.x; s.y += a.y; s.z += a.z; s.w += a.w;
+      n.x += b.x; n.y += b.y; n.z += b.z; n.w += b.w;
+    }
+    sum_s[g * quads + q] = s;
+    count_s[g * quads + q] = n;
+  }
+  if (tid < 32) {
+    int n = 0;
+    for (int r = tid; r < p.parts; r += 32) n += p.part_live[r];
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (tid == 0) live_s = n;
+  }
+  __syncthreads();
+  const float* sums = reinterpret_cast<const float*>(sum_s);
+  const int* counts = reinterpret_cast<const int*>(count_s);
+  route_loss<kRouteFinishThreads>(
+      p, live_s,
+      [&](int e) {
+        float s = 0.f;
+        for (int r = 0; r < groups; ++r) s += sums[(size_t)r * p.columns + e];
+        return s;
+      },
+      [&](int e) {
+        int n = 0;
+        for (int r = 0; r < groups; ++r) n += counts[(size_t)r * p.columns + e];
+        return n;
+      });
 }
 
 // Backward: p comes from the logits and the saved log-sum, the chosen experts' part is put in its place
