@@ -50,7 +50,7 @@ def check(x, u, **kw):
     assert got.dtype == torch.int64 and got.shape == u.shape
     want = reference(x.reshape(-1, x.shape[-1]), u.reshape(-1), **{k: v.reshape(-1) if isinstance(v, torch.Tensor) else v
                                                                     for k, v in kw.items()})
-    assert torch.equal(got.reshape(-1), want)
+    assert torch.equal(got.reshape(-1), want), (kw, got.tolist()[:16], want.tolist()[:16])
 
 
 SETTINGS = [dict(), dict(temperature=0.6), dict(temperature=0.0), dict(top_k=1), dict(top_k=5), dict(top_k=50, temperature=1.7),
@@ -134,9 +134,37 @@ def test_masked_and_extreme_logits(dtype):
     x[8] = x[8] * 1e-3
     x[9] = -x[9].abs() - 1
     x[10, 8] = -float("nan")
+    x[11] = -INF                            # the lowest number is the maximum, beside -inf
+    x[11, 40:50] = torch.finfo(dtype).min
     for kw in SETTINGS:
         check(x, u, **kw)
     assert b200norm.sample(x, u)[[0, 1, 2, 10]].tolist() == [0, -1, -1, -1]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_offsets_and_extreme_temperatures(dtype):
+    # logits far from zero, where a step of fp32 is larger than the temperature, and temperatures at both ends
+    x, u = make(6, 5000, dtype, seed=8)
+    for offset in (1e4, -1e4, 1e10, -1e10, 3e38, -3e38):
+        y = (x.float() + offset).to(dtype)
+        for kw in (dict(), dict(top_p=0.7), dict(top_k=30, min_p=0.1), dict(temperature=0.01), dict(top_p=0.5, temperature=20.0)):
+            check(y, u, **kw)
+    x[:, ::9] = -INF
+    for t in (1e-30, 1e-3, 1e3, 1e35):
+        check(x, u, temperature=t)
+        check(x, u, temperature=t, top_k=700, top_p=0.6)
+        check(x, u, temperature=t, min_p=0.5, top_p=0.9)
+
+
+def test_wide_prefixes():
+    # neither list nor bin holds few tokens: flat rows, many equal logits, top-k beyond the list
+    g = torch.Generator(device=DEV).manual_seed(3)
+    u = torch.rand(8, generator=g, device=DEV)
+    flat = torch.rand(8, 100000, generator=g, device=DEV) * 0.01
+    for x in (flat, flat.bfloat16(), flat * 1e-4 - 7, (flat * 300).round()):
+        for kw in (dict(top_p=0.9), dict(top_k=3000), dict(top_k=99999, top_p=0.999), dict(top_k=600, top_p=0.4, min_p=0.5),
+                   dict(top_k=257), dict(top_k=255), dict(top_p=1e-3), dict(top_k=513, top_p=0.999999)):
+            check(x, u, **kw)
 
 
 def test_uniform_at_its_ends():

@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .functional import _code, _on_device, _ptr, _raw_stream, _require_cuda, _row_stride, _rows
+from .functional import _code, _flat, _on_device, _ptr, _raw_stream, _require_cuda
 
 
 def _setting(value, name, shape, device, dtype, low, high):
@@ -52,12 +52,11 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     p_v, p = _setting(top_p, "top_p", shape, device, torch.float32, 0.0, 1.0)
     m_v, m = _setting(min_p, "min_p", shape, device, torch.float32, 0.0, 1.0)
     tokens = torch.empty(shape, dtype=torch.int64, device=device)
-    u = uniform.to(torch.float32).contiguous()
-    x = _rows(logits.detach())
-    M, V = x.shape
+    u = uniform if uniform.dtype == torch.float32 and uniform.is_contiguous() else uniform.to(torch.float32).contiguous()
+    x, M, V, xs = _flat(logits)
     lib = _lib.load()
     with _on_device(device.index):
-        _lib.check(lib.b200norm_sample(x.data_ptr(), _row_stride(x), u.data_ptr(), _ptr(t_v), t, _ptr(k_v), k, _ptr(p_v), p,
+        _lib.check(lib.b200norm_sample(x.data_ptr(), xs, u.data_ptr(), _ptr(t_v), t, _ptr(k_v), k, _ptr(p_v), p,
                                        _ptr(m_v), m, tokens.data_ptr(), M, V, code, _raw_stream(device.index)))
     return tokens
 
