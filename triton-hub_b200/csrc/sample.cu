@@ -38,10 +38,12 @@ extern "C" int b200norm_sample(const void* logits, int64_t row_stride, const flo
   DeviceState* dev = nullptr;
   if (int rc = device_caches(&dev)) return rc;
   const int es = dtype == B200NORM_F32 ? 4 : 2, vec = 16 / es;
-  // CTAs per row: parts of at most 64 KB, so that two or three CTAs share an SM and one's barriers hide behind
-  // another's arithmetic; and with few rows as many as there are SMs, while a part keeps 4096 tokens.
+  // CTAs per row: as few as let two of them share an SM's 228 KB (1 KB of it reserved per CTA, 14 KB static), so that one's
+  // barriers hide behind the other's arithmetic; and with few rows as many as there are SMs, while a part keeps 4096
+  // tokens.
+  constexpr int64_t kPart = 98 * 1024;
   int cluster = 1;
-  while (cluster < kSampleMaxCluster && V * es > (int64_t)cluster * 65536) cluster *= 2;
+  while (cluster < kSampleMaxCluster && V * es > cluster * kPart) cluster *= 2;
   while (cluster < kSampleMaxCluster && M * cluster * 2 <= dev->sm_count && V >= (int64_t)cluster * 2 * 4096) cluster *= 2;
   SampleParams p = {};
   p.logits = logits; p.stride = row_stride; p.uniform = uniform;
@@ -50,8 +52,9 @@ extern "C" int b200norm_sample(const void* logits, int64_t row_stride, const flo
   p.top_p_v = top_p_v; p.top_p = top_p;
   p.min_p_v = min_p_v; p.min_p = min_p;
   p.tokens = tokens; p.M = M; p.V = static_cast<int>(V);
-  const int64_t per = (V + cluster - 1) / cluster;
-  p.chunk = static_cast<int>((per + vec - 1) / vec * vec);
+  // whole packets, of a row that may start and end inside one
+  const int64_t packets = (V + 2 * vec - 2) / vec;
+  p.chunk = static_cast<int>((packets + cluster - 1) / cluster * vec);
   const size_t smem = static_cast<size_t>(p.chunk) * es;
   const void* fn = dtype == B200NORM_F32 ? sample_fn<float>(cluster)
                    : dtype == B200NORM_F16 ? sample_fn<__half>(cluster) : sample_fn<__nv_bfloat16>(cluster);

@@ -15,7 +15,7 @@
 // rare token's width.
 //
 // Nothing is sorted.  The first k and the shortest prefix are thresholds in the order -- a logit and, among the
-// tokens of that very logit, a number of them -- and a histogram over bins of 1/64 below the maximum tells in
+// tokens of that very logit, a number of them -- and a histogram over bins of 1/32 below the maximum tells in
 // which bin a threshold lies and how much lies before it.
 //   - When the bins down to it hold few tokens (the usual case of a peaked distribution or a small k), these are
 //     listed, and one CTA finishes on the list by comparing its tokens pairwise.
@@ -33,13 +33,12 @@ namespace b200norm {
 
 constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
-constexpr int kSampleBins = 2048;  // four a thread
+constexpr int kSampleBins = 2 * kSampleThreads;  // two a thread
 constexpr int kSampleMaxVocab = 1 << 18;
 constexpr int kSampleMaxCluster = 8;
-constexpr float kSampleBinsPerUnit = 64.f;
-// Tokens that are compared pairwise: all that may be drawn from, or those of a threshold's bin.  512^2 comparisons are
-// 1024 a thread, about as long as two further histograms.
-constexpr int kSampleFinish = 256, kSampleList = 512;
+constexpr float kSampleBinsPerUnit = 32.f;
+constexpr int kSampleBound = 8192;  // a CTA with so many tokens bounds top-k's threshold before it counts
+constexpr int kSampleList = 256;  // tokens that are compared pairwise: all that may be drawn, or those of a threshold's bin
 
 struct SampleParams {
   const void* logits;
@@ -52,7 +51,7 @@ struct SampleParams {
   int64_t* tokens;  // (M,)
   int64_t M;
   int V;
-  int chunk;  // tokens of a row that a CTA holds: a multiple of 16 bytes
+  int chunk;  // tokens of a row that a CTA holds: whole 16-byte packets
 };
 
 using u64 = unsigned long long;
@@ -85,15 +84,19 @@ __device__ __forceinline__ float key_logit(uint32_t k) {
 // below the maximum weigh less than 2^-60, which rounds to 0, like -inf.
 struct Weigh {
   double top, scale;    // y = (x - top) * scale: exactly 0 at the maximum, whose weight is exactly 2^44
-  float least;          // logits down from here weigh nothing
+  float least;          // 42 to 64 temperatures below the maximum; lower logits count as this one
   const double* table;  // 2^(i / 16)
 
-  __device__ __forceinline__ u64 operator()(float x) const {
-    const double y = x > least ? (static_cast<double>(x) - top) * scale : -976.;
-    constexpr double kMagic = 6755399441055744.;  // 1.5 * 2^52: adding it rounds to an integer
+  // 256 + the weight, in units of 2^-44: 256 has just that ulp, so the addition rounds the weight, and the fraction field
+  // of the sum is the integer wanted.
+  static constexpr u64 kBias = 0x4070000000000000ull;
+  static constexpr double kMagic = 6755399441055744.;  // 1.5 * 2^52: adding it rounds to an integer
+  __device__ __forceinline__ u64 biased(float x, int& bin) const {
+    const double y = (static_cast<double>(fmaxf(x, least)) - top) * scale;
     const double t = y + kMagic;
     const int n = __double2loint(t);
     const double g = y - (t - kMagic);
+    bin = -2 * n - (g > 0. ? 1 : 0);
     double e = 1.2716085030349987e-09;
     e = fma(e, g, 1.467644462189871e-07);
     e = fma(e, g, 1.355080777749983e-05);
@@ -102,8 +105,17 @@ struct Weigh {
     e = fma(e, g, 1.0000000000000044);
     e *= table[n & 15];
     const double w = __hiloint2double(__double2hiint(e) + ((n >> 4) << 20), __double2loint(e));
-    // 256 has an ulp of 2^-44: the sum's fraction field is the rounded weight
-    return static_cast<u64>(__double_as_longlong(w + 256.)) & ((1ull << 52) - 1);
+    return static_cast<u64>(__double_as_longlong(w + 256.));
+  }
+  __device__ __forceinline__ u64 operator()(float x) const {
+    int n;
+    return biased(x, n) - kBias;
+  }
+  // The number, 0 at the maximum, of the token's bin: floor(-2 y), bins in which weights differ by at most 2^(1/32).
+  __device__ __forceinline__ int bin_of(float x) const {
+    int bin;
+    biased(x, bin);
+    return bin;
   }
 };
 
@@ -123,18 +135,24 @@ __device__ __forceinline__ u64 warp_scan64(u64 v, int lane) {  // inclusive
 
 template <int C>
 struct SampleShared {
-  uint32_t lo[kSampleBins], hi[kSampleBins];  // a bin's weight (64 bits in two words) or, in lo, its count
+  union {
+    uint32_t bin[3][kSampleBins];  // a bin's weight or count: lo + (mid << 16) + (hi << 32)
+    struct {
+      u64 list[kSampleList];                       // this CTA's listed tokens: key, index
+      u64 item[kSampleList], amount[kSampleList];  // the row's listed tokens
+      u64 weight[C * kSampleWarps];     // per warp segment of the row: weight above the threshold ...
+      uint32_t ties[C * kSampleWarps];  // ... and number of tokens at it
+    };
+  };
+  float pending[kSampleWarps][32];  // logits that a warp has put side by side
   double table[16];
   u64 warp_total[kSampleWarps];
-  float top[C];                  // per CTA: the largest logit
-  u64 weight[C * kSampleWarps];  // per warp segment of the row: weight above the threshold ...
-  uint32_t ties[C * kSampleWarps];  // ... and number of tokens at it
-  u64 list[kSampleList];            // this CTA's listed tokens: key, index
-  u64 item[kSampleList], amount[kSampleList];  // the row's listed tokens
-  float pending[kSampleWarps][64];             // kept logits a warp has yet to weigh
-  u64 found_above, rest;
+  float top[C];                     // per CTA: the largest logit
+  u64 slice[2][C];  // per CTA: the sum of its share of the bins, and the tokens in them
+  u64 found_above, found_here, found_tokens, rest;
   uint32_t found_key;
-  int found_bin, down_to, inside, segment, budget, listed;
+  int found_bin, segment, budget, listed;
+  float warp_float[kSampleWarps];
 };
 
 template <int C>
@@ -179,81 +197,241 @@ __device__ __forceinline__ u64 block_scan64(u64 v, u64* totals, int warp, int la
 template <typename T, int C>
 struct Row {
   static constexpr int VEC = Pack16<T>::kElems;
-  const uint4* packets;  // this CTA's part, in shared memory; past the row's end -inf
+  const uint4* packets;  // this CTA's part, in shared memory; -inf outside the row
   int n;                 // packets
-  int rank, chunk;
+  int seg;               // packets of a warp segment: warp w takes packets w * seg ... of the part
+  int rank;
+  int first;             // token index of this part's first element
   SampleShared<C>* sh;
-  float top;
+  float top, temperature;
   Weigh weigh;
   int tid, lane, warp;
 
-  // f(value, index in the chunk) for every element of packets begin .. end - 1, each by one of `threads` threads
-  template <typename F>
-  __device__ __forceinline__ void each(int begin, int end, int first, int threads, F f) const {
-    for (int i = begin + first; i < end; i += threads) {
-      union { uint4 q; T v[VEC]; } u;
-      u.q = ld_shared16(packets + i);
+  // The part's i-th four values; -inf past its end.
+  __device__ __forceinline__ void four(int i, float (&x)[4]) const {
+    if (i >= n * (VEC / 4)) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) f(u.v[e], i * VEC + e);
+      for (int e = 0; e < 4; ++e) x[e] = -INFINITY;
+    } else if constexpr (VEC == 4) {
+      Pack16<T>::unpack(ld_shared16(packets + i), x);
+    } else {
+      union { uint2 q; T v[4]; } u;
+      u.q = reinterpret_cast<const uint2*>(packets)[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = to_f32(u.v[e]);
     }
   }
-
-  __device__ __forceinline__ int bin_of(float x) const {  // bins of equal width below the maximum; monotone in x
-    return static_cast<int>(fminf((top - x) * kSampleBinsPerUnit, static_cast<float>(kSampleBins - 1)));
+  // f(four values) for every four of packets begin .. end - 1, each by one of `threads` threads
+  template <typename F>
+  __device__ __forceinline__ void each_four(int begin, int end, int first, int threads, F f) const {
+    constexpr int PARTS = VEC / 4;
+    for (int i = begin * PARTS + first; i < end * PARTS; i += threads) {
+      float x[4];
+      four(i, x);
+      f(x);
+    }
+  }
+  // f(value, index in the part) for every element.  One element a turn: the passes that use it rarely do more than compare,
+  // run once, and would spend longer fetching unrolled instructions than executing them.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    const T* values = reinterpret_cast<const T*>(packets);
+#pragma unroll 1
+    for (int i = tid; i < n * VEC; i += kSampleThreads) f(values[i], i);
   }
 
-  __device__ __forceinline__ void clear_bins(bool weights) const {
-    for (int i = tid; i < kSampleBins / 4; i += kSampleThreads) {
-      reinterpret_cast<uint4*>(sh->lo)[i] = make_uint4(0, 0, 0, 0);
-      if (weights) reinterpret_cast<uint4*>(sh->hi)[i] = make_uint4(0, 0, 0, 0);
+  // Tokens that few lanes of a warp have are put side by side and handed on 32 at a time: push(x, keep) by the whole warp,
+  // then drain().  f(x, valid) is called by the whole warp.
+  template <typename F>
+  struct Side {
+    float* slots;
+    int lane, waiting;
+    F f;
+    __device__ __forceinline__ void push(float x, bool keep) {
+      const uint32_t kept = __ballot_sync(0xffffffffu, keep);
+      if (kept == 0) return;
+      const int at = waiting + __popc(kept & ((1u << lane) - 1u));
+      if (keep && at < 32) slots[at] = x;
+      waiting += __popc(kept);
+      if (waiting < 32) return;
+      __syncwarp();
+      const float full = slots[lane];
+      __syncwarp();
+      if (keep && at >= 32) slots[at - 32] = x;
+      waiting -= 32;
+      f(full, true);
     }
+    __device__ __forceinline__ void drain() {
+      __syncwarp();
+      f(slots[lane], lane < waiting);
+      __syncwarp();
+    }
+  };
+  template <typename F>
+  __device__ __forceinline__ Side<F> side(F f) const {
+    return Side<F>{sh->pending[warp], lane, 0, f};
+  }
+
+  // The bin of a token, monotone in its logit: of counts by the distance from the maximum, of weights by the weight.  The
+  // last one takes all that follows.
+  template <bool WEIGHT>
+  __device__ __forceinline__ int bin_of(float x) const {
+    if constexpr (WEIGHT) return min(weigh.bin_of(x), kSampleBins - 1);
+    else return static_cast<int>(fminf((top - x) * kSampleBinsPerUnit, static_cast<float>(kSampleBins - 1)));
+  }
+  // A logit below which no token of bins 0 .. b lies (fp32 errs by far less than half a bin).
+  template <bool WEIGHT>
+  __device__ __forceinline__ float bin_end(int b) const {
+    if (b >= kSampleBins - 1) return -INFINITY;
+    const float width = WEIGHT ? temperature * (0.69314718f / 32.f) : 1.f / kSampleBinsPerUnit;
+    return top - width * static_cast<float>(b + 2) - 1e-5f * fabsf(top);
+  }
+
+  __device__ __forceinline__ void clear_bins() const {
+    #pragma unroll
+    for (int k = 0; k < 3; ++k) reinterpret_cast<u64*>(sh->bin[k])[tid] = 0ull;
     __syncthreads();
   }
+  // 16 bits of a weight at a time, so that 2^16 tokens leave no carry and no addition has to return what it found: that is
+  // several times as fast as a 64-bit addition, or a 32-bit one whose carry is looked for.
+  __device__ __forceinline__ void add_to_bin(int b, u64 w) const {
+    const uint32_t l = static_cast<uint32_t>(w), h = static_cast<uint32_t>(w >> 32);
+    atomicAdd(&sh->bin[0][b], l & 0xffffu);
+    atomicAdd(&sh->bin[1][b], l >> 16);
+    if (h) atomicAdd(&sh->bin[2][b], h);
+  }
+  // The weights of the tokens above `floor`, or the counts of all, into bins 0 .. last; what lies beyond goes to the last bin
+  // of all as one sum.
   template <bool WEIGHT>
-  __device__ __forceinline__ void add_to_bin(int b, float x) const {
+  __device__ __forceinline__ void fill_bins(float floor, int last) const {
+    clear_bins();
+    u64 beyond = 0;
     if constexpr (WEIGHT) {
-      const u64 w = weigh(x);
-      if (w == 0) return;
-      // 64-bit addition in two native 32-bit ones: the low word's carry joins the high word
-      const uint32_t wl = static_cast<uint32_t>(w);
-      const uint32_t old = atomicAdd(&sh->lo[b], wl);
-      const uint32_t wh = static_cast<uint32_t>(w >> 32) + (old + wl < old ? 1u : 0u);
-      if (wh) atomicAdd(&sh->hi[b], wh);
+      each_four(0, n, tid, kSampleThreads, [&](const float (&x)[4]) {
+        // all weights first, without a branch between: their chains of fp64 instructions overlap
+        u64 w[4];
+        int b[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w[e] = weigh.biased(x[e], b[e]) - Weigh::kBias;
+          w[e] = x[e] > floor ? w[e] : 0ull;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (b[e] <= last) add_to_bin(b[e], w[e]);
+          else beyond += w[e];
+        }
+      });
     } else {
-      atomicAdd(&sh->lo[b], 1u);
+      const float end = static_cast<float>(last + 1) * (1.f / kSampleBinsPerUnit);
+      each_four(0, n, tid, kSampleThreads, [&](const float (&x)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // the scale of the bins is a power of two: the comparison is that of the bin numbers
+          if (top - x[e] < end) atomicAdd(&sh->bin[0][bin_of<false>(x[e])], 1u);
+          else ++beyond;
+        }
+      });
     }
+    beyond = warp_sum64(beyond);
+    if (lane == 0) add_to_bin(kSampleBins - 1, beyond);
   }
-  // This thread's four bins, summed over the row's CTAs.  Behind it a row_sync is due before the bins change.
-  template <bool WEIGHT>
-  __device__ __forceinline__ void read_bins(u64 (&bin)[4]) const {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bin[i] = 0;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      uint4 l, h = make_uint4(0, 0, 0, 0);
-      if constexpr (C == 1) {
-        l = reinterpret_cast<const uint4*>(sh->lo)[tid];
-        if (WEIGHT) h = reinterpret_cast<const uint4*>(sh->hi)[tid];
-      } else {
-        l = ld_cluster16(cluster_map(smem_addr(&sh->lo[4 * tid]), c));
-        if (WEIGHT) h = ld_cluster16(cluster_map(smem_addr(&sh->hi[4 * tid]), c));
-      }
-      bin[0] += (static_cast<u64>(h.x) << 32) + l.x;
-      bin[1] += (static_cast<u64>(h.y) << 32) + l.y;
-      bin[2] += (static_cast<u64>(h.z) << 32) + l.z;
-      bin[3] += (static_cast<u64>(h.w) << 32) + l.w;
-    }
+  __device__ __forceinline__ static u64 bin_sum(u64 lo, u64 mid, u64 hi) { return lo + (mid << 16) + (hi << 32); }
+  // An upper bound for the number of tokens with a weight in a bin: its sum over the least that one of them weighs.  Where that
+  // is a few units it says nothing.
+  __device__ __forceinline__ static u64 most_tokens(int b, u64 sum) {
+    const float unit = exp2f(44.f - static_cast<float>(b + 1) / 32.f) * 0.999f;
+    return sum == 0 ? 0ull : unit < 4096.f ? 1ull << 20 : static_cast<u64>(static_cast<float>(sum) / unit);
   }
-  // The bin in which the running sum, `before` ahead of this thread's bins, reaches `need`: into found_bin, found_above.
-  __device__ __forceinline__ void find_bin(const u64 (&bin)[4], u64 before, u64 need) const {
+  // The bin in which the running sum over the bins, `above` ahead of them, reaches what need_of(their total) says: into
+  // found_bin, found_above (what lies before it), found_here and (TOKENS) found_tokens, an upper bound for the tokens down to
+  // it.  It synchronises the row before and after: all CTAs' tokens are in the bins, and the bins may change again.  Each
+  // CTA sums its share of the bins over the row.  MINE: this CTA's bins alone.
+  template <bool TOKENS, bool MINE = C == 1, typename Need>
+  __device__ __forceinline__ void locate(u64 above, Need need_of) const {
+    constexpr int PER = MINE ? 2 : 1, SHARE = MINE ? kSampleBins : kSampleBins / C;  // bins a thread, a CTA
+    u64 sum[PER], tokens[PER];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (before < need && before + bin[i] >= need) {
-        sh->found_bin = 4 * tid + i;
-        sh->found_above = before;
+    for (int i = 0; i < PER; ++i) sum[i] = tokens[i] = 0;
+    if constexpr (MINE) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int b = PER * tid + i;
+        sum[i] = bin_sum(sh->bin[0][b], sh->bin[1][b], sh->bin[2][b]);
       }
-      before += bin[i];
+    } else {
+      row_sync<C>();
+      if (tid < SHARE) {
+        u64 part[3] = {0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int k = 0; k < 3; ++k)
+            part[k] += static_cast<uint32_t>(ld_cluster_i32(cluster_map(smem_addr(&sh->bin[k][rank * SHARE + tid]), c)));
+        sum[0] = bin_sum(part[0], part[1], part[2]);
+      }
     }
+    const int first_bin = MINE ? PER * tid : rank * SHARE + tid;
+    u64 own = 0, own_tokens = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      own += sum[i];
+      if (TOKENS) tokens[i] = most_tokens(first_bin + i, sum[i]);
+      own_tokens += tokens[i];
+    }
+    auto scan = [&](u64 v, u64& total) {
+      const u64 before = block_scan64(v, sh->warp_total, warp, lane);
+      total = 0;
+#pragma unroll
+      for (int k = 0; k < kSampleWarps; ++k) total += sh->warp_total[k];
+      return before;
+    };
+    u64 total, all_tokens = 0;
+    u64 before = scan(own, total), tokens_before = TOKENS ? scan(own_tokens, all_tokens) : 0ull;
+    if constexpr (!MINE) {
+      if (tid < C) {  // thread c tells CTA c
+        st_cluster_u64(cluster_map(smem_addr(&sh->slice[0][rank]), tid), total);
+        st_cluster_u64(cluster_map(smem_addr(&sh->slice[1][rank]), tid), all_tokens);
+      }
+      row_sync<C>();
+      total = 0;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const u64 v = sh->slice[0][c];
+        total += v;
+        if (c < rank) {
+          before += v;
+          tokens_before += sh->slice[1][c];
+        }
+      }
+    }
+    const u64 need = need_of(total);
+    before += above;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (before < need && before + sum[i] >= need) {
+        const int b = first_bin + i;
+        if constexpr (MINE) {
+          sh->found_bin = b;
+          sh->found_above = before;
+          sh->found_here = sum[i];
+          sh->found_tokens = tokens_before + tokens[i];
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < C; ++c) {
+            st_cluster_u32(cluster_map(smem_addr(&sh->found_bin), c), static_cast<uint32_t>(b));
+            st_cluster_u64(cluster_map(smem_addr(&sh->found_above), c), before);
+            st_cluster_u64(cluster_map(smem_addr(&sh->found_here), c), sum[i]);
+            st_cluster_u64(cluster_map(smem_addr(&sh->found_tokens), c), tokens_before + tokens[i]);
+          }
+        }
+      }
+      before += sum[i];
+      tokens_before += tokens[i];
+    }
+    if constexpr (MINE) __syncthreads();
+    else row_sync<C>();
   }
 
   // Lists the row's tokens that `pred` takes.  Returns how many there are; if they are at most kSampleList, the CTAs for
@@ -262,10 +440,10 @@ struct Row {
   __device__ __forceinline__ int gather(bool all, Pred pred) const {
     if (tid == 0) sh->listed = 0;
     __syncthreads();
-    each(0, n, tid, kSampleThreads, [&](T v, int i) {
-      if (!pred(to_f32(v))) return;
+    each([&](T v, int i) {
+      if (!pred(v, to_f32(v))) return;
       const int at = atomicAdd(&sh->listed, 1);
-      if (at < kSampleList) sh->list[at] = (static_cast<u64>(token_key(v)) << 32) | static_cast<uint32_t>(rank * chunk + i);
+      if (at < kSampleList) sh->list[at] = (static_cast<u64>(token_key(v)) << 32) | static_cast<uint32_t>(first + i);
     });
     row_sync<C>();
     int total = 0, from[C + 1];
@@ -293,74 +471,81 @@ struct Threshold {
   u64 ties;
 };
 
-// The threshold within bin found_bin of the first histogram, found_above lying before it: by comparing the bin's tokens
-// pairwise if `few` says that they are not too many, by finer histograms otherwise.  Amounts are weights, of the tokens
-// above `floor`, or (WEIGHT false) counts of all.  Every CTA of the row gets the result.
+// Threads that share a token of a list of n in pairwise comparisons: a power of two, 2 to 16.
+__device__ __forceinline__ int list_share(int n) { return n <= 32 ? 16 : n <= 64 ? 8 : n <= 128 ? 4 : 2; }
+template <typename V>
+__device__ __forceinline__ V share_sum(V v, int share) {
+  for (int o = 1; o < share; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The threshold within bin found_bin of the first histogram, found_above lying before it: by finer histograms, over ranges of
+// the order-preserving key, until one key or few enough tokens for a comparison by pairs are left.  Amounts are weights, of
+// the tokens above `floor`, or (WEIGHT false) counts of all.  Every CTA of the row gets the result.
 template <typename T, int C, bool WEIGHT>
-__device__ __forceinline__ Threshold refine(const Row<T, C>& row, u64 need, float floor, bool few) {
+__device__ __forceinline__ Threshold refine(const Row<T, C>& row, u64 need, float floor) {
   SampleShared<C>* sh = row.sh;
   const int tid = row.tid, b = sh->found_bin;
-  u64 above = sh->found_above;
+  u64 above = sh->found_above, here = sh->found_here;
+  // A range of keys that holds the bin's: its ends in fp32, and 1e-5 of the maximum, by which they err less, to either side.
+  const float margin = 1e-5f * fabsf(row.top);
+  const float width = WEIGHT ? row.temperature * (0.69314718f / 32.f) : 1.f / kSampleBinsPerUnit;
+  const float x1 = fminf(row.top - width * (static_cast<float>(b) - 0.5f) + margin, row.top);
+  const float x0 = b == kSampleBins - 1 ? -INFINITY : row.top - width * (static_cast<float>(b) + 1.5f) - margin;
+  uint32_t lo_key = token_key(from_f32<T>(x0)), hi_key = token_key(from_f32<T>(x1)) + 2;
+  lo_key = lo_key > 1 ? lo_key - 2 : 0;
+  auto inside = [&](float x, uint32_t k) {
+    return k >= lo_key && k < hi_key && (!WEIGHT || x > floor) && row.template bin_of<WEIGHT>(x) == b;
+  };
+  const float unit = WEIGHT ? exp2f(44.f - static_cast<float>(b + 1) / 32.f) * 0.999f : 1.f;  // the least a token of the bin weighs
   Threshold th;
-  if (few) {
-    const int n = row.gather(true, [&](float x) { return (!WEIGHT || x > floor) && row.bin_of(x) == b; });
-    if (n <= kSampleList) {
-      __syncthreads();
-      const uint32_t key = tid < n ? static_cast<uint32_t>(sh->item[tid] >> 32) : 0u;
-      if (tid < n) sh->amount[tid] = WEIGHT ? row.weigh(key_logit<T>(key)) : 1ull;
-      __syncthreads();
-      if (tid < n) {
-        u64 more = above, same = 0;
-        for (int j = 0; j < n; ++j) {
-          const uint32_t k = static_cast<uint32_t>(sh->item[j] >> 32);
-          const u64 a = sh->amount[j];
-          if (k > key) more += a;
-          if (k == key) same += a;
+  while (hi_key - lo_key > 1) {
+    if (unit >= 1.f && static_cast<float>(here) <= unit * kSampleList) {
+      const int n = row.gather(true, [&](T v, float x) { return x >= x0 && x <= x1 && inside(x, token_key(v)); });
+      if (n <= kSampleList) {
+        __syncthreads();
+        if (tid < n) sh->amount[tid] = WEIGHT ? row.weigh(key_logit<T>(static_cast<uint32_t>(sh->item[tid] >> 32))) : 1ull;
+        __syncthreads();
+        const int share = list_share(n), i = tid / share;
+        const uint32_t key = i < n ? static_cast<uint32_t>(sh->item[i] >> 32) : 0u;
+        u64 more = 0, same = 0;
+        if (i < n) {
+#pragma unroll 2
+          for (int j = tid & (share - 1); j < n; j += share) {
+            const uint32_t k = static_cast<uint32_t>(sh->item[j] >> 32);
+            const u64 a = sh->amount[j];
+            more += k > key ? a : 0ull;
+            same += k == key ? a : 0ull;
+          }
         }
-        if (more < need && need <= more + same) {  // the same result in all tokens of that key
+        more = share_sum(more, share) + above;
+        same = share_sum(same, share);
+        if (i < n && more < need && need <= more + same) {  // the same result in all tokens of that key
           sh->found_key = key;
           sh->found_above = more;
         }
+        row_sync<C>();
+        lo_key = sh->found_key;
+        above = sh->found_above;
+        break;
       }
       row_sync<C>();
-      th.key = sh->found_key;
-      const u64 one = WEIGHT ? row.weigh(key_logit<T>(th.key)) : 1ull;
-      th.ties = (need - sh->found_above + one - 1) / one;
-      return th;
     }
-    row_sync<C>();
-  }
-  // The keys of bin b, by bisection over the monotone bin_of: hi_key is the first key above it, lo_key its lowest.
-  const uint32_t top_key = token_key(from_f32<T>(row.top));
-  auto first_key = [&](int want) {  // the lowest key whose bin is at most `want`
-    uint32_t a = 0, z = top_key;
-    while (a < z) {
-      const uint32_t m = a + (z - a) / 2;
-      const float x = key_logit<T>(m);
-      if (x == x && row.bin_of(x) <= want) z = m;  // the keys of negative NaNs lie below every number
-      else a = m + 1;
-    }
-    return a;
-  };
-  uint32_t lo_key = first_key(b), hi_key = b == 0 ? top_key + 1 : first_key(b - 1);
-  while (hi_key - lo_key > 1) {
     int shift = 0;
     while (((hi_key - 1 - lo_key) >> shift) >= static_cast<uint32_t>(kSampleBins)) ++shift;
-    row.clear_bins(WEIGHT);
-    row.each(0, row.n, tid, kSampleThreads, [&](T v, int) {
+    row.clear_bins();
+    row.each([&](T v, int) {
+      const float x = to_f32(v);
+      if (!(x >= x0 && x <= x1)) return;
       const uint32_t k = token_key(v);
-      if (k >= lo_key && k < hi_key && (!WEIGHT || to_f32(v) > floor))
-        row.template add_to_bin<WEIGHT>(static_cast<int>((hi_key - 1 - k) >> shift), to_f32(v));
+      if (inside(x, k)) row.add_to_bin(static_cast<int>((hi_key - 1 - k) >> shift), WEIGHT ? row.weigh(x) : 1ull);
     });
-    row_sync<C>();
-    u64 bin[4];
-    row.template read_bins<WEIGHT>(bin);
-    row.find_bin(bin, above + block_scan64(bin[0] + bin[1] + bin[2] + bin[3], sh->warp_total, row.warp, row.lane), need);
-    row_sync<C>();  // the result is in place, and every CTA has read this one's bins
+    row.template locate<false>(above, [&](u64) { return need; });
     above = sh->found_above;
-    const uint32_t width = 1u << shift;
-    hi_key -= static_cast<uint32_t>(sh->found_bin) * width;
-    lo_key = hi_key - lo_key > width ? hi_key - width : lo_key;
+    here = sh->found_here;
+    const uint32_t span = 1u << shift;
+    hi_key -= static_cast<uint32_t>(sh->found_bin) * span;
+    lo_key = hi_key - lo_key > span ? hi_key - span : lo_key;
   }
   th.key = lo_key;
   const u64 one = WEIGHT ? row.weigh(key_logit<T>(lo_key)) : 1ull;
@@ -394,58 +579,71 @@ __device__ __forceinline__ u64 draw_target(float u, u64 total) {
 }
 
 // Finishes a row on the n listed tokens sh->item, which hold all that can be drawn: top-k (0: none), top-p (by `need`, the
-// weight that the prefix has to reach, or where that is 0 by top_p of the list's total), min-p, the draw.  One thread a
-// token; every sum runs over the whole list.
+// weight that the prefix has to reach, or where that is 0 by top_p of the list's total), min-p, the draw.  Several threads
+// a token; every sum runs over the whole list.
 template <typename T, int C>
 __device__ __forceinline__ void finish_list(const Row<T, C>& row, int n, int top_k, float top_p, u64 need, u64 least, float u,
                                             int64_t* token) {
   SampleShared<C>* sh = row.sh;
   const int tid = row.tid;
+  const int share = list_share(n), i = tid / share, part = tid & (share - 1);
   __syncthreads();
-  const u64 mine = tid < n ? sh->item[tid] : 0ull;
+  const u64 mine = i < n ? sh->item[i] : 0ull;
   const uint32_t key = static_cast<uint32_t>(mine >> 32), index = static_cast<uint32_t>(mine);
-  const u64 full = tid < n ? row.weigh(key_logit<T>(key)) : 0ull;
+  const u64 full = i < n ? row.weigh(key_logit<T>(key)) : 0ull;
   u64 w = full;
   auto ahead = [&](u64 other) {  // `other` comes first in the order
     const uint32_t k = static_cast<uint32_t>(other >> 32);
     return k > key || (k == key && static_cast<uint32_t>(other) < index);
   };
-  if (top_k > 0 && tid < n) {
+  auto whole = [&](auto v) { return share_sum(v, share); };
+  if (top_k > 0) {
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += ahead(sh->item[j]) ? 1 : 0;
-    if (rank >= top_k) w = 0;
+    if (i < n) {
+#pragma unroll 2
+      for (int j = part; j < n; j += share) rank += ahead(sh->item[j]) ? 1 : 0;
+    }
+    if (whole(rank) >= top_k) w = 0;
   }
   if (top_p < 1.f) {
-    if (tid < n) sh->amount[tid] = w;
+    if (i < n && part == 0) sh->amount[i] = w;
     __syncthreads();
-    if (tid < n) {
-      u64 total = 0, before = 0;
-      for (int j = 0; j < n; ++j) {
+    u64 total = 0, before = 0;
+    if (i < n) {
+#pragma unroll 2
+      for (int j = part; j < n; j += share) {
         const u64 a = sh->amount[j];
         total += a;
-        if (ahead(sh->item[j])) before += a;
+        before += ahead(sh->item[j]) ? a : 0ull;
       }
-      if (before >= (need ? need : prefix_weight(top_p, total))) w = 0;
     }
+    total = whole(total);
+    before = whole(before);
+    if (i < n && before >= (need ? need : prefix_weight(top_p, total))) w = 0;
     __syncthreads();
   }
   if (full < least) w = 0;
-  if (tid < n) sh->amount[tid] = w;
+  if (i < n && part == 0) sh->amount[i] = w;
   __syncthreads();
-  if (tid < n) {
-    u64 total = 0, before = 0;
-    for (int j = 0; j < n; ++j) {
+  u64 total = 0, before = 0;
+  if (i < n) {
+#pragma unroll 2
+    for (int j = part; j < n; j += share) {
       const u64 a = sh->amount[j];
       total += a;
-      if (static_cast<uint32_t>(sh->item[j]) < index) before += a;
+      before += static_cast<uint32_t>(sh->item[j]) < index ? a : 0ull;
     }
+  }
+  total = whole(total);
+  before = whole(before);
+  if (i < n && part == 0) {
     const u64 target = draw_target(u, total);
     if (before <= target && target < before + w) *token = static_cast<int64_t>(index);
   }
 }
 
 template <typename T, int C>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleParams p) {
   constexpr int VEC = Pack16<T>::kElems;
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ SampleShared<C> shared;
@@ -464,33 +662,50 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
   const int top_k = p.top_k_v ? p.top_k_v[row_index] : p.top_k;
   const float u = p.uniform[row_index];
 
-  // The row's part into shared memory, and its maximum on the way (which a NaN takes over).
-  const T* src = static_cast<const T*>(p.logits) + row_index * p.stride + (int64_t)rank * p.chunk;
-  const int here = max(0, min(p.chunk, p.V - rank * p.chunk));
+  // The row's part into shared memory, and its maximum on the way (which a NaN takes over).  The parts are cut at
+  // 16-byte boundaries of memory, so that a row of any alignment is loaded in whole packets but for its two ends.
+  const T* logits = static_cast<const T*>(p.logits) + row_index * p.stride;
+  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(logits) & 15u) / sizeof(T));
+  const int first = rank * p.chunk - lead;
   const int n = p.chunk / VEC;
-  const bool packed = (reinterpret_cast<uintptr_t>(src) & 15u) == 0;
   float best = -INFINITY;
-  for (int i = tid; i < n; i += kSampleThreads) {
+  auto take = [&](int i, const uint4& q) {
     union { uint4 q; T v[VEC]; } pk;
-    if (packed && (i + 1) * VEC <= here) {
-      pk.q = ld_stream(reinterpret_cast<const uint4*>(src) + i);
-    } else {
+    pk.q = q;
+    reinterpret_cast<uint4*>(dyn)[i] = q;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) pk.v[e] = i * VEC + e < here ? src[i * VEC + e] : from_f32<T>(-INFINITY);
-    }
-    reinterpret_cast<uint4*>(dyn)[i] = pk.q;
+    for (int e = 0; e < VEC; e += 2)
+      asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(best) : "f"(to_f32(pk.v[e])), "f"(to_f32(pk.v[e + 1])));
+  };
+  const int i0 = first < 0 ? 1 : 0;                             // whole packets: i0 ...
+  const int i1 = max(i0, min(n, (p.V - first) / VEC));  // ... to i1
+  constexpr int kAhead = 4;
+  for (int i = i0 + tid; i < i1; i += kAhead * kSampleThreads) {
+    uint4 q[kAhead];
 #pragma unroll
-    for (int e = 0; e < VEC; e += 2) {
-      const float a = to_f32(pk.v[e]), b = to_f32(pk.v[e + 1]);
-      asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(best) : "f"(best), "f"(a), "f"(b));
-    }
+    for (int k = 0; k < kAhead; ++k)
+      if (i + k * kSampleThreads < i1) q[k] = ld_stream(reinterpret_cast<const uint4*>(logits + first) + i + k * kSampleThreads);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (i + k * kSampleThreads < i1) take(i + k * kSampleThreads, q[k]);
   }
+  for (int i = tid; i < n - (i1 - i0); i += kSampleThreads) {  // the ends, and what lies outside the row
+    const int at = i < i0 ? i : i + (i1 - i0);
+    union { uint4 q; T v[VEC]; } pk;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int t = first + at * VEC + e;
+      pk.v[e] = t >= 0 && t < p.V ? logits[t] : from_f32<T>(-INFINITY);
+    }
+    take(at, pk.q);
+  }
+  const float mine = best;
   asm volatile("redux.sync.max.NaN.f32 %0, %0, 0xffffffff;" : "+f"(best));
-  if (lane == 0) sh->pending[0][warp] = best;
+  if (lane == 0) sh->warp_float[warp] = best;
   __syncthreads();
   if (tid < C) {  // thread c tells CTA c
     float m = -INFINITY;
-    for (int k = 0; k < kSampleWarps; ++k) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(sh->pending[0][k]));
+    for (int k = 0; k < kSampleWarps; ++k) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(sh->warp_float[k]));
     if constexpr (C == 1) sh->top[0] = m;
     else st_cluster_f32(cluster_map(smem_addr(&sh->top[rank]), tid), m);
   }
@@ -505,11 +720,13 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
   top += 0.f;  // -0 is +0
   const bool greedy = !(temperature > 0.f);
   temperature = greedy ? 1.f : fminf(temperature, 1e30f);  // at 1e30 every finite logit a model gives weighs the same
-  // Rounded down: what is cut off weighs less than 2^-60 for certain, the maximum never is, and what is left has y > -976.
+  // Rounded down: what is cut off weighs less than 2^-60 for certain, and the maximum never is.
   float cut = __fsub_rd(top, 42.f * temperature);
-  if (top == INFINITY || cut == -INFINITY) {
-    // The limit of a maximum of +inf: the infinite ones share everything.  A maximum next to the lowest number: all finite
-    // logits lie within a factor of two of it, so that their differences from it are exact.
+  const bool replaced = !(top - cut <= 64.f * temperature);
+  if (replaced) {
+    // A maximum of +inf: in the limit the infinite ones share everything.  A maximum so large that fp32 has no number
+    // between 42 and 64 temperatures below it: logits are replaced by their differences from it, exact within a factor of
+    // two of it, and of no weight beyond.
     for (int i = tid; i < n * VEC; i += kSampleThreads) {
       T* v = reinterpret_cast<T*>(dyn) + i;
       const float x = to_f32(*v);
@@ -522,7 +739,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
 
   Row<T, C> row;
   row.packets = reinterpret_cast<const uint4*>(dyn);
-  row.n = n; row.rank = rank; row.chunk = p.chunk; row.sh = sh; row.top = top;
+  row.n = n; row.seg = (n + kSampleWarps - 1) / kSampleWarps; row.rank = rank; row.first = first; row.sh = sh; row.top = top; row.temperature = temperature;
   row.tid = tid; row.lane = lane; row.warp = warp;
   row.weigh.top = static_cast<double>(top);
   row.weigh.scale = 16. * 1.4426950408889634074 / static_cast<double>(temperature);
@@ -541,82 +758,45 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
   u64 floor_weight = 0;
   if (use_k) {
     const u64 need = static_cast<u64>(top_k);
-    row.clear_bins(false);
-    row.each(0, n, tid, kSampleThreads, [&](T v, int) { row.template add_to_bin<false>(row.bin_of(to_f32(v)), 0.f); });
-    row_sync<C>();
-    u64 bin[4];
-    row.template read_bins<false>(bin);
-    u64 before = block_scan64(bin[0] + bin[1] + bin[2] + bin[3], sh->warp_total, warp, lane);
-    row.find_bin(bin, before, need);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {  // how many tokens the bins down to the threshold's hold, and that one alone
-      if (before < need && before + bin[i] >= need) {
-        sh->down_to = static_cast<int>(before + bin[i]);
-        sh->inside = static_cast<int>(bin[i]);
-      }
-      before += bin[i];
+    int beyond = kSampleBins - 2;
+    if (top_k <= kSampleThreads && n * VEC >= kSampleBound && !replaced) {
+      // Of the largest logits that this CTA's threads have seen the k-th: k tokens are at or above it.
+      row.clear_bins();
+      atomicAdd(&sh->bin[0][row.template bin_of<false>(mine)], 1u);
+      row.template locate<false, true>(0, [&](u64) { return need; });
+      beyond = min(sh->found_bin, beyond);
     }
-    row_sync<C>();
-    const int last = sh->found_bin, inside = sh->inside;
-    if (sh->down_to <= kSampleFinish) {
-      const int got = row.gather(rank == 0, [&](float x) { return row.bin_of(x) <= last; });
+    row.template fill_bins<false>(floor, beyond);
+    row.template locate<false>(0, [&](u64) { return need; });
+    const int last = sh->found_bin;
+    if (sh->found_above + sh->found_here <= kSampleList) {
+      const int got = row.gather(rank == 0, [&](T, float x) { return x > -INFINITY && row.template bin_of<false>(x) <= last; });
       if (rank == 0) finish_list<T, C>(row, got, top_k, top_p, 0ull, least, u, token);
       if constexpr (C > 1) cluster_sync_all();  // rank 0 has read the other lists
       return;
     }
-    th = refine<T, C, false>(row, need, -INFINITY, inside <= kSampleList);
+    th = refine<T, C, false>(row, need, floor);
     floor = key_logit<T>(th.key);
     floor_weight = row.weigh(floor);
   }
   if (use_p) {
     // The weights above top-k's threshold; at it, `ties` tokens more.
-    row.clear_bins(true);
-    row.each(0, n, tid, kSampleThreads, [&](T v, int) {
-      const float x = to_f32(v);
-      if (x > floor) row.template add_to_bin<true>(row.bin_of(x), x);
+    // All tokens that weigh less than (1 - p) / V of the likeliest weigh less than 1 - p of the total together: the prefix
+    // ends before them.
+    const float beyond = 32.f * (log2f(static_cast<float>(p.V)) - log2f(1.f - fmaxf(top_p, 0.f))) + 2.f;
+    row.template fill_bins<true>(floor, static_cast<int>(fminf(beyond, static_cast<float>(kSampleBins - 2))));
+    u64 total, need;
+    row.template locate<true>(0, [&](u64 sum) {
+      total = sum;
+      return need = prefix_weight(top_p, total + th.ties * floor_weight);
     });
-    row_sync<C>();
-    u64 bin[4];
-    row.template read_bins<true>(bin);
-    const u64 before = block_scan64(bin[0] + bin[1] + bin[2] + bin[3], sh->warp_total, warp, lane);
-    u64 total = 0;
-#pragma unroll
-    for (int k = 0; k < kSampleWarps; ++k) total += sh->warp_total[k];
-    const u64 need = prefix_weight(top_p, total + th.ties * floor_weight);
     if (need > total) {  // the prefix ends among the ties at top-k's threshold
       th.ties = (need - total + floor_weight - 1) / floor_weight;
-      row_sync<C>();
     } else {
-      row.find_bin(bin, before, need);
-      row_sync<C>();
-      // How many tokens the bins down to the threshold's hold, from above: a bin's weight over the least that one of its
-      // tokens weighs.  Weights of a few units say nothing.
       const int last = sh->found_bin;
-      const float per_bin = 1.f / (kSampleBinsPerUnit * temperature);
-      float count = 0.f, inside = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int b = 4 * tid + i;
-        const float unit = expf(-static_cast<float>(b + 1) * per_bin) * 17592186044416.f * 0.999f;
-        const float c = b > last || bin[i] == 0 ? 0.f : unit < 4096.f ? 1e9f : static_cast<float>(bin[i]) / unit;
-        count += c;
-        if (b == last) inside = c;
-      }
-      count = warp_sum(count);
-      inside = warp_sum(inside);
-      if (lane == 0) {
-        sh->pending[warp][0] = count;
-        sh->pending[warp][1] = inside;
-      }
-      __syncthreads();
-      count = inside = 0.f;
-#pragma unroll
-      for (int k = 0; k < kSampleWarps; ++k) {
-        count += sh->pending[k][0];
-        inside += sh->pending[k][1];
-      }
-      if (count <= static_cast<float>(kSampleFinish)) {
-        const int got = row.gather(rank == 0, [&](float x) { return x > floor && row.bin_of(x) <= last; });
+      if (sh->found_tokens <= kSampleList / 2) {  // room for some of the bins beyond, which the test may take along
+        const float end = row.template bin_end<true>(last);
+        const int got = row.gather(rank == 0, [&](T, float x) { return x > floor && x >= end; });
         if (got <= kSampleList) {
           if (rank == 0) finish_list<T, C>(row, got, 0, top_p, need, least, u, token);
           if constexpr (C > 1) cluster_sync_all();  // rank 0 has read the other lists
@@ -624,7 +804,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
         }
         row_sync<C>();
       }
-      th = refine<T, C, true>(row, need, floor, inside <= static_cast<float>(kSampleList));
+      th = refine<T, C, true>(row, need, floor);
     }
   }
 
@@ -635,48 +815,38 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
   const bool use_ties = bounded && edge_weight >= least;
   // A logit below which min-p leaves nothing for certain (fp32 errs by far less than the margin).
   float skip = edge;
-  if (least_share > 0.f) skip = fmaxf(skip, top + temperature * (logf(least_share) - 1e-3f) - fabsf(top) * 1e-5f);
-  const int seg = (n + kSampleWarps - 1) / kSampleWarps;  // packets
+  if (least_share > 0.f) skip = fmaxf(skip, top + temperature * (logf(least_share) - 1e-3f) - 1e-5f * fabsf(top));
+  const int seg = row.seg;
   {
     u64 sum = 0;
     uint32_t ties = 0;
     const int begin = min(warp * seg, n), end = min(begin + seg, n);
     if (!(skip > -INFINITY)) {
-      row.each(begin, end, lane, 32, [&](T v, int) { sum += row.weigh(to_f32(v)); });
-    } else {
-      // The kept ones are put side by side first, 32 at a time, since often a warp would weigh a few at a time.
-      float* mine = sh->pending[warp];
-      int waiting = 0;
-      auto add = [&](float x, bool there) {
-        const u64 w = there ? row.weigh(x) : 0ull;
-        sum += w >= least ? w : 0ull;
-      };
-      __syncthreads();  // the counts above have been read
-      for (int i0 = begin; i0 < end; i0 += 32) {
-        union { uint4 q; T v[VEC]; } pk;
-        const bool there = i0 + lane < end;
-        if (there) pk.q = ld_shared16(row.packets + i0 + lane);
+      uint32_t count = 0;
+      row.each_four(begin, end, lane, 32, [&](const float (&x)[4]) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float x = there ? to_f32(pk.v[e]) : -INFINITY;
-          ties += bounded && x == edge ? 1u : 0u;
-          const uint32_t kept = __ballot_sync(0xffffffffu, x > skip);
-          if (kept == 0) continue;
-          if (x > skip) mine[waiting + __popc(kept & ((1u << lane) - 1u))] = x;
-          waiting += __popc(kept);
-          if (waiting >= 32) {
-            __syncwarp();
-            const float now = mine[lane], rest = mine[lane + 32];
-            __syncwarp();
-            mine[lane] = rest;
-            waiting -= 32;
-            add(now, true);
-            __syncwarp();
-          }
+        for (int e = 0; e < 4; ++e) {
+          int bin;
+          sum += row.weigh.biased(x[e], bin);
+        }
+        count += 4;
+      });
+      sum -= count * Weigh::kBias;
+    } else {
+      auto queue = row.side([&](float x, bool valid) {
+        const u64 w = valid ? row.weigh(x) : 0ull;
+        sum += w >= least ? w : 0ull;
+      });
+      for (int i0 = begin * (VEC / 4); i0 < end * (VEC / 4); i0 += 32) {
+        float x[4];
+        row.four(i0 + lane < end * (VEC / 4) ? i0 + lane : INT_MAX, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          ties += bounded && x[e] == edge ? 1u : 0u;
+          queue.push(x[e], x[e] > skip);
         }
       }
-      __syncwarp();
-      add(lane < waiting ? mine[lane] : 0.f, lane < waiting);
+      queue.drain();
     }
     sum = warp_sum64(sum);
     ties = __reduce_add_sync(0xffffffffu, ties);
@@ -753,7 +923,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const SamplePara
     for (int i = b0; i < b1; ++i) {
       const u64 w = weight_at(i, tie);
       if (rest < before + w) {
-        *token = (int64_t)rank * p.chunk + i;
+        *token = first + i;
         break;
       }
       before += w;
