@@ -38,7 +38,7 @@ struct AddNormParams {
   int N;
   int w_dtype;
   float eps;
-  int group;  // 8-bit form: columns per scale, 0 for one scale a row
+  int group;  // 8-bit form, element by element: columns per scale, 0 for one scale a row
   int groups_per_row;
   int e8m0;  // 8-bit form: scales are powers of two, stored as their biased exponent
   int stages;   // backward with a ring: slots per row group
@@ -257,27 +257,28 @@ __device__ __forceinline__ float warp_max_abs(float v) {
 // e4m3 values; the reciprocal of a power of two is exact).
 struct Fp8Scale {
   float scale, inv;
-  uint8_t code;
+  uint32_t code;
 };
 __device__ __forceinline__ Fp8Scale fp8_scale(float amax, bool e8m0) {
   Fp8Scale r;
   amax = max_abs(amax, kAmaxFloor);
-  r.code = 0;
   if (e8m0) {
-    r.scale = amax / kE4m3Max;  // correctly rounded: a power of two must not look like a little more
-    // the next power of two: the exponent field, one more where the fraction is not zero
-    const uint32_t e = r.scale != r.scale ? 255u : (__float_as_uint(r.scale) + 0x7fffffu) >> 23;
-    r.code = static_cast<uint8_t>(e);
-    r.scale = __uint_as_float(e == 255u ? 0x7fffffffu : e << 23);
-    r.inv = __uint_as_float(e == 255u ? 0x7fffffffu : (254u - e) << 23);
+    // The lowest 2^e with amax <= 448 * 2^e = 1.75 * 2^(e + 8): eight below amax's exponent, or seven where its fraction is
+    // above .75.  The reciprocal of a power of two is one, too.
+    const uint32_t bits = __float_as_uint(amax), e = (bits >> 23) - 8u + ((bits & 0x7fffffu) > 0x600000u ? 1u : 0u);
+    const bool bad = bits >= 0x7f800000u;  // infinity and NaN have the NaN code
+    r.code = bad ? 255u : e;
+    r.scale = 0.f;
+    r.inv = __uint_as_float(bad ? 0x7fffffffu : (254u - e) << 23);
   } else {
+    r.code = 0;
     r.scale = amax * (1.f / kE4m3Max);
     r.inv = rcp_fast(r.scale);
   }
   return r;
 }
 __device__ __forceinline__ void store_scale(void* p, int64_t at, const Fp8Scale& s, bool e8m0) {
-  if (e8m0) static_cast<uint8_t*>(p)[at] = s.code;
+  if (e8m0) static_cast<uint8_t*>(p)[at] = static_cast<uint8_t>(s.code);
   else static_cast<float*>(p)[at] = s.scale;
 }
 
@@ -304,7 +305,19 @@ __host__ __device__ constexpr int addnorm_bwd_ctas(int ld, int tpr, bool lean) {
   return n < 1 ? 1 : n;
 }
 
-// Sum over the TPR threads that share a row.
+// After a wait that ran out: the copies that a row group has in flight get a bounded chance to land.
+__device__ __forceinline__ void addnorm_drain(uint64_t* bars, int stages, int64_t rows) {
+  const unsigned long long t0 = global_ns();
+  for (int s = 0; s < stages && s < rows; ++s) {
+    const int64_t fills = (rows - s + stages - 1) / stages;
+    while (!mbar_try_wait(&bars[s], static_cast<uint32_t>((fills - 1) & 1)))
+      if (global_ns() - t0 > 10000000ull) return;
+  }
+}
+
+// Sum over the TPR threads that share a row.  `scratch`: two halves, used in turn, of one float per warp, padded with zeros to
+// whole 16-byte words; every thread adds all warps' sums in one order.
+__host__ __device__ constexpr int row_scratch(int tpr) { return tpr <= 32 ? 4 : (tpr / 32 + 3) / 4 * 4; }
 template <int TPR, int FIRST>
 __device__ __forceinline__ float row_sum(float v, float* scratch, int& phase, int group, int warp_n, int lane) {
   if constexpr (TPR <= 32) {
@@ -312,33 +325,84 @@ __device__ __forceinline__ float row_sum(float v, float* scratch, int& phase, in
     for (int o = TPR / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
   } else {
-    float s[1] = {v};
-    group_sum<TPR / 32, 1, FIRST>(s, scratch, phase, group, warp_n, lane);
-    return s[0];
+    v = warp_sum(v);
+    float* buf = scratch + phase * row_scratch(TPR);
+    if (lane == 0) buf[warp_n] = v;
+    group_sync<TPR / 32, FIRST>(group);
+    float2 s = splat2(0.f);
+#pragma unroll
+    for (int k = 0; k < row_scratch(TPR) / 4; ++k) {
+      const float4 q = reinterpret_cast<const float4*>(buf)[k];
+      s = add2(s, make_float2(q.x, q.y));
+      s = add2(s, make_float2(q.z, q.w));
+    }
+    phase ^= 1;
+    return s.x + s.y;
   }
+}
+
+// The same, and the largest magnitude, with one barrier for both.
+template <int TPR>
+__device__ __forceinline__ float row_sum_max(float v, float& amax, float* scratch, float* max_scratch, int& phase, int group,
+                                             int warp_n, int lane) {
+  if constexpr (TPR <= 32) {
+#pragma unroll
+    for (int o = TPR / 2; o > 0; o >>= 1) amax = max_abs(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  } else {
+    amax = warp_max_abs(amax);
+    float* buf = max_scratch + phase * row_scratch(TPR);
+    if (lane == 0) buf[warp_n] = amax;
+    v = row_sum<TPR, 0>(v, scratch, phase, group, warp_n, lane);
+#pragma unroll
+    for (int k = 0; k < row_scratch(TPR) / 4; ++k) {
+      const float4 q = reinterpret_cast<const float4*>(buf)[k];
+      amax = max_abs3(max_abs3(amax, q.x, q.y), q.z, q.w);
+    }
+    return v;
+  }
+  return row_sum<TPR, 0>(v, scratch, phase, group, warp_n, lane);
 }
 
 // Forward.  OFF: the rows of all buffers start at one common offset within a packet that need not be
 // zero (contiguous tensors of an odd row length); packets are then laid on the buffers' own alignment,
 // the first and the last of a row are partial, and the launch gives every row group rows of one offset
 // only (its step is a multiple of the offsets' period), so that a thread's columns stay the same.
-// FP8: the 8-bit form.  Thread t of a row group holds packets t, t + TPR, ...: neighbouring lanes hold
-// neighbouring columns, so a scale's 32, 64 or 128 columns are 4 to 32 adjacent lanes of one warp.
-template <typename T, typename R, int LD, int TPR, bool OFF, bool FP8>
-__global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR, !OFF && !(FP8 && TPR <= 128)))
+// GROUP: the 8-bit form with a scale for so many columns, 0 for one a row; -1: the output is y.  Thread t of a
+// row group holds packets t, t + TPR, ...: neighbouring lanes hold neighbouring columns, so a scale's 32, 64 or
+// 128 columns are 4 to 32 adjacent lanes of one warp.
+// RING: as in the backward below, the rows of x and r arrive through p.stages shared-memory slots per row group.
+template <typename T, typename R, int LD, int TPR, bool OFF, int GROUP, bool RING>
+__global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR, !OFF && (GROUP < 0 || (GROUP > 0 && RING))))
     addnorm_fwd_kernel(const AddNormParams p) {
-  static_assert(!(OFF && FP8), "scale groups lie on packet boundaries");
+  constexpr bool FP8 = GROUP >= 0, PER_ROW = GROUP == 0;
+  static_assert(!(OFF && (FP8 || RING)), "scale groups lie on packet boundaries, and bulk copies take whole packets");
+  static_assert(!RING || TPR > 32, "a ring belongs to a group with a barrier");
   constexpr int VEC = Pack16<T>::kElems, H = VEC / 2;
   constexpr int GROUPS = addnorm_threads(TPR) / TPR;
-  constexpr int WARPS_N = TPR >= 32 ? TPR / 32 : 1;
   constexpr bool WREG = LD * VEC <= 16;  // the weights fit in registers next to the row
-  extern __shared__ __align__(16) float ws[];  // OFF: the weights
-  __shared__ float scratch[GROUPS][2 * WARPS_N];
-  __shared__ float max_scratch[FP8 ? GROUPS : 1][2 * WARPS_N];
+  extern __shared__ __align__(128) unsigned char dyn[];  // OFF: the weights; RING: the slots
+  float* ws = reinterpret_cast<float*>(dyn);
+  __shared__ __align__(8) uint64_t bars[RING ? GROUPS : 1][kAddNormStages];
+  __shared__ int cta_abort;
+  __shared__ __align__(16) float scratch[GROUPS][2 * row_scratch(TPR)];
+  __shared__ __align__(16) float max_scratch[FP8 ? GROUPS : 1][2 * row_scratch(TPR)];
 
   const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
   const int lane = threadIdx.x & 31, warp_n = TPR >= 32 ? t / 32 : 0;
-  int phase = 0, max_phase = 0;
+  int phase = 0;
+  if constexpr (TPR > 32) {
+    for (int i = threadIdx.x; i < GROUPS * 2 * row_scratch(TPR); i += blockDim.x) {
+      (&scratch[0][0])[i] = 0.f;
+      if (FP8) (&max_scratch[0][0])[i] = 0.f;
+    }
+    if (RING && threadIdx.x == 0) {
+      for (int g = 0; g < GROUPS; ++g)
+        for (int i = 0; i < p.stages; ++i) mbar_init(&bars[g][i], 1);
+      cta_abort = 0;
+      mbar_init_fence();
+    }
+    __syncthreads();
+  }
   grid_dependency_sync();
   trigger_dependents();
 
@@ -349,6 +413,22 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
   const int off = OFF ? static_cast<int>((reinterpret_cast<uintptr_t>(p.x) / sizeof(T) + first * p.x_stride) % VEC) : 0;
   const int packets = (off + p.N + VEC - 1) / VEC;
   const float inv_n = 1.f / static_cast<float>(p.N);
+
+  const uint32_t x_bytes = p.N * sizeof(T), r_bytes = p.r != nullptr ? p.N * sizeof(R) : 0u;
+  unsigned char* slots = dyn + (size_t)group * p.stages * (x_bytes + r_bytes);
+  auto fill = [&](int s, int64_t row) {  // the group's first thread: x and r of a row into slot s
+    unsigned char* dst = slots + (size_t)s * (x_bytes + r_bytes);
+    mbar_expect_tx(&bars[group][s], x_bytes + r_bytes);
+    bulk_load(dst, xs.base + row * xs.stride, x_bytes, &bars[group][s]);
+    if (p.r != nullptr) bulk_load(dst + x_bytes, rs.base + row * rs.stride, r_bytes, &bars[group][s]);
+  };
+  if constexpr (RING) {
+    if (t == 0)
+      for (int s = 0; s < p.stages; ++s)
+        if (first + s * step < p.M) fill(s, first + s * step);
+  }
+  int slot = 0;
+  uint32_t parity = 0;
 
   if constexpr (OFF) {
     stage_w<VEC>(p.w, p.w_dtype, p.N, ws);
@@ -377,14 +457,21 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
     {
       RawVec<T, VEC> xv[LD];
       RawVec<R, VEC> rv[LD];
+      const unsigned char* src = slots + (size_t)slot * (x_bytes + r_bytes);
+      if constexpr (RING) mbar_wait(&bars[group][slot], parity, &cta_abort, p.status);
 #pragma unroll
       for (int j = 0; j < LD; ++j) {
         const int pk = j * TPR + t;
         xv[j].zero();
         rv[j].zero();
         if (!valid || pk >= packets) continue;
-        xv[j] = xs.load(row, pk * VEC - off);
-        if (p.r != nullptr) rv[j] = rs.load(row, pk * VEC - off);
+        if constexpr (RING) {
+          xv[j].load_shared(src + (size_t)pk * VEC * sizeof(T));
+          if (p.r != nullptr) rv[j].load_shared(src + x_bytes + (size_t)pk * VEC * sizeof(R));
+        } else {
+          xv[j] = xs.load(row, pk * VEC - off);
+          if (p.r != nullptr) rv[j] = rs.load(row, pk * VEC - off);
+        }
       }
 #pragma unroll
       for (int j = 0; j < LD; ++j) {
@@ -407,12 +494,43 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
     for (int j = 0; j < LD; ++j)
 #pragma unroll
       for (int k = 0; k < H; ++k) q2 = fma2(hf[j][k], hf[j][k], q2);
-    const float q = row_sum<TPR, 0>(q2.x + q2.y, scratch[group], phase, group, warp_n, lane);
-    const float rstd = 1.f / sqrtf(q * inv_n + p.eps);
+    auto w_of = [&](int j, float2* wf) {
+      if constexpr (WREG) {
+#pragma unroll
+        for (int k = 0; k < H; ++k) wf[k] = wr[j][k];
+      } else {
+        weights((j * TPR + t) * VEC - off, wf);
+      }
+    };
+    // One scale a row: max |y| is rstd * max |h w|, so the maximum is found along with the sum.
+    float q, amax = 0.f;
+    if constexpr (PER_ROW) {
+#pragma unroll
+      for (int j = 0; j < LD; ++j) {
+        if (j * TPR + t >= packets) continue;
+        float2 wf[H];
+        w_of(j, wf);
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+          const float2 v = mul2(hf[j][k], wf[k]);
+          amax = max_abs3(amax, v.x, v.y);
+        }
+      }
+      q = row_sum_max<TPR>(q2.x + q2.y, amax, scratch[group], max_scratch[group], phase, group, warp_n, lane);
+    } else {
+      q = row_sum<TPR, 0>(q2.x + q2.y, scratch[group], phase, group, warp_n, lane);
+    }
+    if constexpr (RING) {  // behind a barrier that every thread passes with its packets read
+      if (t == 0 && row + p.stages * step < p.M) fill(slot, row + p.stages * step);
+      if (++slot == p.stages) {
+        slot = 0;
+        parity ^= 1u;
+      }
+    }
+    const float rstd = rsqrtf(q * inv_n + p.eps);
     if (t == 0 && valid && p.rstd != nullptr) p.rstd[row] = rstd;
     const float2 r2 = splat2(rstd);
 
-    float amax = 0.f;  // one scale a row
     float amax_j[FP8 ? LD : 1];
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
@@ -420,60 +538,52 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
       if constexpr (FP8) amax_j[j] = 0.f;
       if (pk >= packets) continue;
       float2 wf[H];
-      if constexpr (WREG) {
-#pragma unroll
-        for (int k = 0; k < H; ++k) wf[k] = wr[j][k];
-      } else {
-        weights(pk * VEC - off, wf);
-      }
+      w_of(j, wf);
 #pragma unroll
       for (int k = 0; k < H; ++k) hf[j][k] = mul2(mul2(hf[j][k], r2), wf[k]);
       if constexpr (!FP8) {
         RawVec<T, VEC> o;
         o.pack(hf[j]);
         if (valid) ys.store(row, pk * VEC - off, o);
-      } else {
+      } else if constexpr (!PER_ROW) {
         float a = 0.f;
 #pragma unroll
         for (int k = 0; k < H; ++k) a = max_abs3(a, hf[j][k].x, hf[j][k].y);
         amax_j[j] = a;
-        amax = max_abs(amax, a);
       }
     }
 
     if constexpr (FP8) {
       uint8_t* qrow = static_cast<uint8_t*>(p.y) + row * p.y_stride;
       Fp8Scale sc;
-      if (p.group == 0) {
-        if constexpr (TPR >= 32) {
-          amax = warp_max_abs(amax);
-        } else {
+      if constexpr (PER_ROW) {
+        amax *= rstd;
+        // A sum of squares that overflows makes rstd 0 and y 0, or NaN where h is infinite; a product h w may have
+        // overflowed along with it, so the maximum is taken again, of y itself.
+        const bool again = TPR <= 32 ? __any_sync(0xffffffffu, rstd == 0.f) : rstd == 0.f;
+        if (again) {
+          float a = 0.f;
 #pragma unroll
-          for (int o = TPR / 2; o > 0; o >>= 1) amax = max_abs(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        }
-        if constexpr (TPR > 32) {
-          float* buf = max_scratch[group] + max_phase * WARPS_N;
-          if (lane == 0) buf[warp_n] = amax;
-          group_sync<WARPS_N, 0>(group);
+          for (int j = 0; j < LD; ++j)
 #pragma unroll
-          for (int k = 0; k < WARPS_N; ++k) amax = max_abs(amax, buf[k]);
-          max_phase ^= 1;
+            for (int k = 0; k < H; ++k) a = max_abs3(a, hf[j][k].x, hf[j][k].y);
+          row_sum_max<TPR>(0.f, a, scratch[group], max_scratch[group], phase, group, warp_n, lane);
+          if (rstd == 0.f) amax = a;
         }
         sc = fp8_scale(amax, p.e8m0 != 0);
         if (t == 0 && valid) store_scale(p.scale, row, sc, p.e8m0 != 0);
       }
-      const int lanes = p.group == 0 ? 1 : min(p.group / VEC, TPR);  // adjacent lanes that share a scale
+      constexpr int LANES = PER_ROW ? 1 : (GROUP / VEC < TPR ? GROUP / VEC : TPR);  // adjacent lanes that share a scale
 #pragma unroll
       for (int j = 0; j < LD; ++j) {
         const int pk = j * TPR + t;
-        if (p.group != 0) {
+        if constexpr (!PER_ROW) {
           float a = amax_j[j];
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1)
-            if (o < lanes) a = max_abs(a, __shfl_xor_sync(0xffffffffu, a, o));
+          for (int o = 1; o < LANES; o <<= 1) a = max_abs(a, __shfl_xor_sync(0xffffffffu, a, o));
           sc = fp8_scale(a, p.e8m0 != 0);
-          if (valid && pk < packets && (t & (lanes - 1)) == 0)
-            store_scale(p.scale, row * p.groups_per_row + pk * VEC / p.group, sc, p.e8m0 != 0);
+          if (valid && pk < packets && (t & (LANES - 1)) == 0)
+            store_scale(p.scale, row * p.groups_per_row + pk * VEC / (PER_ROW ? 1 : GROUP), sc, p.e8m0 != 0);
         }
         if (valid && pk < packets) {
           const float2 inv2 = splat2(sc.inv);
@@ -489,6 +599,9 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
       }
     }
   }
+  if constexpr (RING) {
+    if (t == 0 && cta_abort) addnorm_drain(bars[group], p.stages, first < p.M ? (p.M - first + step - 1) / step : 0);
+  }
 }
 
 // Backward.  A thread owns fixed columns of every row its group visits and carries their dweight sums:
@@ -500,10 +613,9 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
 // A slot is refilled behind the row's reduction, a barrier that every thread passes with its packets read.
 template <typename T, typename R, int LD, int TPR, bool OFF, bool RING>
 __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_bwd_ctas(LD, TPR, sizeof(R) == sizeof(T) && TPR >= 160)) addnorm_bwd_kernel(const AddNormParams p) {
-  static_assert(!(OFF && RING) && !(RING && TPR < 32), "bulk copies take whole packets; a ring belongs to whole warps");
+  static_assert(!RING || (!OFF && TPR > 32), "bulk copies take whole packets; a ring belongs to a group with a barrier");
   constexpr int VEC = Pack16<T>::kElems, H = VEC / 2;
   constexpr int GROUPS = addnorm_threads(TPR) / TPR;
-  constexpr int WARPS_N = TPR >= 32 ? TPR / 32 : 1;
   constexpr bool WREG = LD * VEC <= 16;
   constexpr bool WIDE = addnorm_wide(LD, VEC, TPR);
   // OFF: the weights; then the sums, WIDE [LD * VEC][TPR] or, of several groups, [GROUPS][N]; RING: the slots, which
@@ -511,13 +623,14 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_bwd_ctas(LD, TPR
   extern __shared__ __align__(128) unsigned char dyn[];
   float* ws = reinterpret_cast<float*>(dyn);
   float* acc = ws + (OFF ? w_slots<VEC>(p.N) : 0);
-  __shared__ float scratch[GROUPS][2 * WARPS_N];
+  __shared__ __align__(16) float scratch[GROUPS][2 * row_scratch(TPR)];
   __shared__ __align__(8) uint64_t bars[RING ? GROUPS : 1][kAddNormStages];
   __shared__ int cta_abort;
 
   const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
   const int lane = threadIdx.x & 31, warp_n = TPR >= 32 ? t / 32 : 0;
   int phase = 0;
+  for (int i = threadIdx.x; i < GROUPS * 2 * row_scratch(TPR); i += blockDim.x) (&scratch[0][0])[i] = 0.f;
   if constexpr (RING) {
     if (threadIdx.x == 0) {
       for (int g = 0; g < GROUPS; ++g)
@@ -525,8 +638,8 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_bwd_ctas(LD, TPR
       cta_abort = 0;
       mbar_init_fence();
     }
-    __syncthreads();
   }
+  __syncthreads();
   grid_dependency_sync();
   trigger_dependents();
 
@@ -639,7 +752,6 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_bwd_ctas(LD, TPR
     }
     const float c1 = row_sum<TPR, (GROUPS == 1 ? 0 : 1)>(s2.x + s2.y, scratch[group], phase, group, warp_n, lane) * inv_n;
     if constexpr (RING) {
-      if (TPR == 32) __syncwarp();
       if (t == 0 && row + p.stages * step < p.M) fill(slot, row + p.stages * step);
       if (++slot == p.stages) {
         slot = 0;
@@ -675,15 +787,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_bwd_ctas(LD, TPR
     }
   }
   if constexpr (RING) {
-    if (t == 0 && cta_abort) {  // a wait ran out: what is still in flight gets a bounded chance to land
-      const int64_t rows = first < p.M ? (p.M - first + step - 1) / step : 0;
-      const unsigned long long t0 = global_ns();
-      for (int s = 0; s < p.stages && s < rows; ++s) {
-        const int64_t fills = (rows - s + p.stages - 1) / p.stages;
-        while (!mbar_try_wait(&bars[group][s], static_cast<uint32_t>((fills - 1) & 1)))
-          if (global_ns() - t0 > 10000000ull) break;
-      }
-    }
+    if (t == 0 && cta_abort) addnorm_drain(bars[group], p.stages, first < p.M ? (p.M - first + step - 1) / step : 0);
   }
 
   if (p.part == nullptr) return;
@@ -880,9 +984,10 @@ __global__ void __launch_bounds__(512) addnorm_bwd_any_kernel(const AddNormParam
 struct AddNormShape {
   int ld, tpr;
   const void* fwd[2];  // [rows at a common offset]
-  const void* fp8;
+  const void* fp8[4];  // a scale per row, 32, 64, 128 columns
   const void* bwd[2];
-  const void* bwd_ring;  // null: none
+  const void* fp8_ring[4];  // null: none
+  const void* bwd_ring;
   int capacity() const { return ld * tpr; }  // packets per row
   int threads() const { return addnorm_threads(tpr); }
   int groups() const { return threads() / tpr; }

@@ -63,7 +63,7 @@ struct Plan {
   size_t smem;
 };
 
-// Slots of a backward ring: as many, up to four, as leave room for three, two or one CTA per SM (228 KB, 1 KB of it
+// Slots of a ring: as many, up to four, as leave room for three, two or one CTA per SM (228 KB, 1 KB of it
 // reserved per CTA, and a little static shared memory), at least two; 0 when two do not fit.
 int ring_stages(size_t slot, size_t fixed, int groups, size_t* smem) {
   for (size_t cap : {74 * 1024, 112 * 1024, 224 * 1024})
@@ -75,8 +75,10 @@ int ring_stages(size_t slot, size_t fixed, int groups, size_t* smem) {
   return 0;
 }
 
-int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, int period, int64_t M, int64_t N, bool has_dh,
-         Plan* out) {
+int scale_kind(int group) { return group == 0 ? 0 : group == 32 ? 1 : group == 64 ? 2 : 3; }
+
+int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, int period, int64_t M, int64_t N,
+         bool has_residual, int group, Plan* out) {
   const int vec = 16 / t->size_t_;
   // packets a row can span: up to one more at either end when it starts inside one
   const int64_t need = layout == kOffset ? (N + 2 * vec - 2) / vec : (N + vec - 1) / vec;
@@ -89,13 +91,21 @@ int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, in
   out->smem = 0;
   if (s != nullptr) {
     groups = s->groups();
-    out->fn = which == kFwd ? s->fwd[layout] : which == kFp8 ? s->fp8 : s->bwd[layout];
+    out->fn = which == kFwd ? s->fwd[layout] : which == kFp8 ? s->fp8[scale_kind(group)] : s->bwd[layout];
     out->threads = s->threads();
     if (layout == kOffset) out->smem = sizeof(float) * (vec == 8 ? w_slots<8>(static_cast<int>(N)) : w_slots<4>(static_cast<int>(N)));
+    if (which == kFp8 && s->fp8_ring[0] != nullptr && M > (int64_t)dev.sm_count * groups) {
+      size_t ring = 0;
+      out->stages = ring_stages(static_cast<size_t>(N) * (t->size_t_ + (has_residual ? t->size_r : 0)), 0, groups, &ring);
+      if (out->stages > 0) {
+        out->fn = s->fp8_ring[scale_kind(group)];
+        out->smem = ring;
+      }
+    }
     if (which == kBwd) {
       const size_t wide = addnorm_wide(s->ld, vec, s->tpr) ? sizeof(float) * s->ld * vec * s->tpr : 0;
       const size_t sums = groups > 1 ? sizeof(float) * groups * N : wide;
-      const size_t slot = static_cast<size_t>(N) * (t->size_t_ + t->size_r * (has_dh ? 2 : 1));
+      const size_t slot = static_cast<size_t>(N) * (t->size_t_ + t->size_r * (has_residual ? 2 : 1));
       size_t ring = 0;
       if (layout == kAligned && s->bwd_ring != nullptr) out->stages = ring_stages(slot, wide, groups, &ring);
       if (out->stages > 0) {
@@ -138,16 +148,17 @@ int forward(bool fp8, const void* x, int64_t xs, const void* r, int64_t rs, cons
   if (r == nullptr && h != nullptr) return fail(B200NORM_ERR_ARG, "h is the sum with a residual: there is none");
   if (xs < N || ys < N || (r && rs < N) || (h && hs < N)) return fail(B200NORM_ERR_ARG, "row stride smaller than N");
   DeviceState* dev = nullptr;
-  if (int rc = device_caches(&dev)) return rc;
+  if (int rc = fp8 ? device_state(&dev) : device_caches(&dev)) return rc;
   const AddNormTable* t = table_for(io, res);
   const Buffer bufs[4] = {{x, xs, t->size_t_}, {r, rs, t->size_r}, {y, ys, fp8 ? 1 : t->size_t_}, {h, hs, t->size_r}};
   int period;
   const Layout layout = layout_of(bufs, 4, N, 16 / t->size_t_, w, &period);
   Plan pl;
-  if (int rc = plan(*dev, t, fp8 ? kFp8 : kFwd, layout, period, M, N, r != nullptr, &pl)) return rc;
+  if (int rc = plan(*dev, t, fp8 ? kFp8 : kFwd, layout, period, M, N, r != nullptr, group, &pl)) return rc;
   AddNormParams p = {};
   p.x = x; p.r = r; p.w = w; p.y = y; p.h = h; p.rstd = rstd; p.scale = scale;
   p.x_stride = xs; p.r_stride = rs; p.y_stride = ys; p.h_stride = hs;
+  p.stages = pl.stages; p.status = dev->status_dev;
   p.M = M; p.N = static_cast<int>(N); p.w_dtype = w_dtype; p.eps = eps;
   p.group = group; p.groups_per_row = group ? static_cast<int>((N + group - 1) / group) : 1; p.e8m0 = e8m0 != 0;
   return launch(pl.fn, dim3(pl.grid), dim3(pl.threads), pl.smem, &p, static_cast<cudaStream_t>(stream));
@@ -183,7 +194,7 @@ size_t b200norm_add_rms_bwd_workspace_bytes(int64_t M, int64_t N, int io_dtype, 
   for (Layout layout : {kAligned, kOffset, kAny})  // whichever the buffers turn out to have
     for (bool has_dh : {false, true}) {
       Plan pl;
-      if (plan(*dev, t, kBwd, layout, 1, M, N, has_dh, &pl)) return 0;
+      if (plan(*dev, t, kBwd, layout, 1, M, N, has_dh, 0, &pl)) return 0;
       rows = std::max<int64_t>(rows, pl.grid);
     }
   return (static_cast<size_t>(rows) * N * sizeof(float) + 255) & ~static_cast<size_t>(255);
@@ -209,7 +220,7 @@ int b200norm_add_rms_bwd(const void* h, int64_t h_row_stride, const void* dy, in
   int period;
   const Layout layout = layout_of(bufs, 5, N, 16 / t->size_t_, w, &period);
   Plan pl;
-  if (int rc = plan(*dev, t, kBwd, layout, period, M, N, dh != nullptr, &pl)) return rc;
+  if (int rc = plan(*dev, t, kBwd, layout, period, M, N, dh != nullptr, 0, &pl)) return rc;
   AddNormParams p = {};
   p.x = dy; p.r = dh; p.w = w; p.y = dx; p.h = const_cast<void*>(h); p.rstd = const_cast<float*>(rstd); p.dr = dres;
   p.x_stride = dy_row_stride; p.r_stride = dh_row_stride; p.y_stride = dx_row_stride; p.h_stride = h_row_stride;
