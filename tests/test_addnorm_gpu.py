@@ -278,6 +278,36 @@ def test_fp8_rows_loop_and_layouts(group):
     check_fp8(x, None, None, 1e-6, group, False)
 
 
+def test_fp8_unlike_alignments():
+    g = torch.Generator(device=DEV).manual_seed(6)
+    for t in (F32, BF16):
+        base = torch.randn(40, 3000, generator=g, device=DEV).to(t)
+        for n in (33, 900, 2500):
+            for group, e8m0 in ((0, False), (32, True), (128, False)):
+                check_fp8(base[:, 1:1 + n], base[:, 40:40 + n], torch.ones(n + 1, device=DEV, dtype=t)[1:], 1e-6, group, e8m0)
+                check_fp8(base.t()[:n].t(), None, None, 1e-6, group, e8m0)
+
+
+@pytest.mark.parametrize("t,r", [(F32, None), (BF16, BF16), (F16, F32)])
+def test_fp8_many_rows_off_the_packets(t, r):
+    # scales whose columns begin and end inside packets, at every kind of row group
+    for M, N in [(70001, 33), (9001, 131), (4001, 777), (700, 4099), (301, 8191)]:
+        x, res, w, _, _ = make(M, N, t, r or t, F32, seed=N)
+        check_fp8(x, res if r else None, w, 1e-6, [0, 32, 64, 128][N % 4], N % 3 == 0)
+
+
+def test_fp8_overflowing_squares():
+    # the sum of squares is infinite and the norm 0, as RMSNorm's, though h * w overflows on the way
+    x = torch.full((3, 512), 3e38, device=DEV)
+    x[1, 5] = float("inf")
+    w = torch.full((512,), 2.0, device=DEV)
+    for xs in (x, x[:, :509]):
+        for group in (0, 64):
+            q, s = b200norm.rmsnorm_fp8(xs, w[:xs.shape[1]], 1e-6, group=group)
+            assert (q[[0, 2]].float() == 0).all() and s[[0, 2]].isfinite().all()
+            assert q[1, 5].float().isnan() and s[1, 0].isnan()
+
+
 def test_fp8_zero_rows_and_poison():
     x = torch.zeros(3, 256, device=DEV)
     x[1] = 1.0

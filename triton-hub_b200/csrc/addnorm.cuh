@@ -369,18 +369,21 @@ __device__ __forceinline__ float row_sum_max(float v, float& amax, float* scratc
 // only (its step is a multiple of the offsets' period), so that a thread's columns stay the same.
 // GROUP: the 8-bit form with a scale for so many columns, 0 for one a row; -1: the output is y.  Thread t of a
 // row group holds packets t, t + TPR, ...: neighbouring lanes hold neighbouring columns, so a scale's 32, 64 or
-// 128 columns are 4 to 32 adjacent lanes of one warp.
+// 128 columns are 4 to 32 adjacent lanes of one warp.  OFF: a packet may belong to two scales' columns, so the
+// maxima are found in shared memory, by one or two atomic maxima a packet; the columns per scale are those of p.group.
 // RING: as in the backward below, the rows of x and r arrive through p.stages shared-memory slots per row group.
 template <typename T, typename R, int LD, int TPR, bool OFF, int GROUP, bool RING>
 __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR, !OFF && (GROUP < 0 || (GROUP > 0 && RING))))
     addnorm_fwd_kernel(const AddNormParams p) {
-  constexpr bool FP8 = GROUP >= 0, PER_ROW = GROUP == 0;
-  static_assert(!(OFF && (FP8 || RING)), "scale groups lie on packet boundaries, and bulk copies take whole packets");
+  constexpr bool FP8 = GROUP >= 0, PER_ROW = GROUP == 0 && !OFF;
+  static_assert(!(OFF && RING) && !(OFF && GROUP > 0), "bulk copies take whole packets; rows off them read p.group");
   static_assert(!RING || TPR > 32, "a ring belongs to a group with a barrier");
   constexpr int VEC = Pack16<T>::kElems, H = VEC / 2;
   constexpr int GROUPS = addnorm_threads(TPR) / TPR;
+  constexpr int WARPS = TPR >= 32 ? TPR / 32 : 1;
   constexpr bool WREG = LD * VEC <= 16;  // the weights fit in registers next to the row
-  extern __shared__ __align__(128) unsigned char dyn[];  // OFF: the weights; RING: the slots
+  // OFF: the weights, and of the 8-bit form the maxima, two halves in turn per row group; RING: the slots
+  extern __shared__ __align__(128) unsigned char dyn[];
   float* ws = reinterpret_cast<float*>(dyn);
   __shared__ __align__(8) uint64_t bars[RING ? GROUPS : 1][kAddNormStages];
   __shared__ int cta_abort;
@@ -390,6 +393,10 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
   const int group = threadIdx.x / TPR, t = threadIdx.x % TPR;
   const int lane = threadIdx.x & 31, warp_n = TPR >= 32 ? t / 32 : 0;
   int phase = 0;
+  // PAIR: the row comes out of shared memory, where neighbouring packets cost nothing: a thread takes them two by two, which
+  // halves the work per scale.
+  constexpr bool PAIR = RING && GROUP > 0 && LD % 2 == 0;
+  auto packet = [&](int j) { return PAIR ? (j / 2 * TPR + t) * 2 + j % 2 : j * TPR + t; };
   if constexpr (TPR > 32) {
     for (int i = threadIdx.x; i < GROUPS * 2 * row_scratch(TPR); i += blockDim.x) {
       (&scratch[0][0])[i] = 0.f;
@@ -430,8 +437,12 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
   int slot = 0;
   uint32_t parity = 0;
 
+  uint32_t* maxima = reinterpret_cast<uint32_t*>(ws + w_slots<VEC>(p.N)) + (size_t)group * 2 * p.groups_per_row;
+  int half = 0;
   if constexpr (OFF) {
     stage_w<VEC>(p.w, p.w_dtype, p.N, ws);
+    if (FP8)
+      for (int i = t; i < 2 * p.groups_per_row; i += TPR) maxima[i] = 0u;
     __syncthreads();
   }
   auto weights = [&](int c0, float2* f) {
@@ -442,7 +453,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
   if constexpr (WREG) {
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
-      const int pk = j * TPR + t;
+      const int pk = packet(j);
       if (pk < packets) weights(pk * VEC - off, wr[j]);
     }
   }
@@ -461,7 +472,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
       if constexpr (RING) mbar_wait(&bars[group][slot], parity, &cta_abort, p.status);
 #pragma unroll
       for (int j = 0; j < LD; ++j) {
-        const int pk = j * TPR + t;
+        const int pk = packet(j);
         xv[j].zero();
         rv[j].zero();
         if (!valid || pk >= packets) continue;
@@ -475,7 +486,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
       }
 #pragma unroll
       for (int j = 0; j < LD; ++j) {
-        const int pk = j * TPR + t;
+        const int pk = packet(j);
         xv[j].unpack(hf[j]);
         if (p.r != nullptr) {
           float2 rf[H];
@@ -499,7 +510,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
 #pragma unroll
         for (int k = 0; k < H; ++k) wf[k] = wr[j][k];
       } else {
-        weights((j * TPR + t) * VEC - off, wf);
+        weights(packet(j) * VEC - off, wf);
       }
     };
     // One scale a row: max |y| is rstd * max |h w|, so the maximum is found along with the sum.
@@ -507,7 +518,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
     if constexpr (PER_ROW) {
 #pragma unroll
       for (int j = 0; j < LD; ++j) {
-        if (j * TPR + t >= packets) continue;
+        if (packet(j) >= packets) continue;
         float2 wf[H];
         w_of(j, wf);
 #pragma unroll
@@ -534,7 +545,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
     float amax_j[FP8 ? LD : 1];
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
-      const int pk = j * TPR + t;
+      const int pk = packet(j);
       if constexpr (FP8) amax_j[j] = 0.f;
       if (pk >= packets) continue;
       float2 wf[H];
@@ -545,7 +556,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
         RawVec<T, VEC> o;
         o.pack(hf[j]);
         if (valid) ys.store(row, pk * VEC - off, o);
-      } else if constexpr (!PER_ROW) {
+      } else if constexpr (!PER_ROW && !OFF) {
         float a = 0.f;
 #pragma unroll
         for (int k = 0; k < H; ++k) a = max_abs3(a, hf[j][k].x, hf[j][k].y);
@@ -553,7 +564,74 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
       }
     }
 
-    if constexpr (FP8) {
+    if constexpr (FP8 && OFF) {
+      // Bit patterns of magnitudes order like the magnitudes, NaN above all.
+      const int span = p.group == 0 ? p.N : p.group;
+      uint32_t* mx = maxima + half * p.groups_per_row;
+      auto parts = [&](int c0, int& g0, int& cut) {  // a packet's first scale, and its elements from which the next one holds
+        const int c = max(c0, 0);
+        g0 = p.group == 0 ? 0 : c / span;
+        cut = (g0 + 1) * span - c0;
+      };
+      float whole = 0.f;
+#pragma unroll
+      for (int j = 0; j < LD; ++j) {
+        const int pk = packet(j), c0 = pk * VEC - off;
+        if (!valid || pk >= packets) continue;
+        int g0, cut;
+        parts(c0, g0, cut);
+        float lo = 0.f, hi = 0.f;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float v = (e & 1) ? hf[j][e / 2].y : hf[j][e / 2].x;
+          if (e < cut) lo = max_abs(lo, v);
+          else hi = max_abs(hi, v);
+        }
+        if (p.group == 0) {
+          whole = max_abs(whole, lo);
+        } else {
+          atomicMax(&mx[g0], __float_as_uint(lo));
+          if (cut < VEC && g0 + 1 < p.groups_per_row) atomicMax(&mx[g0 + 1], __float_as_uint(hi));
+        }
+      }
+      if (p.group == 0 && valid) atomicMax(&mx[0], __float_as_uint(whole));
+      if constexpr (TPR > 32) group_sync<WARPS, 0>(group);
+      else __syncwarp();
+      // the other half is free: every thread is past the row before
+      uint32_t* other = maxima + (half ^ 1) * p.groups_per_row;
+      for (int g = t; g < p.groups_per_row; g += TPR) {
+        if (valid) store_scale(p.scale, row * p.groups_per_row + g, fp8_scale(__uint_as_float(mx[g]), p.e8m0 != 0), p.e8m0 != 0);
+        other[g] = 0u;
+      }
+      if constexpr (TPR <= 32) __syncwarp();  // wider groups meet at the next row's first barrier
+      half ^= 1;
+      uint8_t* qrow = static_cast<uint8_t*>(p.y) + row * p.y_stride;
+#pragma unroll
+      for (int j = 0; j < LD; ++j) {
+        const int pk = packet(j), c0 = pk * VEC - off;
+        if (!valid || pk >= packets) continue;
+        int g0, cut;
+        parts(c0, g0, cut);
+        const float lo = fp8_scale(__uint_as_float(mx[g0]), p.e8m0 != 0).inv;
+        const float hi = cut < VEC && g0 + 1 < p.groups_per_row ? fp8_scale(__uint_as_float(mx[g0 + 1]), p.e8m0 != 0).inv : lo;
+        uint32_t word[VEC / 4];
+#pragma unroll
+        for (int k = 0; k < VEC / 4; ++k) {
+          const float2 a = hf[j][2 * k], b = hf[j][2 * k + 1];
+          word[k] = fp8x2(a.x * (4 * k < cut ? lo : hi), a.y * (4 * k + 1 < cut ? lo : hi)) |
+                    (fp8x2(b.x * (4 * k + 2 < cut ? lo : hi), b.y * (4 * k + 3 < cut ? lo : hi)) << 16);
+        }
+        if (c0 >= 0 && c0 + VEC <= p.N) {
+          if constexpr (VEC == 8) __stcs(reinterpret_cast<uint2*>(qrow + c0), make_uint2(word[0], word[1]));
+          else __stcs(reinterpret_cast<uint32_t*>(qrow + c0), word[0]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (c0 + e >= 0 && c0 + e < p.N) qrow[c0 + e] = static_cast<uint8_t>(word[e / 4] >> (8 * (e & 3)));
+        }
+      }
+    }
+    if constexpr (FP8 && !OFF) {
       uint8_t* qrow = static_cast<uint8_t*>(p.y) + row * p.y_stride;
       Fp8Scale sc;
       if constexpr (PER_ROW) {
@@ -573,12 +651,14 @@ __global__ void __launch_bounds__(addnorm_threads(TPR), addnorm_fwd_ctas(LD, TPR
         sc = fp8_scale(amax, p.e8m0 != 0);
         if (t == 0 && valid) store_scale(p.scale, row, sc, p.e8m0 != 0);
       }
-      constexpr int LANES = PER_ROW ? 1 : (GROUP / VEC < TPR ? GROUP / VEC : TPR);  // adjacent lanes that share a scale
+      constexpr int SPAN = PAIR ? 2 * VEC : VEC;  // neighbouring columns of a thread
+      constexpr int LANES = PER_ROW ? 1 : (GROUP / SPAN < TPR ? GROUP / SPAN : TPR);  // adjacent lanes that share a scale
 #pragma unroll
       for (int j = 0; j < LD; ++j) {
-        const int pk = j * TPR + t;
-        if constexpr (!PER_ROW) {
+        const int pk = packet(j);
+        if (!PER_ROW && !(PAIR && j % 2 == 1)) {
           float a = amax_j[j];
+          if constexpr (PAIR) a = max_abs(a, amax_j[j + 1 < LD ? j + 1 : j]);
 #pragma unroll
           for (int o = 1; o < LANES; o <<= 1) a = max_abs(a, __shfl_xor_sync(0xffffffffu, a, o));
           sc = fp8_scale(a, p.e8m0 != 0);
@@ -985,6 +1065,7 @@ struct AddNormShape {
   int ld, tpr;
   const void* fwd[2];  // [rows at a common offset]
   const void* fp8[4];  // a scale per row, 32, 64, 128 columns
+  const void* fp8_offset;
   const void* bwd[2];
   const void* fp8_ring[4];  // null: none
   const void* bwd_ring;

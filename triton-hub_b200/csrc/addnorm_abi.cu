@@ -84,17 +84,20 @@ int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, in
   const int64_t need = layout == kOffset ? (N + 2 * vec - 2) / vec : (N + vec - 1) / vec;
   const AddNormShape* s = nullptr;
   out->stages = 0;
-  if (layout == kAligned || (layout == kOffset && which != kFp8))
+  if (layout != kAny)
     for (int i = 0; i < t->n && s == nullptr; ++i)
       if (t->shapes[i].capacity() >= need) s = &t->shapes[i];
   int groups = 1;
   out->smem = 0;
   if (s != nullptr) {
     groups = s->groups();
-    out->fn = which == kFwd ? s->fwd[layout] : which == kFp8 ? s->fp8[scale_kind(group)] : s->bwd[layout];
+    out->fn = which == kFwd ? s->fwd[layout] : which == kBwd ? s->bwd[layout]
+              : layout == kOffset ? s->fp8_offset : s->fp8[scale_kind(group)];
     out->threads = s->threads();
     if (layout == kOffset) out->smem = sizeof(float) * (vec == 8 ? w_slots<8>(static_cast<int>(N)) : w_slots<4>(static_cast<int>(N)));
-    if (which == kFp8 && s->fp8_ring[0] != nullptr && M > (int64_t)dev.sm_count * groups) {
+    if (which == kFp8 && layout == kOffset)  // the maxima, two halves per row group
+      out->smem += sizeof(uint32_t) * 2 * groups * (group ? (N + group - 1) / group : 1);
+    if (which == kFp8 && layout == kAligned && s->fp8_ring[0] != nullptr && M > (int64_t)dev.sm_count * groups) {
       size_t ring = 0;
       out->stages = ring_stages(static_cast<size_t>(N) * (t->size_t_ + (has_residual ? t->size_r : 0)), 0, groups, &ring);
       if (out->stages > 0) {
