@@ -89,13 +89,13 @@ class route(torch.autograd.Function):
     def apply(cls, logits, k, normalize=True, mask=None):
         if not torch.is_grad_enabled():  # nothing to record: a decode step's call is spared autograd's bookkeeping
             gates, experts, counts, loss, _ = _route_fwd(logits, k, normalize, mask, need_lse=False)
-            return gates, experts, counts[:-1], loss
+            return gates, experts, counts.narrow(0, 0, logits.shape[-1]), loss
         return super().apply(logits, k, normalize, mask)
 
     @staticmethod
     def forward(ctx, logits, k, normalize=True, mask=None):
         gates, experts, counts, loss, lse = _route_fwd(logits, k, normalize, mask, need_lse=ctx.needs_input_grad[0])
-        chosen = counts[:-1]
+        chosen = counts.narrow(0, 0, logits.shape[-1])
         ctx.mark_non_differentiable(experts, chosen)
         ctx.set_materialize_grads(False)
         if ctx.needs_input_grad[0]:

@@ -7,8 +7,9 @@
 namespace b200norm {
 namespace {
 
-// A single CTA finishes on its own, in one launch: up to this many tokens it is quicker than two launches.
-constexpr int64_t kRouteAloneTokens = 4 * kRouteWarps;
+// Up to this many tokens, two a warp, the grid is one cluster, which finishes in one launch and without a workspace: 128 x 64
+// takes 5 us, with two launches 7; 256 x 64 6.6 and 7.1.
+constexpr int64_t kRouteClusterTokens = 2 * kRouteMaxCluster * kRouteWarps;
 
 const void* route_fn(int dtype, int E, bool bwd) {
 #define B200NORM_ROUTE(EPL)                                                                                    \
@@ -45,14 +46,21 @@ int columns_of(int E) { return (E + 3) / 4 * 4; }
 
 size_t fwd_smem(int E) { return (static_cast<size_t>(kRouteWarps + 1) * columns_of(E) + 1) * 4; }
 
-// Partial rows of the sums and of the counts, and the live tokens, of every CTA; 1 for the CTA that is alone.
-size_t workspace_need(int grid, int E) { return grid == 1 ? 1 : static_cast<size_t>(grid) * (2 * columns_of(E) + 1) * 4; }
+// Partial rows of the sums and of the counts, and the live tokens, of every CTA; 1 for a cluster.
+size_t workspace_need(int grid, int cluster, int E) {
+  return cluster > 0 ? 1 : static_cast<size_t>(grid) * (2 * columns_of(E) + 1) * 4;
+}
 
-int fwd_grid(DeviceState& dev, const void* fn, int64_t T, int E, int* grid) {
-  int occ;
+int fwd_grid(DeviceState& dev, const void* fn, int64_t T, int E, int* grid, int* cluster) {
+  int occ;  // also raises the kernel's shared-memory allowance
   if (int rc = occupancy(dev, fn, kRouteThreads, fwd_smem(E), &occ)) return rc;
-  const int64_t want = (T + kRouteWarps - 1) / kRouteWarps;
-  *grid = T <= kRouteAloneTokens ? 1 : static_cast<int>(std::min<int64_t>(want, (int64_t)dev.sm_count * occ));
+  const int64_t want = std::max<int64_t>(1, (T + kRouteWarps - 1) / kRouteWarps);
+  *cluster = 0;
+  if (T <= kRouteClusterTokens) {
+    *cluster = 1;
+    while (*cluster < std::min<int64_t>(want, kRouteMaxCluster)) *cluster *= 2;
+  }
+  *grid = *cluster > 0 ? *cluster : static_cast<int>(std::min<int64_t>(want, (int64_t)dev.sm_count * occ));
   return B200NORM_OK;
 }
 
@@ -67,9 +75,9 @@ size_t b200norm_route_workspace_bytes(int64_t T, int E, int k, int dtype) {
   if (check(T, E, k, dtype)) return 0;
   DeviceState* dev = nullptr;
   if (device_caches(&dev)) return 0;
-  int grid;
-  if (fwd_grid(*dev, route_fn(dtype, E, false), T, E, &grid)) return 0;
-  return workspace_need(grid, E);
+  int grid, cluster;
+  if (fwd_grid(*dev, route_fn(dtype, E, false), T, E, &grid, &cluster)) return 0;
+  return workspace_need(grid, cluster, E);
 }
 
 int b200norm_route_fwd(const void* logits, int64_t row_stride, const uint8_t* mask, float* gates, int* experts, float* lse,
@@ -81,10 +89,10 @@ int b200norm_route_fwd(const void* logits, int64_t row_stride, const uint8_t* ma
   DeviceState* dev = nullptr;
   if (int rc = device_caches(&dev)) return rc;
   const void* fn = route_fn(dtype, E, false);
-  int grid;
-  if (int rc = fwd_grid(*dev, fn, T, E, &grid)) return rc;
-  const size_t need = workspace_need(grid, E);
-  if (grid > 1 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
+  int grid, cluster;
+  if (int rc = fwd_grid(*dev, fn, T, E, &grid, &cluster)) return rc;
+  const size_t need = workspace_need(grid, cluster, E);
+  if (cluster == 0 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u)))
     return fail(B200NORM_ERR_ARG, "workspace needs %zu bytes, 16-byte aligned (got %zu)", need, workspace_bytes);
   RouteParams p = {};
   p.logits = logits; p.stride = row_stride; p.mask = mask; p.gates = gates; p.experts = experts; p.lse = lse;
@@ -94,10 +102,12 @@ int b200norm_route_fwd(const void* logits, int64_t row_stride, const uint8_t* ma
   p.part_n = reinterpret_cast<int*>(p.part_p + static_cast<size_t>(grid) * p.columns);
   p.part_live = p.part_n + static_cast<size_t>(grid) * p.columns;
   p.T = T; p.E = E; p.k = k; p.normalize = normalize != 0; p.parts = grid;
+  p.cluster = cluster;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-  if (int rc = launch(fn, dim3(grid), dim3(kRouteThreads), fwd_smem(E), &p, stream)) return rc;
-  if (grid == 1) return B200NORM_OK;
-  return launch(reinterpret_cast<const void*>(&route_finish_kernel), dim3(1), dim3(kRouteFinishThreads), 0, &p, stream);
+  if (int rc = launch(fn, dim3(grid), dim3(kRouteThreads), fwd_smem(E), &p, stream, true, std::max(cluster, 1))) return rc;
+  if (cluster > 0) return B200NORM_OK;
+  return launch(reinterpret_cast<const void*>(&route_finish_kernel), dim3(kRouteMaxCluster), dim3(kRouteFinishThreads),
+                0, &p, stream, true, kRouteMaxCluster);
 }
 
 int b200norm_route_bwd(const void* logits, int64_t row_stride, const float* gates, const int* experts, const float* lse,

@@ -12,10 +12,15 @@
 // fewer than k others exist, the slots left over hold -1 and gate 0.
 //
 // A warp takes a token; lane i holds the EPL neighbouring experts from i * EPL on, so the lowest of several
-// lanes with one maximum also has the lowest index.
+// lanes with one maximum also has the lowest index.  Reading the logits once is all that memory asks for (65536 x 128
+// fp32: 6 us); what bounds the forward is the instructions of the choice, the exponentials and the sums, some 400 a token
+// (44 us, 36 of them in route_fwd_kernel), and the backward (16 us for 10 us of traffic) their share of it.  Column sums of p
+// stay in registers over all of a warp's tokens and meet once per CTA, in shared memory; counts are shared-memory integer
+// atomics, whose order cannot show; the CTAs' partial rows are added in one fixed order.
 #pragma once
 
 #include "norm_common.cuh"
+#include "norm_stage.cuh"
 
 namespace b200norm {
 
@@ -25,6 +30,7 @@ constexpr int kRouteBwdThreads = 256;
 constexpr int kRouteBwdWarps = kRouteBwdThreads / 32;
 constexpr int kRouteMaxExperts = 1024;
 constexpr int kRouteMaxK = 32;
+constexpr int kRouteMaxCluster = 8;
 
 struct RouteParams {
   const void* logits;
@@ -46,7 +52,12 @@ struct RouteParams {
   void* dlogits;       // (T, E) contiguous
   int64_t T;
   int E, k, normalize, parts;
+  int cluster;  // CTAs of the forward's one cluster, which finishes by itself; 0: route_finish_kernel does
 };
+
+// exp(d) of a difference from the maximum: good to 2 ulp besides d's own rounding times d, like expf, in two instructions;
+// below 2^-126 it is 0.
+__device__ __forceinline__ float exp_below(float d) { return ex2_fast(d * kLog2e); }
 
 // Order-preserving integer of a float; -0 counts as +0.  -inf maps to kKeyNegInf, 0 is below every number.
 constexpr uint32_t kKeyNegInf = 0x007fffffu;
@@ -91,11 +102,13 @@ __device__ __forceinline__ void load_logits(const T* row, int E, int lane, bool 
 // The k rounds of "maximum over the warp".  After it lane r < c holds the r-th choice (its expert in `chosen`, its
 // logit in `chosen_x`), c = the number of choices returned: fewer than k when only -inf is left.
 //
-// Up to 8 experts a lane are sorted once, descending, by exchanges of neighbours, which keep equal ones in their order;
+// Two to 8 experts a lane are sorted once, descending, by exchanges of neighbours, which keep equal ones in their order;
 // a round then looks at the lanes' first keys only, and the lane that held the maximum moves its list up.  Which
 // expert it was is worked out once, after the rounds: the owner's list of indices and how often it was chosen before.
-// A round is a dozen instructions, most of them on the half-rate integer pipe, which is what bounds the kernel:
-// scanning all of a lane's keys in every round made 65536 x 128 fp32, k = 8, 56 us instead of 27.
+// A round is a dozen instructions, most of them on the half-rate integer pipe.  Scanning all of a lane's keys in every
+// round instead made the forward of 65536 x 128 fp32, k = 8, 55.6 us instead of 48.5 and of 32768 x 256 44.5 instead of
+// 39.7; of one expert a lane (65536 x 32, k = 2) 26.4 instead of 29.5, and 16 a lane (16384 x 512) take 39.2 scanned, 44.2
+// sorted.
 template <int EPL>
 __device__ __forceinline__ int route_choose(const float (&x)[EPL], int k, int lane, float& top, int& chosen, float& chosen_x) {
   uint32_t key[EPL];
@@ -103,7 +116,7 @@ __device__ __forceinline__ int route_choose(const float (&x)[EPL], int k, int la
   for (int i = 0; i < EPL; ++i) key[i] = order_key(x[i]);
   uint32_t mine = 0;
   int r = 0;
-  if constexpr (EPL <= 8) {
+  if constexpr (EPL > 1 && EPL <= 8) {
     uint32_t id[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; ++i) id[i] = i;
@@ -154,7 +167,7 @@ __device__ __forceinline__ int route_choose(const float (&x)[EPL], int k, int la
       if (r == 0) top = key_value(most);
       if (most <= kKeyNegInf) break;
       const int owner = __ffs(__ballot_sync(0xffffffffu, best == most)) - 1;
-      const int e = __shfl_sync(0xffffffffu, lane * EPL + at, owner);
+      const int e = EPL == 1 ? owner : __shfl_sync(0xffffffffu, lane * EPL + at, owner);
       if (lane == r) {
         chosen = e;
         mine = most;
@@ -170,12 +183,26 @@ __device__ __forceinline__ int route_choose(const float (&x)[EPL], int k, int la
   return r;
 }
 
-// Counts, the number of live tokens and the loss from the sums of p and the counts of every expert: `sum(e)`, `count(e)`.
+// A word of the same variable in CTA c of the cluster.
+template <typename V>
+__device__ __forceinline__ V ld_cluster(const V* own, int c) {
+  static_assert(sizeof(V) == 4, "32-bit words");
+  uint32_t v;
+  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(cluster_map(smem_addr(own), c)) : "memory");
+  return reinterpret_cast<const V&>(v);
+}
+
+__device__ __forceinline__ void st_cluster_f64(uint32_t addr, double v) {
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
+}
+
+// The counts of experts e0 .. e1 - 1, from `count(e)`, and in thread 0 the sum over them of count(e) * sum(e), which is the sum
+// of p over the tokens.
 template <int THREADS, typename Sum, typename Count>
-__device__ __forceinline__ void route_loss(const RouteParams& p, int n, Sum sum, Count count) {
+__device__ __forceinline__ double route_share(const RouteParams& p, int e0, int e1, Sum sum, Count count) {
   __shared__ double red[THREADS / 32];
   double share = 0.;
-  for (int e = threadIdx.x; e < p.E; e += THREADS) {
+  for (int e = e0 + threadIdx.x; e < e1; e += THREADS) {
     const int c = count(e);
     p.counts[e] = c;
     share += static_cast<double>(sum(e)) * c;
@@ -184,13 +211,17 @@ __device__ __forceinline__ void route_loss(const RouteParams& p, int n, Sum sum,
   for (int o = 16; o > 0; o >>= 1) share += __shfl_xor_sync(0xffffffffu, share, o);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = share;
   __syncthreads();
+  double total = 0.;
   if (threadIdx.x == 0) {
-    double total = 0.;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) total += red[w];
-    p.counts[p.E] = n;
-    *p.loss = n > 0 ? static_cast<float>(total * p.E / (static_cast<double>(n) * n * p.k)) : 0.f;
   }
+  return total;
+}
+// One thread: the number of live tokens and the loss.
+__device__ __forceinline__ void route_loss(const RouteParams& p, int n, double share) {
+  p.counts[p.E] = n;
+  *p.loss = n > 0 ? static_cast<float>(share * p.E / (static_cast<double>(n) * n * p.k)) : 0.f;
 }
 
 template <typename T, int EPL>
@@ -215,13 +246,18 @@ __global__ void __launch_bounds__(kRouteThreads, EPL <= 8 ? 2 : 1) route_fwd_ker
   const int64_t step = (int64_t)gridDim.x * kRouteWarps;
   int64_t tok = (int64_t)blockIdx.x * kRouteWarps + warp;
   float nx[EPL];
-  if (tok < p.T) load_logits<T, EPL>(logits + tok * p.stride, p.E, lane, packed, nx);
+  uint8_t next_on = 1;
+  auto fetch = [&](int64_t at) {
+    load_logits<T, EPL>(logits + at * p.stride, p.E, lane, packed, nx);
+    if (p.mask != nullptr) next_on = p.mask[at];
+  };
+  if (tok < p.T) fetch(tok);
   for (; tok < p.T; tok += step) {
     float x[EPL];
 #pragma unroll
     for (int i = 0; i < EPL; ++i) x[i] = nx[i];
-    if (tok + step < p.T) load_logits<T, EPL>(logits + (tok + step) * p.stride, p.E, lane, packed, nx);
-    const bool masked = p.mask != nullptr && p.mask[tok] == 0;
+    const bool masked = next_on == 0;
+    if (tok + step < p.T) fetch(tok + step);
 
     float top = 0.f, chosen_x = 0.f;
     int chosen = -1;
@@ -230,11 +266,11 @@ __global__ void __launch_bounds__(kRouteThreads, EPL <= 8 ? 2 : 1) route_fwd_ker
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      x[i] = expf(x[i] - top);
+      x[i] = exp_below(x[i] - top);
       s += x[i];
     }
     s = warp_sum(s);
-    float gate = chosen >= 0 ? expf(chosen_x - top) : 0.f;
+    float gate = chosen >= 0 ? exp_below(chosen_x - top) : 0.f;
     float total = s;
     if (p.normalize) {
       total = gate;
@@ -242,14 +278,14 @@ __global__ void __launch_bounds__(kRouteThreads, EPL <= 8 ? 2 : 1) route_fwd_ker
     }
     if (lane < p.k) {
       const bool choice = live && chosen >= 0;
-      p.gates[tok * p.k + lane] = choice ? gate / total : 0.f;
+      p.gates[tok * p.k + lane] = choice ? gate * rcp_fast(total) : 0.f;
       p.experts[tok * p.k + lane] = choice ? chosen : -1;
       if (choice) atomicAdd(&counts[chosen], 1);
     }
     if (p.lse != nullptr && lane == 0) p.lse[tok] = live ? top + logf(s) : -INFINITY;
     if (live) {
       ++live_tokens;
-      const float inv = 1.f / s;
+      const float inv = rcp_fast(s);  // s >= 1
 #pragma unroll
       for (int i = 0; i < EPL; ++i) acc[i] = fmaf(x[i], inv, acc[i]);
     }
@@ -265,8 +301,20 @@ __global__ void __launch_bounds__(kRouteThreads, EPL <= 8 ? 2 : 1) route_fwd_ker
     for (int w = 0; w < kRouteWarps; ++w) s += sums[(size_t)w * p.columns + e];
     return s;
   };
-  if (gridDim.x == 1) {  // a single CTA finishes by itself: no second launch
-    route_loss<kRouteThreads>(p, counts[p.columns], cta_sum, [&](int e) { return counts[e]; });
+  if (p.cluster > 0) {  // the grid is one cluster: its first CTA adds up the others' rows
+    for (int e = threadIdx.x; e < p.E; e += kRouteThreads) sums[e] = cta_sum(e);  // column e is this thread's alone
+    if (p.cluster > 1) cluster_sync_all();
+    else __syncthreads();
+    if (blockIdx.x == 0) {
+      auto over_ctas = [&](auto* at, auto zero) {
+        for (int c = 0; c < p.cluster; ++c) zero += ld_cluster(at, c);
+        return zero;
+      };
+      const double share = route_share<kRouteThreads>(p, 0, p.E, [&](int e) { return over_ctas(sums + e, 0.f); },
+                                                      [&](int e) { return over_ctas(counts + e, 0); });
+      if (threadIdx.x == 0) route_loss(p, over_ctas(counts + p.columns, 0), share);
+    }
+    if (p.cluster > 1) cluster_sync_all();  // the others' shared memory has been read
     return;
   }
   for (int e = threadIdx.x; e < p.columns; e += kRouteThreads) {
@@ -276,51 +324,73 @@ __global__ void __launch_bounds__(kRouteThreads, EPL <= 8 ? 2 : 1) route_fwd_ker
   if (threadIdx.x == 0) p.part_live[blockIdx.x] = counts[p.columns];
 }
 
-// Adds the CTAs' partial rows, 16 bytes a thread and up to 32 rows side by side, every column in one fixed order.
+// Adds the CTAs' partial rows: a cluster, each of whose CTAs takes its share of the columns, 16 bytes a thread and as many rows
+// side by side as there are threads, then a warp a column; every column in one fixed order.  It is a chain of latencies: one
+// CTA for all columns took 6 us for 128 experts and 15 us for 1024, of 45 and 71 us in all.
 constexpr int kRouteFinishThreads = 1024;
 __global__ void __launch_bounds__(kRouteFinishThreads) route_finish_kernel(const RouteParams p) {
-  __shared__ float4 sum_s[kRouteFinishThreads];
-  __shared__ int4 count_s[kRouteFinishThreads];
-  __shared__ int live_s;
-  const int tid = threadIdx.x;
-  const int quads = p.columns / 4, groups = min(32, kRouteFinishThreads / quads);
-  const int q = tid % quads, g = tid / quads;
+  constexpr int MOST = kRouteMaxExperts / kRouteMaxCluster;  // columns of a CTA
+  constexpr int ROWS = 128;                                  // side by side, at most
+  constexpr int SLOTS = kRouteFinishThreads + ROWS;
+  __shared__ float4 sum_s[SLOTS];
+  __shared__ int4 count_s[SLOTS];
+  __shared__ float column_sum[MOST];
+  __shared__ int column_count[MOST];
+  __shared__ double shares[kRouteMaxCluster];  // of the first CTA: every CTA's part of the loss
+  const int tid = threadIdx.x, lane = tid & 31, rank = static_cast<int>(cluster_cta_rank());
+  const int quads = (p.columns / 4 + kRouteMaxCluster - 1) / kRouteMaxCluster;  // of a CTA, 16 bytes each
+  const int groups = min(min(ROWS, kRouteFinishThreads / quads), p.parts);
+  const int pitch = quads | 1;  // odd: a warp that reads down a column meets a bank four times, not 32
+  const int q = tid % quads, g = tid / quads, column = 4 * (rank * quads + q);
   grid_dependency_sync();
   trigger_dependents();
-  if (g < groups) {
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    int4 n = make_int4(0, 0, 0, 0);
-#pragma unroll 4
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  int4 n = make_int4(0, 0, 0, 0);
+  if (g < groups && column < p.columns) {
+#pragma unroll 2
     for (int r = g; r < p.parts; r += groups) {
-      const float4 a = *reinterpret_cast<const float4*>(p.part_p + (size_t)r * p.columns + 4 * q);
-      const int4 b = *reinterpret_cast<const int4*>(p.part_n + (size_t)r * p.columns + 4 * q);
+      const float4 a = *reinterpret_cast<const float4*>(p.part_p + (size_t)r * p.columns + column);
+      const int4 b = *reinterpret_cast<const int4*>(p.part_n + (size_t)r * p.columns + column);
       s.x += a.x; s.y += a.y; s.z += a.z; s.w += a.w;
       n.x += b.x; n.y += b.y; n.z += b.z; n.w += b.w;
     }
-    sum_s[g * quads + q] = s;
-    count_s[g * quads + q] = n;
   }
-  if (tid < 32) {
-    int n = 0;
-    for (int r = tid; r < p.parts; r += 32) n += p.part_live[r];
-    n = __reduce_add_sync(0xffffffffu, n);
-    if (tid == 0) live_s = n;
+  if (g < groups) {
+    sum_s[g * pitch + q] = s;
+    count_s[g * pitch + q] = n;
+  }
+  int live = 0;
+  if (rank == 0 && tid < 32) {
+    for (int r = tid; r < p.parts; r += 32) live += p.part_live[r];
+    live = __reduce_add_sync(0xffffffffu, live);
+  }
+  cluster_sync_all();
+  for (int c = tid >> 5; c < 4 * quads; c += kRouteFinishThreads / 32) {
+    float cs = 0.f;
+    int cn = 0;
+    for (int r = lane; r < groups; r += 32) {
+      cs += reinterpret_cast<const float*>(sum_s)[r * pitch * 4 + c];
+      cn += reinterpret_cast<const int*>(count_s)[r * pitch * 4 + c];
+    }
+    cs = warp_sum(cs);
+    cn = __reduce_add_sync(0xffffffffu, cn);
+    if (lane == 0) {
+      column_sum[c] = cs;
+      column_count[c] = cn;
+    }
   }
   __syncthreads();
-  const float* sums = reinterpret_cast<const float*>(sum_s);
-  const int* counts = reinterpret_cast<const int*>(count_s);
-  route_loss<kRouteFinishThreads>(
-      p, live_s,
-      [&](int e) {
-        float s = 0.f;
-        for (int r = 0; r < groups; ++r) s += sums[(size_t)r * p.columns + e];
-        return s;
-      },
-      [&](int e) {
-        int n = 0;
-        for (int r = 0; r < groups; ++r) n += counts[(size_t)r * p.columns + e];
-        return n;
-      });
+  const int first = min(rank * quads * 4, p.E), last = min(first + quads * 4, p.E);
+  const double share = route_share<kRouteFinishThreads>(p, first, last, [&](int e) { return column_sum[e - first]; },
+                                                        [&](int e) { return column_count[e - first]; });
+  if (tid == 0) st_cluster_f64(cluster_map(smem_addr(&shares[rank]), 0), share);
+  cluster_sync_all();
+  if (rank == 0 && tid == 0) {
+    double total = 0.;
+#pragma unroll
+    for (int c = 0; c < kRouteMaxCluster; ++c) total += shares[c];
+    route_loss(p, live, total);
+  }
 }
 
 // Backward: p comes from the logits and the saved log-sum, the chosen experts' part is put in its place
@@ -366,7 +436,7 @@ __global__ void __launch_bounds__(kRouteBwdThreads) route_bwd_kernel(const Route
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      x[i] = live ? expf(x[i] - lse) : 0.f;
+      x[i] = live ? exp_below(x[i] - lse) : 0.f;
       s = fmaf(x[i], c[i], s);
     }
     const bool any = e >= 0;

@@ -38,13 +38,18 @@ extern "C" int b200norm_sample(const void* logits, int64_t row_stride, const flo
   DeviceState* dev = nullptr;
   if (int rc = device_caches(&dev)) return rc;
   const int es = dtype == B200NORM_F32 ? 4 : 2, vec = 16 / es;
-  // CTAs per row: as few as let two of them share an SM's 228 KB (1 KB of it reserved per CTA, 14 KB static), so that one's
-  // barriers hide behind the other's arithmetic; and with few rows as many as there are SMs, while a part keeps 4096
-  // tokens.
-  constexpr int64_t kPart = 98 * 1024;
+  // CTAs per row: as few as have parts of up to 112 KB.  Parts of up to 98 KB let two CTAs share an SM (228 KB, 16 of it
+  // static or reserved per CTA), so that one's barriers hide behind the other's arithmetic, but each CTA has its fixed
+  // costs: top-p 0.9 of 512 x 65536 bf16 takes 238 us with 1 CTA a row, 189 with 2, 266 with 4; 512 x 50257 fp32 157 with 2
+  // parts of 98 KB and more, 214 with 4; 512 x 50257 bf16 144 with 1, 160 with 2.
+  // With few rows as many as there are SMs, while a part keeps 4096 tokens: one row of 32768 bf16 takes 34 us with 1 CTA,
+  // 25, 19 and 17 with 2, 4 and 8; one of 8192 is as quick with 1.
+  constexpr int64_t kPart = 112 * 1024;
+  constexpr int64_t kSplit = 16384;
   int cluster = 1;
   while (cluster < kSampleMaxCluster && V * es > cluster * kPart) cluster *= 2;
-  while (cluster < kSampleMaxCluster && M * cluster * 2 <= dev->sm_count && V >= (int64_t)cluster * 2 * 4096) cluster *= 2;
+  while (cluster < kSampleMaxCluster && M * cluster * 2 <= dev->sm_count && V >= std::max<int64_t>(kSplit, cluster * 2 * 4096))
+    cluster *= 2;
   SampleParams p = {};
   p.logits = logits; p.stride = row_stride; p.uniform = uniform;
   p.temperature_v = temperature_v; p.temperature = temperature;

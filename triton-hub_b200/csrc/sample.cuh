@@ -37,7 +37,7 @@ constexpr int kSampleBins = 2 * kSampleThreads;  // two a thread
 constexpr int kSampleMaxVocab = 1 << 18;
 constexpr int kSampleMaxCluster = 8;
 constexpr float kSampleBinsPerUnit = 32.f;
-constexpr int kSampleBound = 8192;  // a CTA with so many tokens bounds top-k's threshold before it counts
+constexpr int kSampleBound = 16384;  // a CTA with so many tokens bounds top-k's threshold before it counts
 constexpr int kSampleList = 256;  // tokens that are compared pairwise: all that may be drawn, or those of a threshold's bin
 
 struct SampleParams {
@@ -781,10 +781,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   }
   if (use_p) {
     // The weights above top-k's threshold; at it, `ties` tokens more.
-    // All tokens that weigh less than (1 - p) / V of the likeliest weigh less than 1 - p of the total together: the prefix
-    // ends before them.
-    const float beyond = 32.f * (log2f(static_cast<float>(p.V)) - log2f(1.f - fmaxf(top_p, 0.f))) + 2.f;
-    row.template fill_bins<true>(floor, static_cast<int>(fminf(beyond, static_cast<float>(kSampleBins - 2))));
+    row.template fill_bins<true>(floor, kSampleBins - 2);
     u64 total, need;
     row.template locate<true>(0, [&](u64 sum) {
       total = sum;
