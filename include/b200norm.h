@@ -20,6 +20,11 @@
  *   b200norm_softmax_fwd/_bwd                                  TritonHub/Activations/softmax.py, logsoftmax.py, softmin.py
  *   b200norm_pnorm_fwd/_bwd, b200norm_normalize_fwd/_bwd       TritonHub/Ops/norm.py, normalize.py
  *
+ * and for the steps of a language model around the same rows, which the reference does not have:
+ *
+ *   b200norm_add_rms_fwd/_bwd   the residual addition and RMSNorm in one;  b200norm_rms_fp8   with an 8-bit output and scales
+ *   b200norm_route_fwd/_bwd     the choice of experts from router logits;  b200norm_sample    the choice of a token
+ *
  * Conventions shared by every entry point
  *   - Rows are the flattened leading dimensions: x is (M, N) with unit column stride and a
  *     row stride given in ELEMENTS (>= N).  y, dy and dx likewise.

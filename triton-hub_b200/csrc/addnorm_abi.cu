@@ -64,7 +64,8 @@ struct Plan {
 };
 
 // Slots of a ring: as many, up to four, as leave room for three, two or one CTA per SM (228 KB, 1 KB of it
-// reserved per CTA, and a little static shared memory), at least two; 0 when two do not fit.
+// reserved per CTA, and a little static shared memory), at least two; 0 when two do not fit.  Four slots always, with fewer
+// CTAs, is the same within 2 % (backward of 16384 x 4096 bf16 84.3 instead of 83.5 us, of 16384 x 1024 29.3 instead of 28.6).
 int ring_stages(size_t slot, size_t fixed, int groups, size_t* smem) {
   for (size_t cap : {74 * 1024, 112 * 1024, 224 * 1024})
     for (int stages = kAddNormStages; stages >= 2; --stages)
@@ -97,6 +98,7 @@ int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, in
     if (layout == kOffset) out->smem = sizeof(float) * (vec == 8 ? w_slots<8>(static_cast<int>(N)) : w_slots<4>(static_cast<int>(N)));
     if (which == kFp8 && layout == kOffset)  // the maxima, two halves per row group
       out->smem += sizeof(uint32_t) * 2 * groups * (group ? (N + group - 1) / group : 1);
+    // rows enough for a second round: 16 x 4096 bf16 takes 2.5 us without a ring and 2.7 with one, 1024 x 4096 5.4 and 5.3
     if (which == kFp8 && layout == kAligned && s->fp8_ring[0] != nullptr && M > (int64_t)dev.sm_count * groups) {
       size_t ring = 0;
       out->stages = ring_stages(static_cast<size_t>(N) * (t->size_t_ + (has_residual ? t->size_r : 0)), 0, groups, &ring);
