@@ -50,7 +50,8 @@ struct AddNormParams {
   int group;  // 8-bit form, element by element: columns per scale, 0 for one scale a row
   int groups_per_row;
   int e8m0;  // 8-bit form: scales are powers of two, stored as their biased exponent
-  int stages;   // backward with a ring: slots per row group
+  int stages;   // with a ring: slots per row group ...
+  int ring_at;  // ... and, 8-bit form, where in the dynamic shared memory they begin
   int* status;  // device status word for bounded waits that ran out
 };
 constexpr int kAddNormStages = 4;  // slots of a ring, at most
@@ -95,15 +96,6 @@ struct RawVec {
                    : "memory");
     }
   }
-  // Zeroes the elements whose column is outside a row of n.
-  __device__ __forceinline__ void mask(int c0, int n) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      if (c0 + e >= 0 && c0 + e < n) continue;
-      if constexpr (sizeof(E) == 4) w[e] = 0u;
-      else w[e / 2] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
-    }
-  }
   __device__ __forceinline__ void unpack(float2* f) const {
     if constexpr (sizeof(E) == 4) {
 #pragma unroll
@@ -126,57 +118,41 @@ struct RawVec {
   }
 };
 
-// A packet of which part lies outside its row, element by element.  Kept out of line: few packets come here.
+// Rows of one buffer.
 template <typename E, int VEC>
-__device__ __noinline__ RawVec<E, VEC> load_elements(const E* row, int c0, int n) {
-  RawVec<E, VEC> r;
-  r.zero();
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    if (c0 + e < 0 || c0 + e >= n) continue;
-    if constexpr (sizeof(E) == 4) r.w[e] = reinterpret_cast<const uint32_t*>(row)[c0 + e];
-    else r.w[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[c0 + e]) << (16 * (e & 1));
-  }
-  return r;
-}
-template <typename E, int VEC>
-__device__ __noinline__ void store_elements(E* row, int c0, int n, RawVec<E, VEC> r) {
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    if (c0 + e < 0 || c0 + e >= n) continue;
-    if constexpr (sizeof(E) == 4) reinterpret_cast<uint32_t*>(row)[c0 + e] = r.w[e];
-    else reinterpret_cast<uint16_t*>(row)[c0 + e] = static_cast<uint16_t>(r.w[e / 2] >> (16 * (e & 1)));
-  }
-}
-
-// Rows of one buffer.  OFF: a row's first and last packet may lie partly outside it.  A load then takes the
-// whole packet and masks it -- its other elements belong to the neighbouring row or to the gap before it -- unless
-// the packet leaves the buffer, which the first packet of the first row and the last of the last row may do.
-template <typename E, int VEC, bool OFF>
 struct Rows {
   E* base;
   int64_t stride;
-  int64_t size;  // elements from the first row's start to the last row's end
-  int n;
 
-  __device__ __forceinline__ Rows(const void* p, int64_t stride, int64_t m, int n)
-      : base(static_cast<E*>(const_cast<void*>(p))), stride(stride), size((m - 1) * stride + n), n(n) {}
+  __device__ __forceinline__ Rows(const void* p, int64_t stride) : base(static_cast<E*>(const_cast<void*>(p))), stride(stride) {}
+  __device__ __forceinline__ E* at(int64_t row, int c) const { return base + row * stride + c; }
   __device__ __forceinline__ RawVec<E, VEC> load(int64_t row, int c0) const {
     RawVec<E, VEC> r;
-    const int64_t at = row * stride + c0;
-    if constexpr (!OFF) {
-      r.load(base + at);
-    } else if (at >= 0 && at + VEC <= size) {
-      r.load(base + at);
-      if (c0 < 0 || c0 + VEC > n) r.mask(c0, n);
-    } else {
-      r = load_elements<E, VEC>(base + row * stride, c0, n);
-    }
+    r.load(at(row, c0));
     return r;
   }
-  __device__ __forceinline__ void store(int64_t row, int c0, const RawVec<E, VEC>& r) const {
-    if (!OFF || (c0 >= 0 && c0 + VEC <= n)) r.store(base + row * stride + c0);
-    else store_elements<E, VEC>(base + row * stride, c0, n, r);
+  __device__ __forceinline__ void store(int64_t row, int c0, const RawVec<E, VEC>& r) const { r.store(at(row, c0)); }
+};
+
+// How a row of n columns lies on packet boundaries when it starts `off` elements behind one: a head of up to VEC - 1
+// elements, whole packets, a tail of up to VEC - 1.  The packets are handled as those of an aligned row; the head's and the
+// tail's elements are dealt out singly, EDGES a thread, and everything is done for them beside the packets, without a branch
+// on their number.
+template <int VEC, int TPR, bool OFF>
+struct Span {
+  static constexpr int EDGES = OFF ? (2 * VEC - 2 + TPR - 1) / TPR : 0;
+  static constexpr int kSlots = OFF ? EDGES : 1;
+  int head, packets, edges;
+
+  __device__ __forceinline__ Span(int off, int n) {
+    head = OFF ? min((VEC - off) % VEC, n) : 0;
+    packets = (n - head) / VEC;
+    edges = n - packets * VEC;
+  }
+  // Column of a thread's k-th single element, or -1.
+  __device__ __forceinline__ int edge(int t, int k) const {
+    const int i = t + k * TPR;
+    return i >= edges ? -1 : i < head ? i : packets * VEC + i;
   }
 };
 
@@ -223,25 +199,25 @@ __device__ __forceinline__ void load_w(const void* p, int dtype, int c0, float2*
   for (int i = 0; i < VEC / 2; ++i) f[i] = make_float2(v[2 * i], v[2 * i + 1]);
 }
 
-// Rows off the packet boundaries: the parameters wait in shared memory as fp32, with a word left free after every
-// VEC of them so that the lanes' reads, VEC words apart, fall into different banks.
+// The same from any column, one by one.
 template <int VEC>
-__host__ __device__ constexpr int w_slots(int n) { return (n + n / VEC + 4) / 4 * 4; }
-template <int VEC>
-__device__ __forceinline__ void stage_w(const void* p, int dtype, int n, float* ws) {
-#pragma unroll 1
-  for (int c = threadIdx.x; c < n; c += blockDim.x) ws[c + c / VEC] = p != nullptr ? load_param(p, dtype, c) : 1.f;
+__device__ __forceinline__ void load_w_any(const void* p, int dtype, int c0, float2* f) {
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i)
+    f[i] = p == nullptr ? splat2(1.f) : make_float2(load_param(p, dtype, c0 + 2 * i), load_param(p, dtype, c0 + 2 * i + 1));
 }
+
+// Rows off the packet boundaries, too wide for the weights to stay in registers: the packets' weights wait in shared memory
+// as fp32, on packet boundaries like the rows' packets.
+__host__ __device__ constexpr int w_slots(int n) { return (n + 31) / 32 * 32; }
 template <int VEC>
-__device__ __forceinline__ void staged_w(const float* ws, int c0, int n, float2* f) {
-  float v[VEC];
+__device__ __forceinline__ void staged_w(const float* ws, int pk, float2* f) {
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    const int c = c0 + e;
-    v[e] = c >= 0 && c < n ? ws[c + c / VEC] : 0.f;
+  for (int i = 0; i < VEC / 4; ++i) {
+    const float4 q = reinterpret_cast<const float4*>(ws + pk * VEC)[i];
+    f[2 * i] = make_float2(q.x, q.y);
+    f[2 * i + 1] = make_float2(q.z, q.w);
   }
-#pragma unroll
-  for (int i = 0; i < VEC / 2; ++i) f[i] = make_float2(v[2 * i], v[2 * i + 1]);
 }
 
 // Maxima of magnitudes that keep a NaN, so that a poisoned group shows in its scale.
@@ -307,8 +283,8 @@ __host__ __device__ constexpr bool addnorm_wide(int ld, int vec, int tpr) { retu
 // CTAs per SM that the register allocation leaves room for: as many threads as run without spills, more (`lean`) where a
 // thread holds little.  Rows off the packet boundaries wait on their loads and barriers: lean made 8182 x 4101 bf16
 // forward 94 -> 79 us, 200000 x 100 backward 101 -> 81.
-__host__ __device__ constexpr int addnorm_fwd_ctas(int ld, int tpr, bool lean) {
-  const int n = (ld > 2 ? 512 : lean ? 1024 : 768) / addnorm_threads(tpr);
+__host__ __device__ constexpr int addnorm_fwd_ctas(int elements, int tpr, bool lean) {
+  const int n = (elements > 16 ? 512 : lean ? 1024 : 768) / addnorm_threads(tpr);
   return n < 1 ? 1 : n;
 }
 __host__ __device__ constexpr int addnorm_bwd_ctas(int ld, int tpr, bool lean) {
@@ -375,8 +351,7 @@ __device__ __forceinline__ float row_sum_max(float v, float& amax, float* scratc
 }
 
 // Forward.  OFF: the rows of all buffers start at one common offset within a packet that need not be
-// zero (contiguous tensors of an odd row length); packets are then laid on the buffers' own alignment,
-// the first and the last of a row are partial, and the launch gives every row group rows of one offset
+// zero (contiguous tensors of an odd row length); see Span.  The launch gives every row group rows of one offset
 // only (its step is a multiple of the offsets' period), so that a thread's columns stay the same.
 // GROUP: the 8-bit form with a scale for so many columns, 0 for one a row; -1: the output is y.  Thread t of a
 // row group holds packets t, t + TPR, ...: neighbouring lanes hold neighbouring columns, so a scale's 32, 64 or
@@ -385,16 +360,17 @@ __device__ __forceinline__ float row_sum_max(float v, float& amax, float* scratc
 // RING: as in the backward below, the rows of x and r arrive through p.stages shared-memory slots per row group.
 template <typename T, typename R, int LD, int TPR, bool OFF, int GROUP, bool RING>
 __global__ void __launch_bounds__(addnorm_threads(TPR),
-                                  addnorm_fwd_ctas(LD, TPR, OFF ? LD == 1 || TPR >= 160 : GROUP < 0 || (GROUP > 0 && RING)))
+                                  addnorm_fwd_ctas(LD * Pack16<T>::kElems, TPR, GROUP < 0 || ((OFF || GROUP > 0) && RING)))
     addnorm_fwd_kernel(const AddNormParams p) {
   constexpr bool FP8 = GROUP >= 0, PER_ROW = GROUP == 0 && !OFF;
-  static_assert(!(OFF && RING) && !(OFF && GROUP > 0), "bulk copies take whole packets; rows off them read p.group");
+  static_assert(!(OFF && GROUP > 0), "rows off the packets read p.group");
   static_assert(!RING || TPR > 32, "a ring belongs to a group with a barrier");
   constexpr int VEC = Pack16<T>::kElems, H = VEC / 2;
   constexpr int GROUPS = addnorm_threads(TPR) / TPR;
   constexpr int WARPS = TPR >= 32 ? TPR / 32 : 1;
   constexpr bool WREG = LD * VEC <= 16;  // the weights fit in registers next to the row
-  // OFF: the weights, and of the 8-bit form the maxima, two halves in turn per row group; RING: the slots
+  static_assert(!OFF || WREG || GROUPS == 1, "staged weights have one offset");
+  // OFF: the weights unless in registers, and of the 8-bit form the maxima, two halves in turn per row group; RING: the slots
   extern __shared__ __align__(128) unsigned char dyn[];
   float* ws = reinterpret_cast<float*>(dyn);
   __shared__ __align__(8) uint64_t bars[RING ? GROUPS : 1][kAddNormStages];
@@ -425,21 +401,24 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
   grid_dependency_sync();
   trigger_dependents();
 
-  const Rows<T, VEC, OFF> xs(p.x, p.x_stride, p.M, p.N), ys(p.y, p.y_stride, p.M, p.N);
-  const Rows<R, VEC, OFF> rs(p.r, p.r_stride, p.M, p.N), hs(p.h, p.h_stride, p.M, p.N);
+  const Rows<T, VEC> xs(p.x, p.x_stride), ys(p.y, p.y_stride);
+  const Rows<R, VEC> rs(p.r, p.r_stride), hs(p.h, p.h_stride);
   const int64_t first = (int64_t)blockIdx.x * GROUPS + group;
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   const int off = OFF ? static_cast<int>((reinterpret_cast<uintptr_t>(p.x) / sizeof(T) + first * p.x_stride) % VEC) : 0;
-  const int packets = (off + p.N + VEC - 1) / VEC;
+  const Span<VEC, TPR, OFF> span(off, p.N);
+  const int packets = span.packets, head = span.head;
   const float inv_n = 1.f / static_cast<float>(p.N);
 
-  const uint32_t x_bytes = p.N * sizeof(T), r_bytes = p.r != nullptr ? p.N * sizeof(R) : 0u;
-  unsigned char* slots = dyn + (size_t)group * p.stages * (x_bytes + r_bytes);
+  // a slot has room for as many packets as rows of any offset have; a row's own may be one fewer
+  const uint32_t x_bytes = p.N / VEC * VEC * sizeof(T), r_bytes = p.r != nullptr ? p.N / VEC * VEC * sizeof(R) : 0u;
+  unsigned char* slots = dyn + p.ring_at + (size_t)group * p.stages * (x_bytes + r_bytes);
   auto fill = [&](int s, int64_t row) {  // the group's first thread: x and r of a row into slot s
     unsigned char* dst = slots + (size_t)s * (x_bytes + r_bytes);
-    mbar_expect_tx(&bars[group][s], x_bytes + r_bytes);
-    bulk_load(dst, xs.base + row * xs.stride, x_bytes, &bars[group][s]);
-    if (p.r != nullptr) bulk_load(dst + x_bytes, rs.base + row * rs.stride, r_bytes, &bars[group][s]);
+    const uint32_t xb = packets * VEC * sizeof(T), rb = p.r != nullptr ? packets * VEC * sizeof(R) : 0u;
+    mbar_expect_tx(&bars[group][s], xb + rb);
+    bulk_load(dst, xs.at(row, head), xb, &bars[group][s]);
+    if (p.r != nullptr) bulk_load(dst + x_bytes, rs.at(row, head), rb, &bars[group][s]);
   };
   if constexpr (RING) {
     if (t == 0)
@@ -449,24 +428,35 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
   int slot = 0;
   uint32_t parity = 0;
 
-  uint32_t* maxima = reinterpret_cast<uint32_t*>(ws + w_slots<VEC>(p.N)) + (size_t)group * 2 * p.groups_per_row;
+  uint32_t* maxima = reinterpret_cast<uint32_t*>(ws + (WREG ? 0 : w_slots(p.N))) + (size_t)group * 2 * p.groups_per_row;
   int half = 0;
+  const int group_bits = 31 - __clz(p.group | 1);  // the columns per scale are a power of two
+  constexpr int EDGES = Span<VEC, TPR, OFF>::EDGES, SLOTS = Span<VEC, TPR, OFF>::kSlots;
+  int ec[SLOTS];  // the single elements' columns and weights
+  float ew[SLOTS];
   if constexpr (OFF) {
-    stage_w<VEC>(p.w, p.w_dtype, p.N, ws);
+#pragma unroll
+    for (int k = 0; k < EDGES; ++k) {
+      ec[k] = span.edge(t, k);
+      ew[k] = ec[k] >= 0 && p.w != nullptr ? load_param(p.w, p.w_dtype, ec[k]) : 1.f;
+    }
+    if constexpr (!WREG)
+      for (int i = threadIdx.x; i < packets * VEC; i += blockDim.x) ws[i] = p.w != nullptr ? load_param(p.w, p.w_dtype, head + i) : 1.f;
     if (FP8)
       for (int i = t; i < 2 * p.groups_per_row; i += TPR) maxima[i] = 0u;
-    __syncthreads();
+    if (!WREG || FP8) __syncthreads();
   }
-  auto weights = [&](int c0, float2* f) {
-    if constexpr (OFF) staged_w<VEC>(ws, c0, p.N, f);
-    else load_w<VEC>(p.w, p.w_dtype, c0, f);
+  auto weights = [&](int pk, float2* f) {
+    if constexpr (!OFF) load_w<VEC>(p.w, p.w_dtype, pk * VEC, f);
+    else if constexpr (WREG) load_w_any<VEC>(p.w, p.w_dtype, head + pk * VEC, f);
+    else staged_w<VEC>(ws, pk, f);
   };
   float2 wr[WREG ? LD : 1][H];
   if constexpr (WREG) {
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
       const int pk = packet(j);
-      if (pk < packets) weights(pk * VEC - off, wr[j]);
+      if (pk < packets) weights(pk, wr[j]);
     }
   }
 
@@ -477,7 +467,18 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
     const bool valid = TPR >= 32 || row < p.M;
 
     float2 hf[LD][H];
+    float eh[SLOTS];
     {
+      T xe[SLOTS];
+      R re[SLOTS];
+#pragma unroll
+      for (int k = 0; k < EDGES; ++k) {  // ahead of the wait for the packets
+        xe[k] = from_f32<T>(0.f);
+        re[k] = from_f32<R>(0.f);
+        if (!valid || ec[k] < 0) continue;
+        xe[k] = *xs.at(row, ec[k]);
+        if (p.r != nullptr) re[k] = *rs.at(row, ec[k]);
+      }
       RawVec<T, VEC> xv[LD];
       RawVec<R, VEC> rv[LD];
       const unsigned char* src = slots + (size_t)slot * (x_bytes + r_bytes);
@@ -492,8 +493,8 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
           xv[j].load_shared(src + (size_t)pk * VEC * sizeof(T));
           if (p.r != nullptr) rv[j].load_shared(src + x_bytes + (size_t)pk * VEC * sizeof(R));
         } else {
-          xv[j] = xs.load(row, pk * VEC - off);
-          if (p.r != nullptr) rv[j] = rs.load(row, pk * VEC - off);
+          xv[j] = xs.load(row, head + pk * VEC);
+          if (p.r != nullptr) rv[j] = rs.load(row, head + pk * VEC);
         }
       }
 #pragma unroll
@@ -507,7 +508,16 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
           for (int k = 0; k < H; ++k) hf[j][k] = add2(hf[j][k], rf[k]);
           rv[j].pack(hf[j]);
           if (sizeof(R) < 4) rv[j].unpack(hf[j]);  // the norm is that of h as stored
-          if (p.h != nullptr && valid && pk < packets) hs.store(row, pk * VEC - off, rv[j]);
+          if (p.h != nullptr && valid && pk < packets) hs.store(row, head + pk * VEC, rv[j]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < EDGES; ++k) {
+        eh[k] = to_f32(xe[k]);
+        if (p.r != nullptr) {
+          const R v = from_f32<R>(eh[k] + to_f32(re[k]));
+          eh[k] = to_f32(v);
+          if (p.h != nullptr && valid && ec[k] >= 0) *hs.at(row, ec[k]) = v;
         }
       }
     }
@@ -517,12 +527,14 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
     for (int j = 0; j < LD; ++j)
 #pragma unroll
       for (int k = 0; k < H; ++k) q2 = fma2(hf[j][k], hf[j][k], q2);
+#pragma unroll
+    for (int k = 0; k < EDGES; ++k) q2.x = fmaf(eh[k], eh[k], q2.x);
     auto w_of = [&](int j, float2* wf) {
       if constexpr (WREG) {
 #pragma unroll
         for (int k = 0; k < H; ++k) wf[k] = wr[j][k];
       } else {
-        weights(packet(j) * VEC - off, wf);
+        weights(packet(j), wf);
       }
     };
     // One scale a row: max |y| is rstd * max |h w|, so the maximum is found along with the sum.
@@ -567,7 +579,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
       if constexpr (!FP8) {
         RawVec<T, VEC> o;
         o.pack(hf[j]);
-        if (valid) ys.store(row, pk * VEC - off, o);
+        if (valid) ys.store(row, head + pk * VEC, o);
       } else if constexpr (!PER_ROW && !OFF) {
         float a = 0.f;
 #pragma unroll
@@ -576,19 +588,24 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
       }
     }
 
+#pragma unroll
+    for (int k = 0; k < EDGES; ++k) {
+      eh[k] = eh[k] * rstd * ew[k];
+      if (!FP8 && valid && ec[k] >= 0) *ys.at(row, ec[k]) = from_f32<T>(eh[k]);
+    }
+
     if constexpr (FP8 && OFF) {
       // Bit patterns of magnitudes order like the magnitudes, NaN above all.
-      const int span = p.group == 0 ? p.N : p.group;
       uint32_t* mx = maxima + half * p.groups_per_row;
+      auto group_of = [&](int c) { return p.group == 0 ? 0 : c >> group_bits; };
       auto parts = [&](int c0, int& g0, int& cut) {  // a packet's first scale, and its elements from which the next one holds
-        const int c = max(c0, 0);
-        g0 = p.group == 0 ? 0 : c / span;
-        cut = (g0 + 1) * span - c0;
+        g0 = group_of(c0);
+        cut = p.group == 0 ? VEC : (g0 + 1) * p.group - c0;
       };
       float whole = 0.f;
 #pragma unroll
       for (int j = 0; j < LD; ++j) {
-        const int pk = packet(j), c0 = pk * VEC - off;
+        const int pk = packet(j), c0 = head + pk * VEC;
         if (!valid || pk >= packets) continue;
         int g0, cut;
         parts(c0, g0, cut);
@@ -603,8 +620,14 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
           whole = max_abs(whole, lo);
         } else {
           atomicMax(&mx[g0], __float_as_uint(lo));
-          if (cut < VEC && g0 + 1 < p.groups_per_row) atomicMax(&mx[g0 + 1], __float_as_uint(hi));
+          if (cut < VEC) atomicMax(&mx[g0 + 1], __float_as_uint(hi));
         }
+      }
+#pragma unroll
+      for (int k = 0; k < EDGES; ++k) {
+        if (!valid || ec[k] < 0) continue;
+        if (p.group == 0) whole = max_abs(whole, eh[k]);
+        else atomicMax(&mx[group_of(ec[k])], __float_as_uint(max_abs(0.f, eh[k])));
       }
       if (p.group == 0 && valid) atomicMax(&mx[0], __float_as_uint(whole));
       if constexpr (TPR > 32) group_sync<WARPS, 0>(group);
@@ -620,12 +643,12 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
       uint8_t* qrow = static_cast<uint8_t*>(p.y) + row * p.y_stride;
 #pragma unroll
       for (int j = 0; j < LD; ++j) {
-        const int pk = packet(j), c0 = pk * VEC - off;
+        const int pk = packet(j), c0 = head + pk * VEC;
         if (!valid || pk >= packets) continue;
         int g0, cut;
         parts(c0, g0, cut);
         const float lo = fp8_scale(__uint_as_float(mx[g0]), p.e8m0 != 0).inv;
-        const float hi = cut < VEC && g0 + 1 < p.groups_per_row ? fp8_scale(__uint_as_float(mx[g0 + 1]), p.e8m0 != 0).inv : lo;
+        const float hi = cut < VEC ? fp8_scale(__uint_as_float(mx[g0 + 1]), p.e8m0 != 0).inv : lo;
         uint32_t word[VEC / 4];
 #pragma unroll
         for (int k = 0; k < VEC / 4; ++k) {
@@ -633,14 +656,14 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
           word[k] = fp8x2(a.x * (4 * k < cut ? lo : hi), a.y * (4 * k + 1 < cut ? lo : hi)) |
                     (fp8x2(b.x * (4 * k + 2 < cut ? lo : hi), b.y * (4 * k + 3 < cut ? lo : hi)) << 16);
         }
-        if (c0 >= 0 && c0 + VEC <= p.N) {
-          if constexpr (VEC == 8) __stcs(reinterpret_cast<uint2*>(qrow + c0), make_uint2(word[0], word[1]));
-          else __stcs(reinterpret_cast<uint32_t*>(qrow + c0), word[0]);
-        } else {
+        if constexpr (VEC == 8) __stcs(reinterpret_cast<uint2*>(qrow + c0), make_uint2(word[0], word[1]));
+        else __stcs(reinterpret_cast<uint32_t*>(qrow + c0), word[0]);
+      }
 #pragma unroll
-          for (int e = 0; e < VEC; ++e)
-            if (c0 + e >= 0 && c0 + e < p.N) qrow[c0 + e] = static_cast<uint8_t>(word[e / 4] >> (8 * (e & 3)));
-        }
+      for (int k = 0; k < EDGES; ++k) {
+        if (!valid || ec[k] < 0) continue;
+        const float inv = fp8_scale(__uint_as_float(mx[group_of(ec[k])]), p.e8m0 != 0).inv;
+        qrow[ec[k]] = static_cast<uint8_t>(fp8x2(eh[k] * inv, 0.f));
       }
     }
     if constexpr (FP8 && !OFF) {
@@ -707,16 +730,17 @@ template <typename T, typename R, int LD, int TPR, bool OFF, bool RING>
 __global__ void __launch_bounds__(addnorm_threads(TPR),
                                   addnorm_bwd_ctas(LD, TPR, (sizeof(R) == sizeof(T) && TPR >= 160) || (OFF && LD == 1)))
     addnorm_bwd_kernel(const AddNormParams p) {
-  static_assert(!RING || (!OFF && TPR > 32), "bulk copies take whole packets; a ring belongs to a group with a barrier");
+  static_assert(!RING || TPR > 32, "a ring belongs to a group with a barrier");
   constexpr int VEC = Pack16<T>::kElems, H = VEC / 2;
   constexpr int GROUPS = addnorm_threads(TPR) / TPR;
   constexpr bool WREG = LD * VEC <= 16;
   constexpr bool WIDE = addnorm_wide(LD, VEC, TPR);
-  // OFF: the weights; then the sums, WIDE [LD * VEC][TPR] or, of several groups, [GROUPS][N]; RING: the slots, which
-  // the sums of several groups reuse
+  static_assert(!OFF || WREG || GROUPS == 1, "staged weights have one offset");
+  // OFF: the weights unless in registers; then the sums, WIDE [LD * VEC][TPR] or, of several groups, [GROUPS][N]; RING: the
+  // slots, which the sums of several groups reuse
   extern __shared__ __align__(128) unsigned char dyn[];
   float* ws = reinterpret_cast<float*>(dyn);
-  float* acc = ws + (OFF ? w_slots<VEC>(p.N) : 0);
+  float* acc = ws + (OFF && !WREG ? w_slots(p.N) : 0);
   __shared__ __align__(16) float scratch[GROUPS][2 * row_scratch(TPR)];
   __shared__ __align__(8) uint64_t bars[RING ? GROUPS : 1][kAddNormStages];
   __shared__ int cta_abort;
@@ -737,37 +761,52 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
   grid_dependency_sync();
   trigger_dependents();
 
-  const Rows<T, VEC, OFF> gs(p.x, p.x_stride, p.M, p.N), dxs(p.y, p.y_stride, p.M, p.N);
-  const Rows<R, VEC, OFF> hs(p.h, p.h_stride, p.M, p.N), ds(p.r, p.r_stride, p.M, p.N), drs(p.dr, p.dr_stride, p.M, p.N);
+  const Rows<T, VEC> gs(p.x, p.x_stride), dxs(p.y, p.y_stride);
+  const Rows<R, VEC> hs(p.h, p.h_stride), ds(p.r, p.r_stride), drs(p.dr, p.dr_stride);
   const int64_t first = (int64_t)blockIdx.x * GROUPS + group;
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   const int off = OFF ? static_cast<int>((reinterpret_cast<uintptr_t>(p.x) / sizeof(T) + first * p.x_stride) % VEC) : 0;
-  const int packets = (off + p.N + VEC - 1) / VEC;
+  const Span<VEC, TPR, OFF> span(off, p.N);
+  const int packets = span.packets, head = span.head;
   const float inv_n = 1.f / static_cast<float>(p.N);
 
-  const uint32_t t_bytes = p.N * sizeof(T), r_bytes = p.N * sizeof(R);
+  // a slot has room for as many packets as rows of any offset have; a row's own may be one fewer
+  const uint32_t t_bytes = p.N / VEC * VEC * sizeof(T), r_bytes = p.N / VEC * VEC * sizeof(R);
   const uint32_t slot_bytes = t_bytes + r_bytes * (p.r != nullptr ? 2 : 1);
-  unsigned char* slots = dyn + (WIDE ? sizeof(float) * LD * VEC * TPR : 0) + (size_t)group * p.stages * slot_bytes;
+  unsigned char* slots = reinterpret_cast<unsigned char*>(acc + (WIDE ? LD * VEC * TPR : 0)) + (size_t)group * p.stages * slot_bytes;
   auto fill = [&](int s, int64_t row) {  // the group's first thread: dy, h, dh of a row into slot s
     unsigned char* dst = slots + (size_t)s * slot_bytes;
     uint64_t* bar = &bars[group][s];
-    mbar_expect_tx(bar, slot_bytes);
-    bulk_load(dst, gs.base + row * gs.stride, t_bytes, bar);
-    bulk_load(dst + t_bytes, hs.base + row * hs.stride, r_bytes, bar);
-    if (p.r != nullptr) bulk_load(dst + t_bytes + r_bytes, ds.base + row * ds.stride, r_bytes, bar);
+    const uint32_t tb = packets * VEC * sizeof(T), rb = packets * VEC * sizeof(R);
+    mbar_expect_tx(bar, tb + rb * (p.r != nullptr ? 2 : 1));
+    bulk_load(dst, gs.at(row, head), tb, bar);
+    bulk_load(dst + t_bytes, hs.at(row, head), rb, bar);
+    if (p.r != nullptr) bulk_load(dst + t_bytes + r_bytes, ds.at(row, head), rb, bar);
   };
   if constexpr (RING) {
     if (t == 0)
       for (int s = 0; s < p.stages; ++s)
         if (first + s * step < p.M) fill(s, first + s * step);
   }
+  constexpr int EDGES = Span<VEC, TPR, OFF>::EDGES, SLOTS = Span<VEC, TPR, OFF>::kSlots;
+  int ec[SLOTS];  // the single elements' columns, weights and dweight sums
+  float ew[SLOTS], edw[SLOTS];
   if constexpr (OFF) {
-    stage_w<VEC>(p.w, p.w_dtype, p.N, ws);
-    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < EDGES; ++k) {
+      ec[k] = span.edge(t, k);
+      ew[k] = ec[k] >= 0 && p.w != nullptr ? load_param(p.w, p.w_dtype, ec[k]) : 1.f;
+      edw[k] = 0.f;
+    }
+    if constexpr (!WREG) {
+      for (int i = threadIdx.x; i < packets * VEC; i += blockDim.x) ws[i] = p.w != nullptr ? load_param(p.w, p.w_dtype, head + i) : 1.f;
+      __syncthreads();
+    }
   }
-  auto weights = [&](int c0, float2* f) {
-    if constexpr (OFF) staged_w<VEC>(ws, c0, p.N, f);
-    else load_w<VEC>(p.w, p.w_dtype, c0, f);
+  auto weights = [&](int pk, float2* f) {
+    if constexpr (!OFF) load_w<VEC>(p.w, p.w_dtype, pk * VEC, f);
+    else if constexpr (WREG) load_w_any<VEC>(p.w, p.w_dtype, head + pk * VEC, f);
+    else staged_w<VEC>(ws, pk, f);
   };
   float2 wr[WREG ? LD : 1][H];
   float2 dw[WIDE ? 1 : LD][H];
@@ -775,7 +814,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
       const int pk = j * TPR + t;
-      if (pk < packets) weights(pk * VEC - off, wr[j]);
+      if (pk < packets) weights(pk, wr[j]);
     }
   }
   if constexpr (WIDE) {
@@ -796,6 +835,17 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
     const bool valid = TPR >= 32 || row < p.M;
     const float rstd = valid ? __ldg(p.rstd + row) : 0.f;
 
+    T ge[SLOTS];
+    R he[SLOTS], de[SLOTS];
+#pragma unroll
+    for (int k = 0; k < EDGES; ++k) {  // ahead of the wait for the packets
+      ge[k] = from_f32<T>(0.f);
+      he[k] = de[k] = from_f32<R>(0.f);
+      if (!valid || ec[k] < 0) continue;
+      ge[k] = *gs.at(row, ec[k]);
+      he[k] = *hs.at(row, ec[k]);
+      if (p.r != nullptr) de[k] = *ds.at(row, ec[k]);
+    }
     RawVec<T, VEC> gv[LD];
     RawVec<R, VEC> hv[LD], dv[LD];
     const unsigned char* src = slots + (size_t)slot * slot_bytes;
@@ -812,9 +862,9 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
         hv[j].load_shared(src + t_bytes + (size_t)pk * VEC * sizeof(R));
         if (p.r != nullptr) dv[j].load_shared(src + t_bytes + r_bytes + (size_t)pk * VEC * sizeof(R));
       } else {
-        gv[j] = gs.load(row, pk * VEC - off);
-        hv[j] = hs.load(row, pk * VEC - off);
-        if (p.r != nullptr) dv[j] = ds.load(row, pk * VEC - off);
+        gv[j] = gs.load(row, head + pk * VEC);
+        hv[j] = hs.load(row, head + pk * VEC);
+        if (p.r != nullptr) dv[j] = ds.load(row, head + pk * VEC);
       }
     }
     float2 s2 = splat2(0.f);
@@ -830,7 +880,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
 #pragma unroll
         for (int k = 0; k < H; ++k) wf[k] = wr[j][k];
       } else {
-        weights(pk * VEC - off, wf);
+        weights(pk, wf);
       }
 #pragma unroll
       for (int k = 0; k < H; ++k) {
@@ -843,6 +893,12 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
           dw[j][k] = add2(dw[j][k], a);
         }
       }
+    }
+#pragma unroll
+    for (int k = 0; k < EDGES; ++k) {
+      const float a = to_f32(ge[k]) * (to_f32(he[k]) * rstd);
+      s2.x = fmaf(ew[k], a, s2.x);
+      edw[k] += a;
     }
     const float c1 = row_sum<TPR, (GROUPS == 1 ? 0 : 1)>(s2.x + s2.y, scratch[group], phase, group, warp_n, lane) * inv_n;
     if constexpr (RING) {
@@ -866,18 +922,25 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
 #pragma unroll
         for (int k = 0; k < H; ++k) wf[k] = wr[j][k];
       } else {
-        weights(pk * VEC - off, wf);
+        weights(pk, wf);
       }
 #pragma unroll
       for (int k = 0; k < H; ++k) df[k] = fma2(mul2(wf[k], rs2), gf[k], fma2(hf[k], kh, df[k]));
       RawVec<T, VEC> o;
       o.pack(df);
-      dxs.store(row, pk * VEC - off, o);
+      dxs.store(row, head + pk * VEC, o);
       if constexpr (sizeof(R) != sizeof(T)) {
         RawVec<R, VEC> od;
         od.pack(df);
-        drs.store(row, pk * VEC - off, od);
+        drs.store(row, head + pk * VEC, od);
       }
+    }
+#pragma unroll
+    for (int k = 0; k < EDGES; ++k) {
+      if (!valid || ec[k] < 0) continue;
+      const float d = fmaf(ew[k] * rstd, to_f32(ge[k]), fmaf(to_f32(he[k]), kh.x, to_f32(de[k])));
+      *dxs.at(row, ec[k]) = from_f32<T>(d);
+      if constexpr (sizeof(R) != sizeof(T)) *drs.at(row, ec[k]) = from_f32<R>(d);
     }
   }
   if constexpr (RING) {
@@ -892,12 +955,14 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
     float* mine = acc + (size_t)group * p.N;
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
-      const int pk = j * TPR + t, c0 = pk * VEC - off;
+      const int pk = j * TPR + t, c0 = head + pk * VEC;
       if (pk >= packets) continue;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k)
-        if (!OFF || (c0 + k >= 0 && c0 + k < p.N)) mine[c0 + k] = (k & 1) ? dw[j][k / 2].y : dw[j][k / 2].x;
+      for (int k = 0; k < VEC; ++k) mine[c0 + k] = (k & 1) ? dw[j][k / 2].y : dw[j][k / 2].x;
     }
+#pragma unroll
+    for (int k = 0; k < EDGES; ++k)
+      if (ec[k] >= 0) mine[ec[k]] = edw[k];
     __syncthreads();
     for (int c = threadIdx.x; c < p.N; c += GROUPS * TPR) {
       float s = 0.f;
@@ -907,7 +972,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
   } else {
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
-      const int pk = j * TPR + t, c0 = pk * VEC - off;
+      const int pk = j * TPR + t, c0 = head + pk * VEC;
       if (pk >= packets) continue;
       float2 a[H];
 #pragma unroll
@@ -919,10 +984,12 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
         st_f32_pairs<H>(out + c0, a);
       } else {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k)
-          if (c0 + k >= 0 && c0 + k < p.N) out[c0 + k] = (k & 1) ? a[k / 2].y : a[k / 2].x;
+        for (int k = 0; k < VEC; ++k) out[c0 + k] = (k & 1) ? a[k / 2].y : a[k / 2].x;
       }
     }
+#pragma unroll
+    for (int k = 0; k < EDGES; ++k)
+      if (ec[k] >= 0) out[ec[k]] = edw[k];
   }
 }
 
@@ -1079,10 +1146,10 @@ struct AddNormShape {
   int ld, tpr;
   const void* fwd[2];  // [rows at a common offset]
   const void* fp8[4];  // a scale per row, 32, 64, 128 columns
-  const void* fp8_offset;
-  const void* bwd[2];
+  const void* fp8_offset[2];  // [with a ring]; null: none
   const void* fp8_ring[4];  // null: none
-  const void* bwd_ring;
+  const void* bwd[2];       // null: the ring always fits
+  const void* bwd_ring[2];  // null: none
   int capacity() const { return ld * tpr; }  // packets per row
   int threads() const { return addnorm_threads(tpr); }
   int groups() const { return threads() / tpr; }

@@ -59,7 +59,7 @@ Layout layout_of(const Buffer* b, int n, int64_t N, int vec, const void* w, int*
 
 struct Plan {
   const void* fn;
-  int threads, grid, stages;
+  int threads, grid, stages, ring_at;
   size_t smem;
 };
 
@@ -81,10 +81,9 @@ int scale_kind(int group) { return group == 0 ? 0 : group == 32 ? 1 : group == 6
 int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, int period, int64_t M, int64_t N,
          bool has_residual, int group, Plan* out) {
   const int vec = 16 / t->size_t_;
-  // packets a row can span: up to one more at either end when it starts inside one
-  const int64_t need = layout == kOffset ? (N + 2 * vec - 2) / vec : (N + vec - 1) / vec;
+  const int64_t need = N / vec;  // whole packets, at most
   const AddNormShape* s = nullptr;
-  out->stages = 0;
+  out->stages = out->ring_at = 0;
   if (layout != kAny)
     for (int i = 0; i < t->n && s == nullptr; ++i)
       if (t->shapes[i].capacity() >= need) s = &t->shapes[i];
@@ -93,35 +92,39 @@ int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, in
   if (s != nullptr) {
     groups = s->groups();
     out->fn = which == kFwd ? s->fwd[layout] : which == kBwd ? s->bwd[layout]
-              : layout == kOffset ? s->fp8_offset : s->fp8[scale_kind(group)];
+              : layout == kOffset ? s->fp8_offset[0] : s->fp8[scale_kind(group)];
     out->threads = s->threads();
-    if (layout == kOffset) out->smem = sizeof(float) * (vec == 8 ? w_slots<8>(static_cast<int>(N)) : w_slots<4>(static_cast<int>(N)));
-    if (which == kFp8 && layout == kOffset)  // the maxima, two halves per row group
-      out->smem += sizeof(uint32_t) * 2 * groups * (group ? (N + group - 1) / group : 1);
-    // rows enough for a second round: 16 x 4096 bf16 takes 2.5 us without a ring and 2.7 with one, 1024 x 4096 5.4 and 5.3
-    if (which == kFp8 && layout == kAligned && s->fp8_ring[0] != nullptr && M > (int64_t)dev.sm_count * groups) {
-      size_t ring = 0;
-      out->stages = ring_stages(static_cast<size_t>(N) * (t->size_t_ + (has_residual ? t->size_r : 0)), 0, groups, &ring);
-      if (out->stages > 0) {
-        out->fn = s->fp8_ring[scale_kind(group)];
-        out->smem = ring;
+    // off the packet boundaries, weights that are not in registers
+    const size_t weights = layout == kOffset && s->ld * vec > 16 ? sizeof(float) * w_slots(static_cast<int>(N)) : 0;
+    out->smem = weights;
+    if (which == kFp8) {
+      size_t fixed = 0;
+      if (layout == kOffset)  // the maxima, two halves per row group
+        fixed = weights + (sizeof(uint32_t) * 2 * groups * (group ? (N + group - 1) / group : 1) + 127) / 128 * 128;
+      out->smem = fixed;
+      const void* ring_fn = layout == kOffset ? s->fp8_offset[1] : s->fp8_ring[scale_kind(group)];
+      // rows enough for a second round: 16 x 4096 bf16 takes 2.5 us without a ring and 2.7 with one, 1024 x 4096 5.4 and 5.3
+      if (ring_fn != nullptr && M > (int64_t)dev.sm_count * groups) {
+        size_t ring = 0;
+        out->stages = ring_stages(static_cast<size_t>(need) * vec * (t->size_t_ + (has_residual ? t->size_r : 0)), fixed, groups, &ring);
+        if (out->stages > 0) {
+          out->fn = ring_fn;
+          out->smem = ring;
+          out->ring_at = static_cast<int>(fixed);
+        }
       }
     }
     if (which == kBwd) {
-      const size_t wide = addnorm_wide(s->ld, vec, s->tpr) ? sizeof(float) * s->ld * vec * s->tpr : 0;
-      const size_t sums = groups > 1 ? sizeof(float) * groups * N : wide;
-      const size_t slot = static_cast<size_t>(N) * (t->size_t_ + t->size_r * (has_residual ? 2 : 1));
+      const size_t fixed = weights + (addnorm_wide(s->ld, vec, s->tpr) ? sizeof(float) * s->ld * vec * s->tpr : 0);
+      const size_t sums = groups > 1 ? sizeof(float) * groups * N : 0;
+      const size_t slot = static_cast<size_t>(need) * vec * (t->size_t_ + t->size_r * (has_residual ? 2 : 1));
       size_t ring = 0;
-      if (layout == kAligned && s->bwd_ring != nullptr) out->stages = ring_stages(slot, wide, groups, &ring);
-      if (out->stages > 0) {
-        out->fn = s->bwd_ring;
-        out->smem = std::max(ring, sums);
-      } else {
-        out->smem += sums;
-      }
+      if (s->bwd_ring[layout] != nullptr) out->stages = ring_stages(slot, fixed, groups, &ring);
+      if (out->stages > 0) out->fn = s->bwd_ring[layout];
+      out->smem = std::max(ring, fixed + sums);
     }
-    // the widest rows off the packet boundaries: their weights and sums do not fit beside one another
-    if (out->smem > kMaxSmemPerCta - 4096) s = nullptr;
+    // a row without a kernel that fits
+    if (out->fn == nullptr || out->smem > kMaxSmemPerCta - 4096) s = nullptr;
   }
   if (s == nullptr) {
     out->fn = which == kFwd ? t->fwd_any : which == kFp8 ? t->fp8_any : t->bwd_any;
@@ -163,7 +166,7 @@ int forward(bool fp8, const void* x, int64_t xs, const void* r, int64_t rs, cons
   AddNormParams p = {};
   p.x = x; p.r = r; p.w = w; p.y = y; p.h = h; p.rstd = rstd; p.scale = scale;
   p.x_stride = xs; p.r_stride = rs; p.y_stride = ys; p.h_stride = hs;
-  p.stages = pl.stages; p.status = dev->status_dev;
+  p.stages = pl.stages; p.ring_at = pl.ring_at; p.status = dev->status_dev;
   p.M = M; p.N = static_cast<int>(N); p.w_dtype = w_dtype; p.eps = eps;
   p.group = group; p.groups_per_row = group ? static_cast<int>((N + group - 1) / group) : 1; p.e8m0 = e8m0 != 0;
   return launch(pl.fn, dim3(pl.grid), dim3(pl.threads), pl.smem, &p, static_cast<cudaStream_t>(stream));
