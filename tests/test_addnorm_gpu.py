@@ -391,3 +391,22 @@ def test_other_stream():
     torch.cuda.current_stream().wait_stream(s)
     check_forward(x, r, w, 1e-6, y, h)
     check_backward(h, dy, dh, w, 1e-6, *out)
+
+
+@pytest.mark.parametrize("t,r", TYPES)
+def test_short_rows_of_every_length(t, r):
+    # heads and tails of every size around few or no whole packets, several rows to a warp
+    for N in list(range(1, 41)) + [119, 127, 135, 255, 257, 263]:
+        check(37, N, t, r, F32 if N % 2 else None, with_dh=N % 3 != 0)
+        check(6, N, t, r, t, layout="offset")
+        x, res, w, _, _ = make(37, N, t, r, t, seed=N)
+        check_fp8(x, res if N % 2 else None, w, 1e-6, [0, 32, 64, 128][N % 4], N % 5 == 0)
+
+
+@pytest.mark.parametrize("t,r", TYPES)
+def test_wide_rows_more_than_a_ring_holds(t, r):
+    for M, N in [(1301, 4101), (1301, 8199), (901, 10001), (901, 10240), (650, 12296), (650, 16377)]:
+        check(M, N, t, r, F32 if N % 2 else t, with_dh=N != 16377)
+        x, res, w, _, _ = make(M, N, t, r, t, seed=N)
+        check_fp8(x, res if N % 2 else None, w, 1e-6, [0, 32, 64, 128][M % 4], N % 3 == 0)
+        check_fp8(x, res, None, 1e-6, 0, False)

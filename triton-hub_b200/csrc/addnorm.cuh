@@ -278,7 +278,7 @@ __host__ __device__ constexpr int addnorm_threads(int tpr) { return tpr < 160 ? 
 
 // Whether a backward thread's LD * VEC dweight sums go to shared memory: they would not fit in the
 // registers beside the row.
-__host__ __device__ constexpr bool addnorm_wide(int ld, int vec, int tpr) { return ld * vec > 24 || tpr > 512; }
+__host__ __device__ constexpr bool addnorm_wide(int ld, int vec, int tpr) { return ld * vec > 24 || tpr > 768; }
 
 // CTAs per SM that the register allocation leaves room for: as many threads as run without spills, more (`lean`) where a
 // thread holds little.  Rows off the packet boundaries wait on their loads and barriers: lean made 8182 x 4101 bf16
@@ -1142,14 +1142,13 @@ __global__ void __launch_bounds__(512) addnorm_bwd_any_kernel(const AddNormParam
 // ---------------------------------------------------------------------------------------
 // What the launch code needs to know of the compiled kernels, one table per (T, R).
 // ---------------------------------------------------------------------------------------
-struct AddNormShape {
+struct AddNormShape {  // null: the shape is not for this
   int ld, tpr;
-  const void* fwd[2];  // [rows at a common offset]
-  const void* fp8[4];  // a scale per row, 32, 64, 128 columns
-  const void* fp8_offset[2];  // [with a ring]; null: none
-  const void* fp8_ring[4];  // null: none
-  const void* bwd[2];       // null: the ring always fits
-  const void* bwd_ring[2];  // null: none
+  const void* fwd[2];       // [rows at a common offset]
+  const void* fp8[5];       // a scale per row, 32, 64, 128 columns; rows at a common offset
+  const void* fp8_ring[5];
+  const void* bwd[2];
+  const void* bwd_ring[2];
   int capacity() const { return ld * tpr; }  // packets per row
   int threads() const { return addnorm_threads(tpr); }
   int groups() const { return threads() / tpr; }

@@ -76,7 +76,7 @@ int ring_stages(size_t slot, size_t fixed, int groups, size_t* smem) {
   return 0;
 }
 
-int scale_kind(int group) { return group == 0 ? 0 : group == 32 ? 1 : group == 64 ? 2 : 3; }
+int scale_kind(Layout layout, int group) { return layout == kOffset ? 4 : group == 0 ? 0 : group == 32 ? 1 : group == 64 ? 2 : 3; }
 
 int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, int period, int64_t M, int64_t N,
          bool has_residual, int group, Plan* out) {
@@ -84,15 +84,19 @@ int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, in
   const int64_t need = N / vec;  // whole packets, at most
   const AddNormShape* s = nullptr;
   out->stages = out->ring_at = 0;
+  const int kind = layout == kAny ? 0 : scale_kind(layout, group);
   if (layout != kAny)
-    for (int i = 0; i < t->n && s == nullptr; ++i)
-      if (t->shapes[i].capacity() >= need) s = &t->shapes[i];
+    for (int i = 0; i < t->n && s == nullptr; ++i) {
+      const AddNormShape& c = t->shapes[i];
+      const bool has = which == kFwd ? c.fwd[layout] != nullptr : which == kFp8 ? c.fp8[kind] != nullptr
+                       : c.bwd[layout] != nullptr || c.bwd_ring[layout] != nullptr;
+      if (has && c.capacity() >= need) s = &c;
+    }
   int groups = 1;
   out->smem = 0;
   if (s != nullptr) {
     groups = s->groups();
-    out->fn = which == kFwd ? s->fwd[layout] : which == kBwd ? s->bwd[layout]
-              : layout == kOffset ? s->fp8_offset[0] : s->fp8[scale_kind(group)];
+    out->fn = which == kFwd ? s->fwd[layout] : which == kBwd ? s->bwd[layout] : s->fp8[kind];
     out->threads = s->threads();
     // off the packet boundaries, weights that are not in registers
     const size_t weights = layout == kOffset && s->ld * vec > 16 ? sizeof(float) * w_slots(static_cast<int>(N)) : 0;
@@ -102,7 +106,7 @@ int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, in
       if (layout == kOffset)  // the maxima, two halves per row group
         fixed = weights + (sizeof(uint32_t) * 2 * groups * (group ? (N + group - 1) / group : 1) + 127) / 128 * 128;
       out->smem = fixed;
-      const void* ring_fn = layout == kOffset ? s->fp8_offset[1] : s->fp8_ring[scale_kind(group)];
+      const void* ring_fn = s->fp8_ring[kind];
       // rows enough for a second round: 16 x 4096 bf16 takes 2.5 us without a ring and 2.7 with one, 1024 x 4096 5.4 and 5.3
       if (ring_fn != nullptr && M > (int64_t)dev.sm_count * groups) {
         size_t ring = 0;
