@@ -58,7 +58,7 @@
 extern "C" {
 #endif
 
-#define B200NORM_VERSION 101 /* major*10000 + minor*100 + patch */
+#define B200NORM_VERSION 102 /* major*10000 + minor*100 + patch */
 
 #if defined(__GNUC__)
 #define B200NORM_API __attribute__((visibility("default")))

@@ -16,10 +16,11 @@
 // enough of them in flight.  A row lives in the registers of TPR threads, LD 16-byte packets each.
 //   16384 x 4096 bf16           forward 84 us, backward 84: 0.97 of the copy bandwidth
 //   6001 x 5120 bf16, fp32 h    forward 63 us (0.89), backward 76 (0.98)
-//   16384 x 5120 bf16 to 8 bits, a scale a row, with residual  102 us (0.88)
+//   16384 x 5120 bf16 to 8 bits, a scale a row, with residual  100 us (0.89)
 //   8191 x 4104 fp16 to 8 bits, a scale per 32 columns  31 us (0.49), bound by instructions: 23 an element, issue slots 69 % busy
-//   8182 x 4101 bf16 (rows off the packet boundaries)  forward 79 us (0.51), backward 112 (0.37), 3001 x 1001 fp16 10 and 14 us
-//     (0.36, 0.19): masked packets, the weights from shared memory, no bulk copies
+//   8182 x 4101 bf16 (rows off the packet boundaries)  forward 45 us (0.91), backward 54 (0.76); 3001 x 1001 fp16 7 and 11 us,
+//     of which the launches, the first loads and the column reduce are half
+//   229824 x 146 bf16  forward 75 us (0.55), backward 87 (0.47): 18 packets on 32 lanes, and as many instructions as for 32
 // The backward's ring makes 8192 x 8192 bf16 113 -> 86 us and 6001 x 5120 with fp32 h 100 -> 76; 16384 x 1024 is as quick
 // without one.  The forward needs none (it writes as much as it reads), but for the 8-bit form, which computes more: 16384 x 4096
 // bf16, 128 columns a scale, 65 -> 48 us.
@@ -280,9 +281,10 @@ __host__ __device__ constexpr int addnorm_threads(int tpr) { return tpr < 160 ? 
 // registers beside the row.
 __host__ __device__ constexpr bool addnorm_wide(int ld, int vec, int tpr) { return ld * vec > 24 || tpr > 768; }
 
-// CTAs per SM that the register allocation leaves room for: as many threads as run without spills, more (`lean`) where a
-// thread holds little.  Rows off the packet boundaries wait on their loads and barriers: lean made 8182 x 4101 bf16
-// forward 94 -> 79 us, 200000 x 100 backward 101 -> 81.
+// CTAs per SM that the register allocation leaves room for: as many threads as run without spills, by the elements a
+// thread holds; more (`lean`) where that pays.  Lean makes the forward of 8182 x 4101 bf16 50 -> 45 us, of 4091 x 4101 fp32 61
+// -> 45, the 8-bit form of 8192 x 8192 bf16 58 -> 48, the backward of 229824 x 146 bf16 106 -> 87, and costs 16384 x 2048 bf16
+// forward 2 us of 43.
 __host__ __device__ constexpr int addnorm_fwd_ctas(int elements, int tpr, bool lean) {
   const int n = (elements > 16 ? 512 : lean ? 1024 : 768) / addnorm_threads(tpr);
   return n < 1 ? 1 : n;
@@ -728,7 +730,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
 // A slot is refilled behind the row's reduction, a barrier that every thread passes with its packets read.
 template <typename T, typename R, int LD, int TPR, bool OFF, bool RING>
 __global__ void __launch_bounds__(addnorm_threads(TPR),
-                                  addnorm_bwd_ctas(LD, TPR, (sizeof(R) == sizeof(T) && TPR >= 160) || (OFF && LD == 1)))
+                                  addnorm_bwd_ctas(LD, TPR, LD == 1))
     addnorm_bwd_kernel(const AddNormParams p) {
   static_assert(!RING || TPR > 32, "a ring belongs to a group with a barrier");
   constexpr int VEC = Pack16<T>::kElems, H = VEC / 2;
