@@ -45,7 +45,7 @@ def _add_rmsnorm_fwd(x, residual, weight, eps, *, need_rstd=True):
     Fn._check_dim(x, N)
     weight, _, wcode = _params(weight, None, N, device)
     y, h = _like(x, xr), _like(residual, r)
-    rstd = torch.empty((M,), dtype=torch.float32, device=device) if need_rstd else None
+    rstd = torch.empty(M, dtype=torch.float32, device=device) if need_rstd else None
     lib = _lib.load()
     index = device.index
     with _on_device(index):
@@ -87,7 +87,7 @@ def _add_rmsnorm_bwd(h, dy, dh, weight, rstd, *, need_dw=True):
                 if ws_bytes == 0:
                     _lib.check(_lib.ERR_ARG)
                 _ADD_WS[key] = ws_bytes
-            ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=device)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
         _lib.check(lib.b200norm_add_rms_bwd(
             hr.data_ptr(), hs, dyr.data_ptr(), dys, _ptr(dhr), dhs, _ptr(weight), rstd.data_ptr(), dx.data_ptr(), N, _ptr(dres),
             N, _ptr(dw), _ptr(ws), ws_bytes, M, N, io, res, wcode, _raw_stream(index)))
@@ -151,8 +151,8 @@ def rmsnorm_fp8(x, weight=None, eps=1e-5, *, residual=None, group=0, scale_dtype
         r, _, _, rs = _flat(residual)
         h, rcode = _like(residual, r), _code(r, "residual")
     weight, _, wcode = _params(weight, None, N, device)
-    q = torch.empty(shape, dtype=torch.float8_e4m3fn, device=device)
-    scale = torch.empty((*shape[:-1], -(-N // group) if group else 1), dtype=scale_dtype, device=device)
+    q = torch.empty(*shape, dtype=torch.float8_e4m3fn, device=device)
+    scale = torch.empty(*shape[:-1], -(-N // group) if group else 1, dtype=scale_dtype, device=device)
     lib = _lib.load()
     index = device.index
     with _on_device(index):

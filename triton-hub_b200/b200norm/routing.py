@@ -31,11 +31,11 @@ def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True):
                                f"{tuple(mask.shape)} of {mask.dtype} on {mask.device}")
         mask = mask.contiguous()
     x, T, E, xs = _flat(logits)
-    gates = torch.empty((*shape, k), dtype=torch.float32, device=device)
-    experts = torch.empty((*shape, k), dtype=torch.int32, device=device)
-    counts = torch.empty((E + 1,), dtype=torch.int32, device=device)
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    lse = torch.empty((T,), dtype=torch.float32, device=device) if need_lse else None
+    gates = torch.empty(*shape, k, dtype=torch.float32, device=device)
+    experts = torch.empty(*shape, k, dtype=torch.int32, device=device)
+    counts = torch.empty(E + 1, dtype=torch.int32, device=device)
+    loss = gates.new_empty(())
+    lse = torch.empty(T, dtype=torch.float32, device=device) if need_lse else None
     lib = _lib.load()
     index = device.index
     with _on_device(index):
@@ -46,7 +46,7 @@ def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True):
             if ws_bytes == 0:
                 _lib.check(_lib.ERR_ARG)
             _WS_BYTES[key] = ws_bytes
-        ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=device) if ws_bytes > 1 else None
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes > 1 else None
         _lib.check(lib.b200norm_route_fwd(
             x.data_ptr(), xs, _ptr(mask), gates.data_ptr(), experts.data_ptr(), _ptr(lse), counts.data_ptr(),
             loss.data_ptr(), _ptr(ws), ws_bytes, T, E, k, int(bool(normalize)), code, _raw_stream(index)))
@@ -89,13 +89,13 @@ class route(torch.autograd.Function):
     def apply(cls, logits, k, normalize=True, mask=None):
         if not torch.is_grad_enabled():  # nothing to record: a decode step's call is spared autograd's bookkeeping
             gates, experts, counts, loss, _ = _route_fwd(logits, k, normalize, mask, need_lse=False)
-            return gates, experts, counts.narrow(0, 0, logits.shape[-1]), loss
+            return gates, experts, counts[:-1], loss
         return super().apply(logits, k, normalize, mask)
 
     @staticmethod
     def forward(ctx, logits, k, normalize=True, mask=None):
         gates, experts, counts, loss, lse = _route_fwd(logits, k, normalize, mask, need_lse=ctx.needs_input_grad[0])
-        chosen = counts.narrow(0, 0, logits.shape[-1])
+        chosen = counts[:-1]
         ctx.mark_non_differentiable(experts, chosen)
         ctx.set_materialize_grads(False)
         if ctx.needs_input_grad[0]:

@@ -51,7 +51,7 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     k_v, k = _setting(top_k, "top_k", shape, device, torch.int32, 0, 2 ** 31 - 1)
     p_v, p = _setting(top_p, "top_p", shape, device, torch.float32, 0.0, 1.0)
     m_v, m = _setting(min_p, "min_p", shape, device, torch.float32, 0.0, 1.0)
-    tokens = torch.empty(shape, dtype=torch.int64, device=device)
+    tokens = torch.empty(*shape, dtype=torch.int64, device=device) if shape else uniform.new_empty((), dtype=torch.int64)
     u = uniform if uniform.dtype == torch.float32 and uniform.is_contiguous() else uniform.to(torch.float32).contiguous()
     x, M, V, xs = _flat(logits)
     lib = _lib.load()
