@@ -63,12 +63,12 @@ struct Plan {
   size_t smem;
 };
 
-// Slots of a ring: as many, up to four, as leave room for three, two or one CTA per SM (228 KB, 1 KB of it
+// Slots of a ring: as many, up to `most`, as leave room for three, two or one CTA per SM (228 KB, 1 KB of it
 // reserved per CTA, and a little static shared memory), at least two; 0 when two do not fit.  Four slots always, with fewer
 // CTAs, is the same within 2 % (backward of 16384 x 4096 bf16 84.3 instead of 83.5 us, of 16384 x 1024 29.3 instead of 28.6).
-int ring_stages(size_t slot, size_t fixed, int groups, size_t* smem) {
+int ring_stages(size_t slot, int most, size_t fixed, int groups, size_t* smem) {
   for (size_t cap : {74 * 1024, 112 * 1024, 224 * 1024})
-    for (int stages = kAddNormStages; stages >= 2; --stages)
+    for (int stages = most; stages >= 2; --stages)
       if (fixed + slot * stages * groups <= cap) {
         *smem = fixed + slot * stages * groups;
         return stages;
@@ -107,10 +107,11 @@ int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, in
         fixed = weights + (sizeof(uint32_t) * 2 * groups * (group ? (N + group - 1) / group : 1) + 127) / 128 * 128;
       out->smem = fixed;
       const void* ring_fn = s->fp8_ring[kind];
-      // rows enough for a second round: 16 x 4096 bf16 takes 2.5 us without a ring and 2.7 with one, 1024 x 4096 5.4 and 5.3
-      if (ring_fn != nullptr && M > (int64_t)dev.sm_count * groups) {
+      // Two slots: four make 20480 x 4096 bf16 with a scale per 32 columns 56.4 instead of 54.8 us.
+      // Rows enough for a second round: 16 x 4096 bf16 takes 2.5 us without a ring and 2.7 with one, 1024 x 4096 5.4 and 5.3
+      if (ring_fn != nullptr && !has_residual && M > (int64_t)dev.sm_count * groups) {
         size_t ring = 0;
-        out->stages = ring_stages(static_cast<size_t>(need) * vec * (t->size_t_ + (has_residual ? t->size_r : 0)), fixed, groups, &ring);
+        out->stages = ring_stages(static_cast<size_t>(need) * vec * t->size_t_, 2, fixed, groups, &ring);
         if (out->stages > 0) {
           out->fn = ring_fn;
           out->smem = ring;
@@ -123,7 +124,7 @@ int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, in
       const size_t sums = groups > 1 ? sizeof(float) * groups * N : 0;
       const size_t slot = static_cast<size_t>(need) * vec * (t->size_t_ + t->size_r * (has_residual ? 2 : 1));
       size_t ring = 0;
-      if (s->bwd_ring[layout] != nullptr) out->stages = ring_stages(slot, fixed, groups, &ring);
+      if (s->bwd_ring[layout] != nullptr) out->stages = ring_stages(slot, kAddNormStages, fixed, groups, &ring);
       if (out->stages > 0) out->fn = s->bwd_ring[layout];
       out->smem = std::max(ring, fixed + sums);
     }
