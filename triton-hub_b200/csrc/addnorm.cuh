@@ -877,7 +877,8 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
 #pragma unroll
     for (int j = 0; j < LD; ++j) {
       const int pk = j * TPR + t;
-      if (!WREG && pk >= packets) continue;
+      // With 768 threads, hence 80 registers, the test keeps these from being spilled (5000 x 12288 bf16: 87 -> 79 us).
+      if ((!WREG || TPR > 512) && pk >= packets) continue;
       float2 gf[H], hf[H], wf[H];
       gv[j].unpack(gf);
       hv[j].unpack(hf);
