@@ -14,16 +14,16 @@
 // Most of it is bound by memory: the forward reads x, r and writes h, y, the backward reads h, dy, dh and
 // writes one gradient (two when R is not T), so the aim is only to touch each byte once and to keep
 // enough of them in flight.  A row lives in the registers of TPR threads, LD 16-byte packets each.
-//   16384 x 4096 bf16           forward 84 us, backward 84: 0.97 of the copy bandwidth
-//   6001 x 5120 bf16, fp32 h    forward 63 us (0.89), backward 76 (0.98)
-//   16384 x 5120 bf16 to 8 bits, a scale a row, with residual  95 us (0.94)
-//   8191 x 4104 fp16 to 8 bits, a scale per 32 columns  31 us (0.49), bound by instructions: 23 an element, issue slots 69 % busy
-//   8182 x 4101 bf16 (rows off the packet boundaries)  forward 45 us (0.91), backward 54 (0.76); 3001 x 1001 fp16 7 and 11 us,
-//     of which the launches, the first loads and the column reduce are half
-//   229824 x 146 bf16  forward 75 us (0.55), backward 87 (0.47): 18 packets on 32 lanes, and as many instructions as for 32
+//   16384 x 4096 bf16           forward 84 us, backward 83: 0.98 of the copy bandwidth
+//   6001 x 5120 bf16, fp32 h    forward 63 us (0.90), backward 76 (0.99)
+//   16384 x 5120 bf16 to 8 bits, a scale a row, with residual  93 us (0.96)
+//   8191 x 4104 fp16 to 8 bits, a scale per 32 columns  28 us (0.56), bound by instructions
+//   8182 x 4101 bf16 (rows off the packet boundaries)  forward 45 us (0.91), backward 52 (0.79), to 8 bits per 128 columns 44
+//     (0.36); 3001 x 1001 fp16 7 and 11 us, of which the launches, the first loads and the column reduce are half
+//   229824 x 146 bf16  forward 74 us (0.55), backward 85 (0.48): 18 packets on 32 lanes, and as many instructions as for 32
 // The backward's ring makes 8192 x 8192 bf16 113 -> 86 us and 6001 x 5120 with fp32 h 100 -> 76; 16384 x 1024 is as quick
-// without one.  The forward needs none (it writes as much as it reads), but for the 8-bit form, which computes more: 16384 x 4096
-// bf16, 128 columns a scale, 65 -> 48 us.
+// without one.  The forward needs none (it writes as much as it reads), but for the 8-bit form without a residual: 20480 x 4096
+// bf16, a scale per 32 columns, 63 -> 51 us.
 #pragma once
 
 #include "norm_common.cuh"

@@ -107,9 +107,8 @@ int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, in
         fixed = weights + (sizeof(uint32_t) * 2 * groups * (group ? (N + group - 1) / group : 1) + 127) / 128 * 128;
       out->smem = fixed;
       const void* ring_fn = s->fp8_ring[kind];
-      // Two slots: four make 20480 x 4096 bf16 with a scale per 32 columns 56.4 instead of 54.8 us.
-      // Rows enough for a second round: 16 x 4096 bf16 takes 2.5 us without a ring and 2.7 with one, 1024 x 4096 5.4 and 5.3
-      if (ring_fn != nullptr && !has_residual && M > (int64_t)dev.sm_count * groups) {
+      // two slots: four make 20480 x 4096 bf16 with a scale per 32 columns 56.4 instead of 54.8 us
+      if (ring_fn != nullptr && !has_residual) {
         size_t ring = 0;
         out->stages = ring_stages(static_cast<size_t>(need) * vec * t->size_t_, 2, fixed, groups, &ring);
         if (out->stages > 0) {
