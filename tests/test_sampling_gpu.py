@@ -246,3 +246,16 @@ def test_refusals():
         b200norm.sample(x.double(), u)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         b200norm.sample(x.cpu(), u.cpu())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prefixes_that_end_above_and_below_min_p(dtype):
+    x, u = make(40, 30011, dtype, seed=8)
+    flat = (torch.randn(40, 30011, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV) * 0.7).to(dtype)
+    for rows in (x, flat):
+        for p in (0.05, 0.5, 0.9, 0.999):
+            for mp in (1e-9, 1e-4, 0.02, 0.4, 0.999, 1.0):
+                check(rows, u, top_p=p, min_p=mp)
+                check(rows, u, top_p=p, min_p=mp, top_k=3000, temperature=1.4)
+    spread = torch.linspace(0, 1, 40, device=DEV)
+    check(x, u, top_p=0.3 + 0.7 * spread.flip(0), min_p=0.1 * spread ** 3, temperature=0.8)

@@ -787,7 +787,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
   }
   if (use_p) {
     // The weights above top-k's threshold; at it, `ties` tokens more.
-    row.template fill_bins<true>(floor, kSampleBins - 2);
+    // Tokens too light for min-p need no bins of their own, only their sum: when the prefix ends among them, it keeps all that
+    // min-p does.  (A bin is floor(-32 log2 w); one more for the rounding of min-p's.)  64 x 131072 bf16, p = 0.95 and
+    // min-p up to 0.02 a row: 50 -> 41 us.
+    const int heavy = least_share > 0.f ? static_cast<int>(fminf(-32.f * log2f(least_share), 2.f * kSampleBins)) + 2 : kSampleBins;
+    const bool light = heavy < kSampleBins - 2;
+    row.template fill_bins<true>(floor, min(heavy, kSampleBins - 2));
     u64 total, need;
     row.template locate<true>(0, [&](u64 sum) {
       total = sum;
@@ -795,7 +800,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleP
     });
     if (need > total) {  // the prefix ends among the ties at top-k's threshold
       th.ties = (need - total + floor_weight - 1) / floor_weight;
-    } else {
+    } else if (!light || sh->found_bin < kSampleBins - 1) {
       const int last = sh->found_bin;
       if (sh->found_tokens <= kSampleList / 2) {  // room for some of the bins beyond, which the test may take along
         const float end = row.template bin_end<true>(last);
