@@ -359,8 +359,8 @@ B200NORM_API int b200norm_rms_fp8(const void* x, int64_t x_row_stride, const voi
  * top_k tokens in order of (logit descending, index ascending), of those the shortest prefix that holds
  * top_p of their weight, of those the ones of weight >= min_p; drawn is the lowest index at which the
  * running sum of the kept weights, in index order, exceeds uniform * total.  temperature <= 0: the likeliest
- * token; top_k outside [1, V), top_p >= 1, min_p <= 0: off.  tokens (M,): -1 for a row that holds a NaN or
- * nothing above -inf.  Needs no workspace.
+ * token; top_k outside [1, V), top_p >= 1, min_p <= 0: off.  Logits of +inf share the draw among themselves.
+ * tokens (M,): -1 for a row that holds a NaN or nothing above -inf.  Needs no workspace.
  */
 B200NORM_API int b200norm_sample(const void* logits, int64_t row_stride, const float* uniform,
                                  const float* temperature_v, float temperature, const int* top_k_v, int top_k,

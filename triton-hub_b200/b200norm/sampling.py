@@ -37,7 +37,8 @@ def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     uniform: one number in [0, 1) a row.  temperature (0: the likeliest token, the lowest index among equals), top_k
     (0: all), top_p (1: all) and min_p (0: all) are numbers, or tensors of one value a row, whose values are not
     checked: a temperature that is not positive means 0, a top_k outside [1, V) all, a min_p above 1 means 1.
-    Logits of -inf are never drawn.  A row that holds a NaN, or nothing above -inf, gives -1."""
+    Logits of -inf are never drawn; those of +inf share the draw among themselves.  A row that holds a NaN, or nothing
+    above -inf, gives -1."""
     _require_cuda(logits)
     if logits.dtype == torch.float64:
         raise RuntimeError("b200norm: logits dtype torch.float64 is not supported (float32, float16, bfloat16)")

@@ -9,6 +9,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <exception>
 #include <mutex>
 #include <unordered_map>
 
@@ -87,7 +88,8 @@ int device_state(DeviceState** out) {
   return B200NORM_OK;
 }
 
-int occupancy(DeviceState& s, const void* fn, int threads, size_t smem, int* out, int cluster) {
+// Behind a C entry point: a map that cannot grow is an error code, too.
+int occupancy(DeviceState& s, const void* fn, int threads, size_t smem, int* out, int cluster) try {
   const unsigned long long key =
       (reinterpret_cast<unsigned long long>(fn) * 0x9E3779B97F4A7C15ull) ^ (unsigned long long)smem;
   std::lock_guard<std::mutex> lock(s.mu);
@@ -129,6 +131,8 @@ int occupancy(DeviceState& s, const void* fn, int threads, size_t smem, int* out
   s.occupancy.emplace(key, n);
   *out = n;
   return B200NORM_OK;
+} catch (const std::exception& e) {
+  return fail(B200NORM_ERR_CUDA, "launch planning: %s", e.what());
 }
 
 namespace {
