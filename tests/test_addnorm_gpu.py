@@ -410,3 +410,13 @@ def test_wide_rows_more_than_a_ring_holds(t, r):
         x, res, w, _, _ = make(M, N, t, r, t, seed=N)
         check_fp8(x, res if N % 2 else None, w, 1e-6, [0, 32, 64, 128][M % 4], N % 3 == 0)
         check_fp8(x, res, None, 1e-6, 0, False)
+
+
+@pytest.mark.parametrize("group,e8m0", [(32, True), (64, False), (128, False)])
+@pytest.mark.parametrize("t", [F32, F16, BF16])
+def test_fp8_scales_over_several_packets_of_a_thread(t, group, e8m0):
+    # short rows, where a scale's columns are more than the lanes of a row hold at once
+    for N in (8, 24, 40, 64, 72, 96, 104, 120, 128, 136, 192, 200, 256, 264, 512):
+        x, res, w, _, _ = make(3001, N, t, t, F32, seed=N)
+        check_fp8(x, None, w, 1e-6, group, e8m0)
+        check_fp8(x[:5], res[:5], None, 1e-6, group, e8m0)

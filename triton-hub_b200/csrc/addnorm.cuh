@@ -20,7 +20,7 @@
 //   8191 x 4104 fp16 to 8 bits, a scale per 32 columns  28 us (0.56), bound by instructions
 //   8182 x 4101 bf16 (rows off the packet boundaries)  forward 45 us (0.91), backward 52 (0.79), to 8 bits per 128 columns 44
 //     (0.36); 3001 x 1001 fp16 7 and 11 us, of which the launches, the first loads and the column reduce are half
-//   229824 x 146 bf16  forward 74 us (0.55), backward 85 (0.48): 18 packets on 32 lanes, and as many instructions as for 32
+//   229824 x 146 bf16  forward 66 us (0.62), backward 73 (0.56): 18 packets cost the instructions of 32
 // The backward's ring makes 8192 x 8192 bf16 113 -> 86 us and 6001 x 5120 with fp32 h 100 -> 76; 16384 x 1024 is as quick
 // without one.  The forward needs none (it writes as much as it reads), but for the 8-bit form without a residual: 20480 x 4096
 // bf16, a scale per 32 columns, 63 -> 51 us.
@@ -283,14 +283,14 @@ __host__ __device__ constexpr bool addnorm_wide(int ld, int vec, int tpr) { retu
 
 // CTAs per SM that the register allocation leaves room for: as many threads as run without spills, by the elements a
 // thread holds; more (`lean`) where that pays.  Lean makes the forward of 8182 x 4101 bf16 50 -> 45 us, of 4091 x 4101 fp32 61
-// -> 45, the 8-bit form of 8192 x 8192 bf16 58 -> 48, the backward of 229824 x 146 bf16 106 -> 87, and costs 16384 x 2048 bf16
+// -> 45, the 8-bit form of 8192 x 8192 bf16 58 -> 48, the backward of 335544 x 100 bf16 85 -> 72, and costs 16384 x 2048 bf16
 // forward 2 us of 43.
 __host__ __device__ constexpr int addnorm_fwd_ctas(int elements, int tpr, bool lean) {
   const int n = (elements > 16 ? 512 : lean ? 1024 : 768) / addnorm_threads(tpr);
   return n < 1 ? 1 : n;
 }
-__host__ __device__ constexpr int addnorm_bwd_ctas(int ld, int tpr, bool lean) {
-  const int n = (ld > 2 ? 512 : lean ? 768 : 512) / addnorm_threads(tpr);
+__host__ __device__ constexpr int addnorm_bwd_ctas(int tpr, bool lean) {
+  const int n = (lean ? 768 : 512) / addnorm_threads(tpr);
   return n < 1 ? 1 : n;
 }
 
@@ -357,7 +357,7 @@ __device__ __forceinline__ float row_sum_max(float v, float& amax, float* scratc
 // only (its step is a multiple of the offsets' period), so that a thread's columns stay the same.
 // GROUP: the 8-bit form with a scale for so many columns, 0 for one a row; -1: the output is y.  Thread t of a
 // row group holds packets t, t + TPR, ...: neighbouring lanes hold neighbouring columns, so a scale's 32, 64 or
-// 128 columns are 4 to 32 adjacent lanes of one warp.  OFF: a packet may belong to two scales' columns, so the
+// 128 columns are 4 to 32 adjacent lanes of one warp, or all lanes of a group of 8 or 16 and several of their packets.  OFF: a packet may belong to two scales' columns, so the
 // maxima are found in shared memory, by one or two atomic maxima a packet; the columns per scale are those of p.group.
 // RING: as in the backward below, the rows of x arrive through p.stages shared-memory slots per row group.  For the 8-bit form
 // without a residual; with one, as for y, as much is written as read, and direct loads by more threads are quicker: 20480 x
@@ -691,11 +691,14 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
       }
       constexpr int SPAN = PAIR ? 2 * VEC : VEC;  // neighbouring columns of a thread
       constexpr int LANES = PER_ROW ? 1 : (GROUP / SPAN < TPR ? GROUP / SPAN : TPR);  // adjacent lanes that share a scale
+      constexpr int JS = PER_ROW || GROUP <= TPR * SPAN ? 1 : GROUP / (TPR * SPAN) < LD ? GROUP / (TPR * SPAN) : LD;  // ... and packets of a lane
 #pragma unroll
       for (int j = 0; j < LD; ++j) {
         const int pk = packet(j);
-        if (!PER_ROW && !(PAIR && j % 2 == 1)) {
+        if (!PER_ROW && !(PAIR && j % 2 == 1) && j % JS == 0) {
           float a = amax_j[j];
+#pragma unroll
+          for (int k = 1; k < JS; ++k) a = max_abs(a, amax_j[j + k < LD ? j + k : j]);
           if constexpr (PAIR) a = max_abs(a, amax_j[j + 1 < LD ? j + 1 : j]);
 #pragma unroll
           for (int o = 1; o < LANES; o <<= 1) a = max_abs(a, __shfl_xor_sync(0xffffffffu, a, o));
@@ -731,7 +734,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
 // A slot is refilled behind the row's reduction, a barrier that every thread passes with its packets read.
 template <typename T, typename R, int LD, int TPR, bool OFF, bool RING>
 __global__ void __launch_bounds__(addnorm_threads(TPR),
-                                  addnorm_bwd_ctas(LD, TPR, LD == 1))
+                                  addnorm_bwd_ctas(TPR, !RING && LD * Pack16<T>::kElems <= 8))
     addnorm_bwd_kernel(const AddNormParams p) {
   static_assert(!RING || TPR > 32, "a ring belongs to a group with a barrier");
   constexpr int VEC = Pack16<T>::kElems, H = VEC / 2;
