@@ -397,3 +397,32 @@ def test_rows_beyond_32_bit_offsets():
     assert torch.equal(R._route_bwd(x, *a[:3], a[4], a[0], a[3]), R._route_bwd(c, *b[:3], b[4], b[0], b[3]))
     u = rand(3)
     assert torch.equal(b200norm.sample(x, u, top_p=0.9), b200norm.sample(c, u, top_p=0.9))
+
+
+def test_a_single_row_without_a_leading_dimension():
+    x, r = randn(1, 512, dtype=BF16), randn(1, 512, seed=1, dtype=BF16)
+    for a, b in zip(b200norm.add_rmsnorm.apply(x[0], r[0], None, 1e-6), b200norm.add_rmsnorm.apply(x, r, None, 1e-6)):
+        assert a.shape == (512,) and torch.equal(a, b[0])
+    for a, b in zip(b200norm.rmsnorm_fp8(x[0], group=64), b200norm.rmsnorm_fp8(x, group=64)):
+        assert torch.equal(a.view(torch.uint8), b[0].view(torch.uint8))
+    a, b = b200norm.route.apply(x[0, :64], 4), b200norm.route.apply(x[:, :64], 4)
+    assert a[0].shape == a[1].shape == (4,) and torch.equal(a[0], b[0][0]) and torch.equal(a[1], b[1][0]) and torch.equal(a[2], b[2])
+    u = rand(1)
+    token = b200norm.sample(x[0], u[0])
+    assert token.shape == () and int(token) == int(b200norm.sample(x, u)[0])
+
+
+def test_settings_of_other_integer_types():
+    import numpy as np
+    x, u = randn(6, 1000, scale=3.0), rand(6)
+    want = b200norm.sample(x, u, top_k=7, temperature=0.5)
+    assert torch.equal(b200norm.sample(x, u, top_k=np.int64(7), temperature=np.float64(0.5)), want)
+    k = torch.full((6,), 7, dtype=torch.int64, device=DEV)
+    assert torch.equal(b200norm.sample(x, u, top_k=k, temperature=0.5), want)
+    assert torch.equal(b200norm.sample(x, u, top_k=k + 2 ** 32), b200norm.sample(x, u))  # more than there are: all
+    with pytest.raises(TypeError):
+        b200norm.sample(x, u, top_k=7.5)
+    a, b = b200norm.route.apply(x[:, :64], np.int32(4)), b200norm.route.apply(x[:, :64], 4)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    for p, q in zip(b200norm.rmsnorm_fp8(x, group=np.int64(32)), b200norm.rmsnorm_fp8(x, group=32)):
+        assert torch.equal(p.view(torch.uint8), q.view(torch.uint8))

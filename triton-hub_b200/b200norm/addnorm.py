@@ -157,7 +157,7 @@ def rmsnorm_fp8(x, weight=None, eps=1e-5, *, residual=None, group=0, scale_dtype
     index = device.index
     with _on_device(index):
         _lib.check(lib.b200norm_rms_fp8(
-            x.data_ptr(), xs, _ptr(r), rs, _ptr(weight), q.data_ptr(), N, scale.data_ptr(), _ptr(h), N, M, N, eps, group,
+            x.data_ptr(), xs, _ptr(r), rs, _ptr(weight), q.data_ptr(), N, scale.data_ptr(), _ptr(h), N, M, N, eps, int(group),
             0 if scale_dtype == torch.float32 else 1, code, rcode, wcode, _raw_stream(index)))
     return (q, scale) if h is None else (q, scale, h)
 

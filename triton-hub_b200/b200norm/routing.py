@@ -8,6 +8,8 @@ The gradient reaches the logits through the gates and through P; f is a count.  
 """
 from __future__ import annotations
 
+from operator import index as as_int
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -31,6 +33,7 @@ def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True):
                                f"{tuple(mask.shape)} of {mask.dtype} on {mask.device}")
         mask = mask.contiguous()
     x, T, E, xs = _flat(logits)
+    k = as_int(k)
     gates = torch.empty(*shape, k, dtype=torch.float32, device=device)
     experts = torch.empty(*shape, k, dtype=torch.int32, device=device)
     counts = torch.empty(E + 1, dtype=torch.int32, device=device)

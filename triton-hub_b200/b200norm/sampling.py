@@ -11,6 +11,8 @@ integers.
 """
 from __future__ import annotations
 
+from operator import index
+
 import torch
 
 from . import _lib
@@ -25,10 +27,12 @@ def _setting(value, name, shape, device, dtype, low, high):
                                f"{tuple(value.shape)} on {value.device}")
         if value.dtype == torch.bool or value.is_floating_point() != (dtype == torch.float32):
             raise RuntimeError(f"b200norm: {name} of dtype {value.dtype}")
+        if value.dtype == torch.int64:  # a larger number means the same as the largest of 32 bits
+            value = value.clamp(-1, 2 ** 31 - 1)
         return value.to(dtype).contiguous(), 0
     if not low <= value <= high:
         raise RuntimeError(f"b200norm: {name} must lie in [{low}, {high}], got {value}")
-    return None, value
+    return None, float(value) if dtype == torch.float32 else index(value)
 
 
 def sample(logits, uniform, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
