@@ -420,3 +420,39 @@ def test_fp8_scales_over_several_packets_of_a_thread(t, group, e8m0):
         x, res, w, _, _ = make(3001, N, t, t, F32, seed=N)
         check_fp8(x, None, w, 1e-6, group, e8m0)
         check_fp8(x[:5], res[:5], None, 1e-6, group, e8m0)
+
+
+def exact_rows(M, N, dtype, seed):
+    """Rows of +-1, whose root mean square is exactly 1, so that y is the weight with a sign."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randint(0, 2, (M, N), generator=g, device=DEV) * 2 - 1).to(dtype)
+
+
+@pytest.mark.parametrize("group", [0, 32, 64, 128])
+@pytest.mark.parametrize("t,r", [(F32, None), (BF16, None), (BF16, BF16), (F16, F32)])
+def test_fp8_quotients_on_a_border_between_two_values(t, r, group):
+    # 1 / N and N products of it with 1 add up to 1 in fp32 at these lengths: y is known without an error, and so are
+    # its scale, max |y| times 1 / 448, and its quotients, all of them rounded to fp32.  The weights are odd multiples of half
+    # a step of e4m3 and of the scale, so the quotients are borders between two values: an ulp either way shows.
+    for N in (32, 100, 256, 1000, 1001, 2048, 4104, 8192, 16384):
+        g = torch.Generator(device=DEV).manual_seed(N)
+        amax = 1.75 * (1 + torch.randint(0, 32, (), generator=g, device=DEV).float() / 32)
+        scale = (amax / 448).item()
+        half = (1 + (2 * torch.randint(0, 8, (N,), generator=g, device=DEV) + 1).float() / 16)
+        w = half * torch.exp2(torch.randint(0, 8, (N,), generator=g, device=DEV).float()) * scale
+        w[::32] = amax
+        for off in (0, 1):
+            n = N - off
+            x = exact_rows(5, N + 32, t, N)[:, off:n + off]
+            res = torch.zeros(5, N + 32, dtype=r, device=DEV)[:, off:n + off] if r else None
+            if float(torch.tensor(1.0) / n * n) != 1.0:
+                continue
+            q, s, *_ = b200norm.rmsnorm_fp8(x, w[:n], 0.0, residual=res, group=group)
+            y = x.float() * w[:n]
+            size = group or n
+            G = -(-n // size)
+            pad = torch.nn.functional.pad(y, (0, G * size - n)).reshape(5, G, size)
+            want = pad.abs().amax(-1) * (torch.ones((), device=DEV) / 448)
+            assert torch.equal(s, want), (N, off)
+            quot = (pad / want[..., None]).reshape(5, G * size)[:, :n].to(torch.float8_e4m3fn)
+            assert torch.equal(q.float(), quot.float()), (N, off)

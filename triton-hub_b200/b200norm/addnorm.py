@@ -125,9 +125,10 @@ def rmsnorm_fp8(x, weight=None, eps=1e-5, *, residual=None, group=0, scale_dtype
     """RMSNorm with an 8-bit output: returns (q, scale), or (q, scale, h) with a residual, where
     q.float() * scale (each scale over its columns) is the norm of h = x + residual (of x without one).
 
-    q: float8_e4m3fn, shaped like x, rounded once from fp32.  group: columns that share a scale: 32, 64 or 128
-    (the last group of a row may be shorter), or 0 for the whole row.  scale: x.shape[:-1] + (ceil(N / group),),
-    the group's largest magnitude / 448, as float32, or as float8_e8m0fnu rounded up to a power of two.
+    q: float8_e4m3fn, shaped like x, the nearest value to the norm / scale in fp32.  group: columns that share a scale: 32,
+    64 or 128 (the last group of a row may be shorter), or 0 for the whole row.  scale: x.shape[:-1] + (ceil(N / group),),
+    the group's largest magnitude / 448, as float32 (good to two roundings of its own), or as float8_e8m0fnu rounded up to
+    a power of two.
     A group of zeros has the scale 2^-64 / 448; one that holds a NaN has the scale NaN.
 
     For inference: it has no gradient, and refuses inputs that ask for one."""

@@ -238,16 +238,19 @@ __device__ __forceinline__ float warp_max_abs(float v) {
   return r;
 }
 
-// A group's scale from its largest magnitude, the byte that a power-of-two scale is stored as, and 1 / scale
-// (one instruction good to an ulp: it moves a value only where that lies within an ulp of a border between two
-// e4m3 values; the reciprocal of a power of two is exact).
+// A group's scale from its largest magnitude, the byte that a power-of-two scale is stored as, and 1 / scale as a sum of two
+// numbers.  An fp32 scale is the product with 1 / 448, within an ulp of the quotient.  With 48 bits of 1 / scale a quotient
+// y / scale comes out correctly rounded (but for one within 2^-24 of an ulp of the middle between two fp32 numbers).  One that lies
+// on a border between two e4m3 values has to: y * (1 / scale) alone, an ulp off now and then, put 6 % of those on the wrong side,
+// and 16-bit rows and weights have such quotients (one in 10^4 of 16384 x 5120 bf16).
 struct Fp8Scale {
-  float scale, inv;
+  float scale, inv, inv_low;
   uint32_t code;
 };
 __device__ __forceinline__ Fp8Scale fp8_scale(float amax, bool e8m0) {
   Fp8Scale r;
   amax = max_abs(amax, kAmaxFloor);
+  r.inv_low = 0.f;
   if (e8m0) {
     // The lowest 2^e with amax <= 448 * 2^e = 1.75 * 2^(e + 8): eight below amax's exponent, or seven where its fraction is
     // above .75.  The reciprocal of a power of two is one, too.
@@ -260,9 +263,12 @@ __device__ __forceinline__ Fp8Scale fp8_scale(float amax, bool e8m0) {
     r.code = 0;
     r.scale = amax * (1.f / kE4m3Max);
     r.inv = rcp_fast(r.scale);
+    if (r.scale < INFINITY) r.inv_low = fmaf(-r.scale, r.inv, 1.f) * r.inv;  // of an infinite scale 0: 0 / inf is 0
   }
   return r;
 }
+__device__ __forceinline__ float2 fp8_quotient2(float2 y, float2 inv, float2 low) { return fma2(y, inv, mul2(y, low)); }
+__device__ __forceinline__ float fp8_quotient(float y, const Fp8Scale& s) { return fmaf(y, s.inv, y * s.inv_low); }
 __device__ __forceinline__ void store_scale(void* p, int64_t at, const Fp8Scale& s, bool e8m0) {
   if (e8m0) static_cast<uint8_t*>(p)[at] = static_cast<uint8_t>(s.code);
   else static_cast<float*>(p)[at] = s.scale;
@@ -650,23 +656,25 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
         if (!valid || pk >= packets) continue;
         int g0, cut;
         parts(c0, g0, cut);
-        const float lo = fp8_scale(__uint_as_float(mx[g0]), p.e8m0 != 0).inv;
-        const float hi = cut < VEC ? fp8_scale(__uint_as_float(mx[g0 + 1]), p.e8m0 != 0).inv : lo;
+        const Fp8Scale lo = fp8_scale(__uint_as_float(mx[g0]), p.e8m0 != 0);
+        const Fp8Scale hi = cut < VEC ? fp8_scale(__uint_as_float(mx[g0 + 1]), p.e8m0 != 0) : lo;
+        auto pair = [&](int e) {  // elements e and e + 1
+          const float2 inv = make_float2(e < cut ? lo.inv : hi.inv, e + 1 < cut ? lo.inv : hi.inv);
+          const float2 low = make_float2(e < cut ? lo.inv_low : hi.inv_low, e + 1 < cut ? lo.inv_low : hi.inv_low);
+          const float2 v = fp8_quotient2(hf[j][e / 2], inv, low);
+          return fp8x2(v.x, v.y);
+        };
         uint32_t word[VEC / 4];
 #pragma unroll
-        for (int k = 0; k < VEC / 4; ++k) {
-          const float2 a = hf[j][2 * k], b = hf[j][2 * k + 1];
-          word[k] = fp8x2(a.x * (4 * k < cut ? lo : hi), a.y * (4 * k + 1 < cut ? lo : hi)) |
-                    (fp8x2(b.x * (4 * k + 2 < cut ? lo : hi), b.y * (4 * k + 3 < cut ? lo : hi)) << 16);
-        }
+        for (int k = 0; k < VEC / 4; ++k) word[k] = pair(4 * k) | (pair(4 * k + 2) << 16);
         if constexpr (VEC == 8) __stcs(reinterpret_cast<uint2*>(qrow + c0), make_uint2(word[0], word[1]));
         else __stcs(reinterpret_cast<uint32_t*>(qrow + c0), word[0]);
       }
 #pragma unroll
       for (int k = 0; k < EDGES; ++k) {
         if (!valid || ec[k] < 0) continue;
-        const float inv = fp8_scale(__uint_as_float(mx[group_of(ec[k])]), p.e8m0 != 0).inv;
-        qrow[ec[k]] = static_cast<uint8_t>(fp8x2(eh[k] * inv, 0.f));
+        const Fp8Scale sc = fp8_scale(__uint_as_float(mx[group_of(ec[k])]), p.e8m0 != 0);
+        qrow[ec[k]] = static_cast<uint8_t>(fp8x2(fp8_quotient(eh[k], sc), 0.f));
       }
     }
     if constexpr (FP8 && !OFF) {
@@ -707,13 +715,17 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
             store_scale(p.scale, row * p.groups_per_row + pk * VEC / (PER_ROW ? 1 : GROUP), sc, p.e8m0 != 0);
         }
         if (valid && pk < packets) {
-          const float2 inv2 = splat2(sc.inv);
+          const float2 inv2 = splat2(sc.inv), low2 = splat2(sc.inv_low);
           uint32_t word[VEC / 4];
+          auto divide = [&](auto quotient) {
 #pragma unroll
-          for (int k = 0; k < VEC / 4; ++k) {
-            const float2 lo = mul2(hf[j][2 * k], inv2), hi = mul2(hf[j][2 * k + 1], inv2);
-            word[k] = fp8x2(lo.x, lo.y) | (fp8x2(hi.x, hi.y) << 16);
-          }
+            for (int k = 0; k < VEC / 4; ++k) {
+              const float2 lo = quotient(hf[j][2 * k]), hi = quotient(hf[j][2 * k + 1]);
+              word[k] = fp8x2(lo.x, lo.y) | (fp8x2(hi.x, hi.y) << 16);
+            }
+          };
+          if (p.e8m0) divide([&](float2 v) { return mul2(v, inv2); });
+          else divide([&](float2 v) { return fp8_quotient2(v, inv2, low2); });
           if constexpr (VEC == 8) __stcs(reinterpret_cast<uint2*>(qrow + pk * VEC), make_uint2(word[0], word[1]));
           else __stcs(reinterpret_cast<uint32_t*>(qrow + pk * VEC), word[0]);
         }
@@ -1083,7 +1095,7 @@ __global__ void __launch_bounds__(512) addnorm_fwd_any_kernel(const AddNormParam
         for (int k = 0; k < 16; ++k) amax = max_abs(amax, max_scratch[k]);
         const Fp8Scale sc = fp8_scale(amax, p.e8m0 != 0);
         if (threadIdx.x == 0) store_scale(p.scale, row, sc, p.e8m0 != 0);
-        for (int c = threadIdx.x; c < p.N; c += 512) qrow[c] = static_cast<uint8_t>(fp8x2(hs[c] * sc.inv, 0.f));
+        for (int c = threadIdx.x; c < p.N; c += 512) qrow[c] = static_cast<uint8_t>(fp8x2(fp8_quotient(hs[c], sc), 0.f));
       } else {
         for (int g = warp; g < p.groups_per_row; g += 16) {
           const int c0 = g * p.group;
@@ -1099,7 +1111,7 @@ __global__ void __launch_bounds__(512) addnorm_fwd_any_kernel(const AddNormParam
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int c = c0 + k * 32 + lane;
-            if (k * 32 < p.group && c < p.N) qrow[c] = static_cast<uint8_t>(fp8x2(v[k] * sc.inv, 0.f));
+            if (k * 32 < p.group && c < p.N) qrow[c] = static_cast<uint8_t>(fp8x2(fp8_quotient(v[k], sc), 0.f));
           }
         }
       }
