@@ -456,3 +456,18 @@ def test_fp8_quotients_on_a_border_between_two_values(t, r, group):
             assert torch.equal(s, want), (N, off)
             quot = (pad / want[..., None]).reshape(5, G * size)[:, :n].to(torch.float8_e4m3fn)
             assert torch.equal(q.float(), quot.float()), (N, off)
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_fp8_row_scale_is_finite_where_the_norm_is(t):
+    # h w passes the largest number, h w / |h| does not
+    for N in (64, 200, 1000, 1001, 4096, 16384):
+        x = torch.full((4, N), 1e17, device=DEV).to(t)
+        x[1, ::2] *= -1
+        x[2] = 1.0
+        w = torch.ones(N, device=DEV)
+        w[3::5] = 1e22
+        w[4::7] = -1e22
+        check_fp8(x, None, w, 1e-6, 0, False)
+        check_fp8(x, torch.zeros_like(x), w, 1e-6, 0, True)
+        check_fp8(x, None, w, 1e-6, 128, False)

@@ -681,10 +681,11 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
       uint8_t* qrow = static_cast<uint8_t*>(p.y) + row * p.y_stride;
       Fp8Scale sc;
       if constexpr (PER_ROW) {
+        // A sum of squares that overflows makes rstd 0 and y 0, or NaN where h is infinite; and a product h w may overflow,
+        // along with it or for a large weight alone, where y does not.  The maximum is then taken again, of y itself.
+        const bool over = rstd == 0.f || amax == INFINITY;
         amax *= rstd;
-        // A sum of squares that overflows makes rstd 0 and y 0, or NaN where h is infinite; a product h w may have
-        // overflowed along with it, so the maximum is taken again, of y itself.
-        const bool again = TPR <= 32 ? __any_sync(0xffffffffu, rstd == 0.f) : rstd == 0.f;
+        const bool again = TPR <= 32 ? __any_sync(0xffffffffu, over) : over;
         if (again) {
           float a = 0.f;
 #pragma unroll
@@ -692,7 +693,7 @@ __global__ void __launch_bounds__(addnorm_threads(TPR),
 #pragma unroll
             for (int k = 0; k < H; ++k) a = max_abs3(a, hf[j][k].x, hf[j][k].y);
           row_sum_max<TPR>(0.f, a, scratch[group], max_scratch[group], phase, group, warp_n, lane);
-          if (rstd == 0.f) amax = a;
+          if (over) amax = a;
         }
         sc = fp8_scale(amax, p.e8m0 != 0);
         if (t == 0 && valid) store_scale(p.scale, row, sc, p.e8m0 != 0);
