@@ -58,7 +58,7 @@
 extern "C" {
 #endif
 
-#define B200NORM_VERSION 102 /* major*10000 + minor*100 + patch */
+#define B200NORM_VERSION 103 /* major*10000 + minor*100 + patch */
 
 #if defined(__GNUC__)
 #define B200NORM_API __attribute__((visibility("default")))
@@ -376,6 +376,8 @@ B200NORM_API int b200norm_sample(const void* logits, int64_t row_stride, const f
  * Not live: tokens whose mask (T,) byte is 0 (mask may be NULL) or whose logits are all -inf; they get
  * experts -1, gates 0.  Slots left over when fewer than k logits are above -inf get the same.
  * lse (T,), needed for backward only (else NULL): log-sum-exp of the logits, -inf for tokens not live.
+ * b200norm_route_fwd_kept: the same, with the counts written to `kept` (E + 1), too (NULL: not wanted), for callers that hand
+ *   `counts` on to code that may change them (a sum over ranks, say) and give `kept` to the backward.
  * b200norm_route_bwd: gradients dgates (T, k) and dloss (one fp32 value on the device), either NULL, to dlogits (T, E)
  *   contiguous; counts are taken as constants.
  * workspace: at least b200norm_route_workspace_bytes bytes, 16-byte aligned; where that is 1 none is needed, and
@@ -386,6 +388,10 @@ B200NORM_API int b200norm_route_fwd(const void* logits, int64_t row_stride, cons
                                     int* experts, float* lse, int* counts, float* loss, void* workspace,
                                     size_t workspace_bytes, int64_t T, int E, int k, int normalize, int io_dtype,
                                     void* stream);
+B200NORM_API int b200norm_route_fwd_kept(const void* logits, int64_t row_stride, const uint8_t* mask, float* gates,
+                                         int* experts, float* lse, int* counts, int* kept, float* loss, void* workspace,
+                                         size_t workspace_bytes, int64_t T, int E, int k, int normalize, int io_dtype,
+                                         void* stream);
 B200NORM_API int b200norm_route_bwd(const void* logits, int64_t row_stride, const float* gates, const int* experts,
                                     const float* lse, const int* counts, const float* dgates,
                                     int64_t dgates_row_stride, const float* dloss, void* dlogits, int64_t T, int E,

@@ -242,3 +242,18 @@ def test_refusals():
         b200norm.route.apply(x.double(), 2)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         b200norm.route.apply(x.cpu(), 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_returned_counts_are_the_callers(dtype):
+    for T in (100, 3000):
+        x = logits(T, 64, dtype, seed=1)
+        grads = []
+        # as it is; behind the version counter's back, as a collective changes it; in the open
+        for change in (lambda c: None, lambda c: c.data.mul_(8), lambda c: c.mul_(8)):
+            v = x.clone().requires_grad_(True)
+            gates, experts, counts, loss = b200norm.route.apply(v, 4)
+            change(counts)
+            (loss + gates.square().sum()).backward()
+            grads.append(v.grad)
+        assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])

@@ -82,6 +82,7 @@ SIGNATURES = {
     "b200norm_sample": (_int, [_vp, _i64, _vp, _vp, _f32, _vp, _int, _vp, _f32, _vp, _f32, _vp, _i64, _i64, _int, _vp]),
     "b200norm_route_workspace_bytes": (_sz, [_i64, _int, _int, _int]),
     "b200norm_route_fwd": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _int, _int, _int, _int, _vp]),
+    "b200norm_route_fwd_kept": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _int, _int, _int, _int, _vp]),
     "b200norm_route_bwd": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _int, _int, _int, _int, _vp]),
     "b200norm_rms_bwd_static": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _int, _int, _vp]),
 }

@@ -19,9 +19,9 @@ from .functional import _code, _flat, _on_device, _ptr, _raw_stream, _require_cu
 _WS_BYTES = {}  # (device, T, E, k, dtype code) -> workspace bytes; the answer never changes
 
 
-def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True):
+def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True, kept=None):
     """Returns (gates fp32 (..., k), experts int32 (..., k), counts int32 (E + 1,) whose last is the number of live
-    tokens, loss fp32 scalar, lse fp32 (T,) or None)."""
+    tokens, loss fp32 scalar, lse fp32 (T,) or None).  `kept`: a second tensor for the counts."""
     _require_cuda(logits)
     if logits.dtype == torch.float64:
         raise RuntimeError("b200norm: router logits of dtype torch.float64 are not supported (float32, float16, bfloat16)")
@@ -50,8 +50,8 @@ def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True):
                 _lib.check(_lib.ERR_ARG)
             _WS_BYTES[key] = ws_bytes
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes > 1 else None
-        _lib.check(lib.b200norm_route_fwd(
-            x.data_ptr(), xs, _ptr(mask), gates.data_ptr(), experts.data_ptr(), _ptr(lse), counts.data_ptr(),
+        _lib.check(lib.b200norm_route_fwd_kept(
+            x.data_ptr(), xs, _ptr(mask), gates.data_ptr(), experts.data_ptr(), _ptr(lse), counts.data_ptr(), _ptr(kept),
             loss.data_ptr(), _ptr(ws), ws_bytes, T, E, k, int(bool(normalize)), code, _raw_stream(index)))
     return gates, experts, counts, loss, lse
 
@@ -97,12 +97,15 @@ class route(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, k, normalize=True, mask=None):
-        gates, experts, counts, loss, lse = _route_fwd(logits, k, normalize, mask, need_lse=ctx.needs_input_grad[0])
+        # The backward's counts are its own: those that are returned may be summed over ranks, which no version counter tells.
+        wanted = ctx.needs_input_grad[0]
+        kept = torch.empty(logits.shape[-1] + 1, dtype=torch.int32, device=logits.device) if wanted else None
+        gates, experts, counts, loss, lse = _route_fwd(logits, k, normalize, mask, need_lse=wanted, kept=kept)
         chosen = counts[:-1]
         ctx.mark_non_differentiable(experts, chosen)
         ctx.set_materialize_grads(False)
-        if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(logits, gates, experts, counts, lse)
+        if wanted:
+            ctx.save_for_backward(logits, gates, experts, kept, lse)
             ctx.normalize = normalize
         return gates, experts, chosen, loss
 
@@ -111,8 +114,8 @@ class route(torch.autograd.Function):
     def backward(ctx, dgates, _dexperts, _dcounts, dloss):
         if dgates is None and dloss is None:
             return None, None, None, None
-        logits, gates, experts, counts, lse = ctx.saved_tensors
-        return _route_bwd(logits, gates, experts, counts, lse, dgates, dloss, ctx.normalize), None, None, None
+        logits, gates, experts, kept, lse = ctx.saved_tensors
+        return _route_bwd(logits, gates, experts, kept, lse, dgates, dloss, ctx.normalize), None, None, None
 
 
 class Router:

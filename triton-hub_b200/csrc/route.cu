@@ -82,7 +82,14 @@ size_t b200norm_route_workspace_bytes(int64_t T, int E, int k, int dtype) {
 
 int b200norm_route_fwd(const void* logits, int64_t row_stride, const uint8_t* mask, float* gates, int* experts, float* lse,
                        int* counts, float* loss, void* workspace, size_t workspace_bytes, int64_t T, int E, int k,
-                       int normalize, int dtype, void* stream_v) {
+                       int normalize, int dtype, void* stream) {
+  return b200norm_route_fwd_kept(logits, row_stride, mask, gates, experts, lse, counts, nullptr, loss, workspace, workspace_bytes,
+                                 T, E, k, normalize, dtype, stream);
+}
+
+int b200norm_route_fwd_kept(const void* logits, int64_t row_stride, const uint8_t* mask, float* gates, int* experts, float* lse,
+                            int* counts, int* kept, float* loss, void* workspace, size_t workspace_bytes, int64_t T, int E,
+                            int k, int normalize, int dtype, void* stream_v) {
   if (int rc = check(T, E, k, dtype)) return rc;
   if (!counts || !loss || (T > 0 && (!logits || !gates || !experts))) return fail(B200NORM_ERR_ARG, "null buffer");
   if (row_stride < E) return fail(B200NORM_ERR_ARG, "row stride smaller than the number of experts");
@@ -96,7 +103,7 @@ int b200norm_route_fwd(const void* logits, int64_t row_stride, const uint8_t* ma
     return fail(B200NORM_ERR_ARG, "workspace needs %zu bytes, 16-byte aligned (got %zu)", need, workspace_bytes);
   RouteParams p = {};
   p.logits = logits; p.stride = row_stride; p.mask = mask; p.gates = gates; p.experts = experts; p.lse = lse;
-  p.counts = counts; p.loss = loss;
+  p.counts = counts; p.kept = kept; p.loss = loss;
   p.part_p = static_cast<float*>(workspace);
   p.columns = columns_of(E);
   p.part_n = reinterpret_cast<int*>(p.part_p + static_cast<size_t>(grid) * p.columns);

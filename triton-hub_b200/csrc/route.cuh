@@ -40,6 +40,7 @@ struct RouteParams {
   int* experts;         // (T, k)
   float* lse;           // (T,) log of the softmax's denominator; -inf marks a token that is not live
   int* counts;          // (E + 1): per expert, then the number of live tokens
+  int* kept;            // the same once more, for a backward whose caller gives `counts` away; may be null
   float* loss;
   float* part_p;  // (gridDim.x, columns) partial sums of p
   int* part_n;    // (gridDim.x, columns) partial counts
@@ -205,6 +206,7 @@ __device__ __forceinline__ double route_share(const RouteParams& p, int e0, int 
   for (int e = e0 + threadIdx.x; e < e1; e += THREADS) {
     const int c = count(e);
     p.counts[e] = c;
+    if (p.kept != nullptr) p.kept[e] = c;
     share += static_cast<double>(sum(e)) * c;
   }
 #pragma unroll
@@ -221,6 +223,7 @@ __device__ __forceinline__ double route_share(const RouteParams& p, int e0, int 
 // One thread: the number of live tokens and the loss.
 __device__ __forceinline__ void route_loss(const RouteParams& p, int n, double share) {
   p.counts[p.E] = n;
+  if (p.kept != nullptr) p.kept[p.E] = n;
   *p.loss = n > 0 ? static_cast<float>(share * p.E / (static_cast<double>(n) * n * p.k)) : 0.f;
 }
 
