@@ -375,7 +375,7 @@ B200NORM_API int b200norm_sample(const void* logits, int64_t row_stride, const f
  * loss = E * sum_e (counts_e / (n k)) * (sum_t p_te / n), 0 when n = 0.
  * Not live: tokens whose mask (T,) byte is 0 (mask may be NULL) or whose logits are all -inf; they get
  * experts -1, gates 0.  Slots left over when fewer than k logits are above -inf get the same.
- * lse (T,), needed for backward only (else NULL): log-sum-exp of the logits, -inf for tokens not live.
+ * lse (T,), needed for backward only (else NULL): log-sum-exp of the logits, rounded to fp32; -inf for tokens not live.
  * b200norm_route_fwd_kept: the same, with the counts written to `kept` (E + 1), too (NULL: not wanted), for callers that hand
  *   `counts` on to code that may change them (a sum over ranks, say) and give `kept` to the backward.
  * b200norm_route_bwd: gradients dgates (T, k) and dloss (one fp32 value on the device), either NULL, to dlogits (T, E)

@@ -257,3 +257,18 @@ def test_returned_counts_are_the_callers(dtype):
             (loss + gates.square().sum()).backward()
             grads.append(v.grad)
         assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("normalize", [False, True])
+def test_logits_far_from_zero(dtype, normalize):
+    # The kernels' exponentials are good to 2 u and, beyond what check() derives, to |d| 1.3 u more for the product d log2 e
+    # (half an ulp of it, and log2 e's own): below 32 u for the differences d of up to 13 here, of 44 u.
+    for E, k in ((64, 4), (7, 2), (33, 3), (160, 6), (512, 8)):
+        x = logits(90, E, torch.float32, seed=E)
+        for offset in (1e4, -1e4, 1e6, -1e6, 1e30, -1e30):
+            check((x + offset).to(dtype), k, normalize)
+        y = x.to(dtype)
+        y[::2] = torch.finfo(dtype).min
+        y[1] = torch.finfo(dtype).max
+        check(y, k, normalize)

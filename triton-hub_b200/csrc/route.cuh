@@ -56,8 +56,8 @@ struct RouteParams {
   int cluster;  // CTAs of the forward's one cluster, which finishes by itself; 0: route_finish_kernel does
 };
 
-// exp(d) of a difference from the maximum: good to 2 ulp besides d's own rounding times d, like expf, in two instructions;
-// below 2^-126 it is 0.
+// exp(d) of a difference d <= 0 from the maximum, in two instructions: good to 2 ulp, and to |d| ulp more for the product with log2 e
+// and its rounding, which expf does without (at d = -10, where a gate is below 5e-5, 7e-7 of it).  Below 2^-126 it is 0.
 __device__ __forceinline__ float exp_below(float d) { return ex2_fast(d * kLog2e); }
 
 // Order-preserving integer of a float; -0 counts as +0.  -inf maps to kKeyNegInf, 0 is below every number.
@@ -397,7 +397,9 @@ __global__ void __launch_bounds__(kRouteFinishThreads) route_finish_kernel(const
 }
 
 // Backward: p comes from the logits and the saved log-sum, the chosen experts' part is put in its place
-// through a row of shared memory per warp.
+// through a row of shared memory per warp.  The log-sum, one fp32 number, has lost of the sum what lies below half an ulp of a
+// large maximum (logits around 1e4: 3e-4 of p; whole rows at the type's lowest value: all of it), so it only shifts the
+// exponentials, and p are their shares of their own sum.
 template <typename T, int EPL>
 __global__ void __launch_bounds__(kRouteBwdThreads) route_bwd_kernel(const RouteParams p) {
   __shared__ __align__(16) float place[kRouteBwdWarps][32 * EPL];
@@ -436,27 +438,31 @@ __global__ void __launch_bounds__(kRouteBwdThreads) route_bwd_kernel(const Route
       gate = p.gates[tok * p.k + lane];
       if (p.dgates != nullptr) dg = p.dgates[tok * p.dgates_stride + lane];
     }
-    float s = 0.f;
+    float s = 0.f, total = 0.f;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
       x[i] = live ? exp_below(x[i] - lse) : 0.f;
+      total += x[i];
       s = fmaf(x[i], c[i], s);
     }
     const bool any = e >= 0;
     float g = any ? gate * dg : 0.f;
-    if (p.normalize) {
-      g -= gate * warp_sum(g);
-      s = warp_sum(s);
-    } else {
-      s = warp_sum(s + g);
-    }
+    total = warp_sum(total);
+    const float inv = live ? rcp_fast(total) : 0.f, sum_g = warp_sum(g);
+    s = warp_sum(s) * inv;
+    if (p.normalize) g -= gate * sum_g;
+    else s += sum_g;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) x[i] *= inv;
     if (any) mine[e] = g;
     __syncwarp();
     T* out = static_cast<T*>(p.dlogits) + tok * p.E;
     const int e0 = lane * EPL;
     float d[EPL];
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) d[i] = x[i] * (c[i] - s) + mine[e0 + i];
+    for (int i = 0; i < EPL; ++i) d[i] = mine[e0 + i];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) d[i] = fmaf(x[i], c[i] - s, d[i]);
     __syncwarp();
     if (any) mine[e] = 0.f;
     if (packed && EPL * sizeof(T) >= 16 && p.E * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.dlogits) & 15u) == 0) {
