@@ -272,3 +272,14 @@ def test_logits_far_from_zero(dtype, normalize):
         y[::2] = torch.finfo(dtype).min
         y[1] = torch.finfo(dtype).max
         check(y, k, normalize)
+
+
+def test_masked_tokens_get_no_gradient_whatever_the_loss():
+    x = logits(40, 32, torch.float32)
+    x[::3, 5] = float("nan")
+    mask = torch.arange(40, device=DEV) % 3 != 0
+    for dl in (float("inf"), float("nan")):
+        v = x.clone().requires_grad_(True)
+        gates, _, _, loss = b200norm.route.apply(v, 4, True, mask)
+        torch.autograd.backward([gates, loss], [torch.full_like(gates, float("inf")), torch.full((), dl, device=DEV)])
+        assert (v.grad[~mask] == 0).all()

@@ -447,8 +447,7 @@ __global__ void __launch_bounds__(kRouteBwdThreads) route_bwd_kernel(const Route
     }
     const bool any = e >= 0;
     float g = any ? gate * dg : 0.f;
-    total = warp_sum(total);
-    const float inv = live ? rcp_fast(total) : 0.f, sum_g = warp_sum(g);
+    const float inv = rcp_fast(warp_sum(total)), sum_g = warp_sum(g);
     s = warp_sum(s) * inv;
     if (p.normalize) g -= gate * sum_g;
     else s += sum_g;
@@ -462,7 +461,7 @@ __global__ void __launch_bounds__(kRouteBwdThreads) route_bwd_kernel(const Route
 #pragma unroll
     for (int i = 0; i < EPL; ++i) d[i] = mine[e0 + i];
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) d[i] = fmaf(x[i], c[i] - s, d[i]);
+    for (int i = 0; i < EPL; ++i) d[i] = live ? fmaf(x[i], c[i] - s, d[i]) : 0.f;  // c may be infinite
     __syncwarp();
     if (any) mine[e] = 0.f;
     if (packed && EPL * sizeof(T) >= 16 && p.E * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(p.dlogits) & 15u) == 0) {
