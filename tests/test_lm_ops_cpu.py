@@ -142,3 +142,23 @@ def test_cpu_tensors_are_refused():
             call()
         with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensors only"):
             call()
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_raises_with_and_without_gradients(grad, monkeypatch):
+    # stand-ins for the kernels' calls: what matters is which way a call takes.  no_grad leaves forward mode on
+    def route_fwd(x, k, *args, **kwargs):
+        return x[..., :k] * 1, x[..., :k].int(), torch.zeros(x.shape[-1] + 1, dtype=torch.int32), x.sum() * 0, None
+
+    monkeypatch.setattr(b200norm.addnorm, "_add_rmsnorm_fwd", lambda x, r, w, eps, **kwargs: (x * 1, x + r, None))
+    monkeypatch.setattr(b200norm.routing, "_route_fwd", route_fwd)
+    x = torch.randn(4, 64)
+    with torch.set_grad_enabled(grad):
+        y, h = b200norm.add_rmsnorm.apply(x, x, None, 1e-6)
+        gates, experts, counts, loss = b200norm.route.apply(x, 2)
+        assert torch.equal(h, x + x) and gates.shape == (4, 2) and counts.shape == (64,)
+        with torch.autograd.forward_ad.dual_level():
+            d = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+            for call in (lambda: b200norm.add_rmsnorm.apply(d, x, None, 1e-6), lambda: b200norm.route.apply(d, 2)):
+                with pytest.raises(NotImplementedError, match="jvp"):
+                    call()

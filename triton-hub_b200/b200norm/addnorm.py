@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import functional as Fn
-from .functional import _code, _flat, _on_device, _params, _ptr, _raw_stream, _require_cuda
+from .functional import _code, _dual_level, _flat, _on_device, _params, _ptr, _raw_stream, _require_cuda, _unrecorded
 
 _ADD_WS = {}  # (device, M, N, dtype codes) -> workspace bytes; the answer never changes
 
@@ -99,7 +99,7 @@ class add_rmsnorm(torch.autograd.Function):
 
     @classmethod
     def apply(cls, x, residual, weight, eps):
-        if not torch.is_grad_enabled():  # nothing to record: a decode step's call is spared autograd's bookkeeping
+        if _unrecorded():  # a decode step's call is spared autograd's bookkeeping
             return _add_rmsnorm_fwd(x, residual, weight, eps, need_rstd=False)[:2]
         return super().apply(x, residual, weight, eps)
 

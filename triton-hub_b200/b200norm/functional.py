@@ -109,6 +109,16 @@ def _params(weight, bias, N, device):
     return weight, bias, (_code(ref, "weight") if ref is not None else _lib.F32)
 
 
+def _dual_level() -> int:
+    """Forward-mode differentiation: the level that is open, -1 without one (0, as if one were, where torch does not say)."""
+    return getattr(torch.autograd.forward_ad, "_current_level", 0)
+
+
+def _unrecorded() -> bool:
+    """Nothing of a call is to be recorded.  no_grad alone does not say so: it leaves forward mode on."""
+    return not torch.is_grad_enabled() and _dual_level() < 0
+
+
 def _ptr(t):
     return t.data_ptr() if t is not None else None
 

@@ -14,7 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .functional import _code, _flat, _on_device, _ptr, _raw_stream, _require_cuda
+from .functional import _code, _flat, _on_device, _ptr, _raw_stream, _require_cuda, _unrecorded
 
 _WS_BYTES = {}  # (device, T, E, k, dtype code) -> workspace bytes; the answer never changes
 
@@ -90,7 +90,7 @@ class route(torch.autograd.Function):
 
     @classmethod
     def apply(cls, logits, k, normalize=True, mask=None):
-        if not torch.is_grad_enabled():  # nothing to record: a decode step's call is spared autograd's bookkeeping
+        if _unrecorded():  # a decode step's call is spared autograd's bookkeeping
             gates, experts, counts, loss, _ = _route_fwd(logits, k, normalize, mask, need_lse=False)
             return gates, experts, counts[:-1], loss
         return super().apply(logits, k, normalize, mask)
