@@ -162,3 +162,13 @@ def test_forward_mode_raises_with_and_without_gradients(grad, monkeypatch):
             for call in (lambda: b200norm.add_rmsnorm.apply(d, x, None, 1e-6), lambda: b200norm.route.apply(d, 2)):
                 with pytest.raises(NotImplementedError, match="jvp"):
                     call()
+
+
+def test_rmsnorm_fp8_refuses_a_tangent(monkeypatch):
+    monkeypatch.setattr(b200norm.addnorm, "_require_cuda", lambda x: None)  # refused before any CUDA call
+    x = torch.randn(4, 64)
+    with torch.no_grad(), torch.autograd.forward_ad.dual_level():
+        d = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for kw in (dict(x=d), dict(x=x, residual=d), dict(x=x, weight=d[0])):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                b200norm.rmsnorm_fp8(**kw)

@@ -133,8 +133,11 @@ def rmsnorm_fp8(x, weight=None, eps=1e-5, *, residual=None, group=0, scale_dtype
 
     For inference: it has no gradient, and refuses inputs that ask for one."""
     _require_cuda(x)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, residual)):
+    given = [t for t in (x, weight, residual) if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
         raise RuntimeError("b200norm: rmsnorm_fp8 has no gradient; call it under torch.no_grad()")
+    if _dual_level() >= 0 and any(torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in given):
+        raise RuntimeError("b200norm: rmsnorm_fp8 has no gradient, nor a forward-mode derivative")
     if group not in (0, 32, 64, 128):
         raise RuntimeError(f"b200norm: a scale covers 32, 64 or 128 columns, or (0) a row; got {group}")
     if scale_dtype not in (torch.float32, torch.float8_e8m0fnu):
