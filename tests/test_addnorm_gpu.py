@@ -471,3 +471,27 @@ def test_fp8_row_scale_is_finite_where_the_norm_is(t):
         check_fp8(x, None, w, 1e-6, 0, False)
         check_fp8(x, torch.zeros_like(x), w, 1e-6, 0, True)
         check_fp8(x, None, w, 1e-6, 128, False)
+
+
+def kernels_of(call):
+    """Names of the operators' kernels that a call launches."""
+    call()
+    torch.cuda.synchronize()
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as p:
+        call()
+        torch.cuda.synchronize()
+    names = [e.name for e in p.events() if "addnorm" in e.name]
+    return names or pytest.skip("the profiler shows no kernels here")
+
+
+@pytest.mark.parametrize("t,r,lengths", [(F32, F32, (6340, 6344, 6356, 6368, 6372)), (BF16, BF16, (13568, 13576, 13632, 13648, 13656)),
+                                         (F16, F32, (7608, 7616, 7640, 7648, 11416, 11424, 11464, 11472))])
+def test_lengths_where_a_ring_just_fits(t, r, lengths):
+    # a slot more than the row's kernel has room for sent these to the kernel for unlike alignments
+    for N in lengths:
+        x, res, w, dy, dh = make(300, N, t, r, t, seed=N)
+        y, h, rstd = A._add_rmsnorm_fwd(x, res, w, 1e-6)
+        check_backward(h, dy, dh, w, 1e-6, *A._add_rmsnorm_bwd(h, dy, dh, w, rstd))
+        check_backward(h, dy, None, w, 1e-6, *A._add_rmsnorm_bwd(h, dy, None, w, rstd))
+        names = kernels_of(lambda: A._add_rmsnorm_bwd(h, dy, dh, w, rstd))
+        assert any("addnorm_bwd_kernel" in n for n in names), (N, names)  # not the one that works element by element

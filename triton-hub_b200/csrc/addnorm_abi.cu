@@ -63,11 +63,14 @@ struct Plan {
   size_t smem;
 };
 
+// Dynamic shared memory of a CTA, at most: the rest is its static part.
+constexpr size_t kMostSmem = kMaxSmemPerCta - 4096;
+
 // Slots of a ring: as many, up to `most`, as leave room for three, two or one CTA per SM (228 KB, 1 KB of it
 // reserved per CTA, and a little static shared memory), at least two; 0 when two do not fit.  Four slots always, with fewer
 // CTAs, is the same within 2 % (backward of 16384 x 4096 bf16 84.3 instead of 83.5 us, of 16384 x 1024 29.3 instead of 28.6).
 int ring_stages(size_t slot, int most, size_t fixed, int groups, size_t* smem) {
-  for (size_t cap : {74 * 1024, 112 * 1024, 224 * 1024})
+  for (size_t cap : {size_t{74 * 1024}, size_t{112 * 1024}, kMostSmem})
     for (int stages = most; stages >= 2; --stages)
       if (fixed + slot * stages * groups <= cap) {
         *smem = fixed + slot * stages * groups;
@@ -128,7 +131,7 @@ int plan(DeviceState& dev, const AddNormTable* t, Which which, Layout layout, in
       out->smem = std::max(ring, fixed + sums);
     }
     // a row without a kernel that fits
-    if (out->fn == nullptr || out->smem > kMaxSmemPerCta - 4096) s = nullptr;
+    if (out->fn == nullptr || out->smem > kMostSmem) s = nullptr;
   }
   if (s == nullptr) {
     out->fn = which == kFwd ? t->fwd_any : which == kFp8 ? t->fp8_any : t->bwd_any;
