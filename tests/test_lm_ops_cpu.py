@@ -172,3 +172,29 @@ def test_rmsnorm_fp8_refuses_a_tangent(monkeypatch):
         for kw in (dict(x=d), dict(x=x, residual=d), dict(x=x, weight=d[0])):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 b200norm.rmsnorm_fp8(**kw)
+
+
+def test_addresses_inside_an_element_are_refused(lib):
+    B, F = _lib.BF16, _lib.F32
+
+    def refused(rc):
+        return rc == ERR and said(lib, b"inside an element")
+
+    for name in ("x", "r", "y", "h"):
+        assert refused(add_fwd(lib, **{name: P + 2})) and refused(add_fwd(lib, io=B, res=B, **{name: P + 1}))
+    for name in ("h", "dy", "rstd", "dx"):
+        assert refused(add_bwd(lib, **{name: P + 2}))
+        assert refused(add_bwd(lib, io=B, dres=P, **{name: P + 1}))
+    assert refused(add_bwd(lib, io=B, dres=P + 2)) and refused(add_bwd(lib, dw=P + 2))
+    assert refused(fp8(lib, x=P + 2)) and refused(fp8(lib, scale=P + 1)) and refused(fp8(lib, r=P + 2)) and refused(fp8(lib, r=P, h=P + 3))
+    for dtype, step in ((F, 2), (B, 1)):
+        assert refused(route_fwd(lib, dtype=dtype, logits=P + step)) and refused(route_bwd(lib, dtype=dtype, logits=P + step))
+        assert refused(route_bwd(lib, dtype=dtype, dlogits=P + step)) and refused(sample(lib, dtype=dtype, logits=P + step))
+    for name in ("gates", "experts", "counts"):
+        assert refused(route_fwd(lib, **{name: P + 2})) and refused(route_bwd(lib, **{name: P + 2}))
+    assert refused(route_fwd(lib, loss=P + 1)) and refused(route_bwd(lib, lse=P + 2))
+    assert refused(sample(lib, uniform=P + 2)) and refused(sample(lib, tokens=P + 4))
+    # a weight's and a weight gradient's elements are those of its own type
+    for w, step in ((_lib.F64, 4), (F, 2), (B, 1)):
+        rc = lib.b200norm_add_rms_fwd(P, 8, P, 8, P + step, P, 8, P, 8, P, 4, 8, 1e-6, F, F, w, None)
+        assert refused(rc)

@@ -46,7 +46,6 @@ Layout layout_of(const Buffer* b, int n, int64_t N, int vec, const void* w, int*
   for (int i = 0; i < n; ++i) {
     if (b[i].p == nullptr) continue;
     const uintptr_t a = reinterpret_cast<uintptr_t>(b[i].p);
-    if (a % b[i].size != 0) return kAny;
     const int64_t ph = static_cast<int64_t>((a / b[i].size) % vec), st = b[i].stride % vec;
     if (phase >= 0 && (ph != phase || st != stride)) return kAny;
     phase = ph;
@@ -162,9 +161,12 @@ int forward(bool fp8, const void* x, int64_t xs, const void* r, int64_t rs, cons
   if (!x || !y || (fp8 && !scale) || (!fp8 && (!r || !h))) return fail(B200NORM_ERR_ARG, "null buffer");
   if (r == nullptr && h != nullptr) return fail(B200NORM_ERR_ARG, "h is the sum with a residual: there is none");
   if (xs < N || ys < N || (r && rs < N) || (h && hs < N)) return fail(B200NORM_ERR_ARG, "row stride smaller than N");
+  const AddNormTable* t = table_for(io, res);
+  if (!on_element(x, t->size_t_) || !on_element(r, t->size_r) || !on_element(w, dtype_size(w_dtype)) ||
+      !on_element(y, fp8 ? 1 : t->size_t_) || !on_element(h, t->size_r) || !on_element(rstd, 4) || !on_element(scale, e8m0 ? 1 : 4))
+    return fail_off_element();
   DeviceState* dev = nullptr;
   if (int rc = fp8 ? device_state(&dev) : device_caches(&dev)) return rc;
-  const AddNormTable* t = table_for(io, res);
   const Buffer bufs[4] = {{x, xs, t->size_t_}, {r, rs, t->size_r}, {y, ys, fp8 ? 1 : t->size_t_}, {h, hs, t->size_r}};
   int period;
   const Layout layout = layout_of(bufs, 4, N, 16 / t->size_t_, w, &period);
@@ -227,9 +229,12 @@ int b200norm_add_rms_bwd(const void* h, int64_t h_row_stride, const void* dy, in
     return fail(B200NORM_ERR_ARG, "dres is written only when the residual's type is not that of the rows: it equals dx");
   if (h_row_stride < N || dy_row_stride < N || dx_row_stride < N || (dh && dh_row_stride < N) || (dres && dres_row_stride < N))
     return fail(B200NORM_ERR_ARG, "row stride smaller than N");
+  const AddNormTable* t = table_for(io_dtype, res_dtype);
+  if (!on_element(h, t->size_r) || !on_element(dy, t->size_t_) || !on_element(dh, t->size_r) || !on_element(w, dtype_size(w_dtype)) ||
+      !on_element(rstd, 4) || !on_element(dx, t->size_t_) || !on_element(dres, t->size_r) || !on_element(dw, dtype_size(w_dtype)))
+    return fail_off_element();
   DeviceState* dev = nullptr;
   if (int rc = device_state(&dev)) return rc;
-  const AddNormTable* t = table_for(io_dtype, res_dtype);
   const Buffer bufs[5] = {{dy, dy_row_stride, t->size_t_}, {h, h_row_stride, t->size_r}, {dh, dh_row_stride, t->size_r},
                           {dx, dx_row_stride, t->size_t_}, {dres, dres_row_stride, t->size_r}};
   int period;

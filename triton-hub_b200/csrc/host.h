@@ -18,6 +18,11 @@ constexpr size_t kMaxSmemPerCta = 227 * 1024;  // opt-in dynamic + static shared
 // Stores the thread's error text and returns `code`.
 int fail(int code, const char* fmt, ...);
 
+// Whether a buffer (or none) starts on a boundary of its elements, `size` bytes each, a power of two.
+inline bool on_element(const void* p, size_t size) { return (reinterpret_cast<uintptr_t>(p) & (size - 1)) == 0; }
+inline int fail_off_element() { return fail(B200NORM_ERR_ARG, "a buffer starts inside an element: its address is no multiple of their size"); }
+inline size_t dtype_size(int dtype) { return dtype == B200NORM_F64 ? 8 : dtype == B200NORM_F32 ? 4 : 2; }
+
 struct DeviceState {
   // Launch planning: SM count, occupancies, shared-memory allowances.  Set up without allocating
   // anything, and shared by every entry point -- a kernel's shared-memory allowance is a property

@@ -93,6 +93,9 @@ int b200norm_route_fwd_kept(const void* logits, int64_t row_stride, const uint8_
   if (int rc = check(T, E, k, dtype)) return rc;
   if (!counts || !loss || (T > 0 && (!logits || !gates || !experts))) return fail(B200NORM_ERR_ARG, "null buffer");
   if (row_stride < E) return fail(B200NORM_ERR_ARG, "row stride smaller than the number of experts");
+  if (!on_element(logits, dtype_size(dtype)) || !on_element(gates, 4) || !on_element(experts, 4) || !on_element(lse, 4) ||
+      !on_element(counts, 4) || !on_element(kept, 4) || !on_element(loss, 4))
+    return fail_off_element();
   DeviceState* dev = nullptr;
   if (int rc = device_caches(&dev)) return rc;
   const void* fn = route_fn(dtype, E, false);
@@ -124,6 +127,9 @@ int b200norm_route_bwd(const void* logits, int64_t row_stride, const float* gate
   if (T == 0) return B200NORM_OK;
   if (!logits || !gates || !experts || !lse || !counts || !dlogits) return fail(B200NORM_ERR_ARG, "null buffer");
   if (row_stride < E || (dgates && dgates_row_stride < k)) return fail(B200NORM_ERR_ARG, "row stride smaller than the row");
+  if (!on_element(logits, dtype_size(dtype)) || !on_element(gates, 4) || !on_element(experts, 4) || !on_element(lse, 4) ||
+      !on_element(counts, 4) || !on_element(dgates, 4) || !on_element(dloss, 4) || !on_element(dlogits, dtype_size(dtype)))
+    return fail_off_element();
   DeviceState* dev = nullptr;
   if (int rc = device_caches(&dev)) return rc;
   const void* fn = route_fn(dtype, E, true);

@@ -35,9 +35,12 @@ extern "C" int b200norm_sample(const void* logits, int64_t row_stride, const flo
   if (M > INT32_MAX / kSampleMaxCluster) return fail(B200NORM_ERR_ARG, "too many rows: %lld", (long long)M);
   if (!logits || !uniform || !tokens) return fail(B200NORM_ERR_ARG, "null logits / uniform / tokens");
   if (row_stride < V) return fail(B200NORM_ERR_ARG, "row stride smaller than the vocabulary");
+  const int es = static_cast<int>(dtype_size(dtype)), vec = 16 / es;
+  if (!on_element(logits, es) || !on_element(uniform, 4) || !on_element(temperature_v, 4) || !on_element(top_k_v, 4) ||
+      !on_element(top_p_v, 4) || !on_element(min_p_v, 4) || !on_element(tokens, 8))
+    return fail_off_element();
   DeviceState* dev = nullptr;
   if (int rc = device_caches(&dev)) return rc;
-  const int es = dtype == B200NORM_F32 ? 4 : 2, vec = 16 / es;
   // CTAs per row: as few as have parts of up to 112 KB.  Parts of up to 98 KB let two CTAs share an SM (228 KB, 16 of it
   // static or reserved per CTA), so that one's barriers hide behind the other's arithmetic, but each CTA has its fixed
   // costs: top-p 0.9 of 512 x 65536 bf16 takes 238 us with 1 CTA a row, 189 with 2, 266 with 4; 512 x 50257 fp32 157 with 2
