@@ -33,9 +33,9 @@
  *     (a cudaStream_t passed as void*; NULL = legacy default stream).  It never
  *     synchronises, never changes the current device and, after the first call on a device,
  *     never allocates.  The first call on a device caches the device's SM count, the
- *     occupancy of each kernel and maps a small pinned status word; make that call before
- *     any stream capture.
- *   - Alignment.  Any base address, row stride and row length are accepted, like the reference's
+ *     occupancy of each kernel and maps a small pinned status word; it may be a captured one.
+ *   - Alignment.  Any base address on an element's boundary (the residual norms, the expert
+ *     and the token choice refuse others), row stride and row length are accepted, like the reference's
  *     masked loads (layernorm.py:28-46, `cols < N`).  Fastest: every row of every buffer starts on
  *     a 16-byte boundary and is a multiple of 16 bytes long.  Next: rows of at least 0.5 - 2 KB
  *     whose buffers are misaligned ALIKE (x, y -- and dy, dx -- start each row at the same offset

@@ -1,6 +1,9 @@
 """The residual norms, the expert choice and the token choice as they are used together: a training step, a serving step in
 one CUDA graph, several streams and threads, outputs inside larger buffers, rows more than 2^31 elements apart."""
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -426,3 +429,30 @@ def test_settings_of_other_integer_types():
     assert all(torch.equal(p, q) for p, q in zip(a, b))
     for p, q in zip(b200norm.rmsnorm_fp8(x, group=np.int64(32)), b200norm.rmsnorm_fp8(x, group=32)):
         assert torch.equal(p.view(torch.uint8), q.view(torch.uint8))
+
+
+FIRST_CALL = """
+import sys, torch
+sys.path.insert(0, %r)
+import b200norm
+from b200norm import addnorm as A, routing as R
+x = torch.randn(3000, 4096, device="cuda:0")
+u = torch.rand(3000, device="cuda:0")
+calls = {"fp8": lambda: b200norm.rmsnorm_fp8(x, group=128), "add": lambda: A._add_rmsnorm_bwd(x, x, None, u.new_ones(4096), u),
+         "route": lambda: R._route_fwd(x[:, :64], 4), "sample": lambda: (b200norm.sample(x, u, top_p=0.9),)}
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = calls[sys.argv[1]]()
+graph.replay()
+for a, b in zip(got, calls[sys.argv[1]]()):
+    assert torch.equal(a.reshape(-1).view(torch.uint8), b.reshape(-1).view(torch.uint8))
+print("same")
+"""
+
+
+@pytest.mark.parametrize("name", ["fp8", "add", "route", "sample"])
+def test_the_first_call_of_a_process_may_be_a_captured_one(name):
+    root = str(Path(b200norm.__file__).resolve().parent.parent)
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL % root, name], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]

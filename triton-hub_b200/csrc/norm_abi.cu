@@ -77,7 +77,12 @@ int device_state(DeviceState** out) {
   DeviceState* s = nullptr;
   if (int rc = device_caches(&s)) return rc;
   std::call_once(s->status_once, [&]() {
+    // The word is no part of what a capture records; a capture on this thread only has to let the allocation pass.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    s->status_err = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (s->status_err != cudaSuccess) return;
     s->status_err = cudaHostAlloc(reinterpret_cast<void**>(&s->status_host), 64, cudaHostAllocMapped);
+    cudaThreadExchangeStreamCaptureMode(&mode);
     if (s->status_err != cudaSuccess) return;
     std::memset(s->status_host, 0, 64);
     s->status_err = cudaHostGetDevicePointer(reinterpret_cast<void**>(&s->status_dev), s->status_host, 0);
