@@ -259,3 +259,12 @@ def test_prefixes_that_end_above_and_below_min_p(dtype):
                 check(rows, u, top_p=p, min_p=mp, top_k=3000, temperature=1.4)
     spread = torch.linspace(0, 1, 40, device=DEV)
     check(x, u, top_p=0.3 + 0.7 * spread.flip(0), min_p=0.1 * spread ** 3, temperature=0.8)
+
+
+def test_top_k_of_64_bits_without_a_sign():
+    x, u = make(6, 1000, torch.float32)
+    for many in (2 ** 32 + 5, 2 ** 63 + 5):
+        k = torch.full((6,), many, dtype=torch.uint64, device=DEV)
+        assert torch.equal(b200norm.sample(x, u, top_k=k), b200norm.sample(x, u))
+    k = torch.full((6,), 5, dtype=torch.uint64, device=DEV)
+    assert torch.equal(b200norm.sample(x, u, top_k=k), b200norm.sample(x, u, top_k=5))

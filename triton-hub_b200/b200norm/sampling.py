@@ -27,8 +27,8 @@ def _setting(value, name, shape, device, dtype, low, high):
                                f"{tuple(value.shape)} on {value.device}")
         if value.dtype == torch.bool or value.is_floating_point() != (dtype == torch.float32):
             raise RuntimeError(f"b200norm: {name} of dtype {value.dtype}")
-        if value.dtype == torch.int64:  # a larger number means the same as the largest of 32 bits
-            value = value.clamp(-1, 2 ** 31 - 1)
+        if value.dtype in (torch.int64, torch.uint64):  # a larger number means the same as the largest of 32 bits, or as -1
+            value = value.view(torch.int64).clamp(-1, 2 ** 31 - 1)
         return value.to(dtype).contiguous(), 0
     if not low <= value <= high:
         raise RuntimeError(f"b200norm: {name} must lie in [{low}, {high}], got {value}")
