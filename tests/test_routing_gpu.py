@@ -283,3 +283,13 @@ def test_masked_tokens_get_no_gradient_whatever_the_loss():
         gates, _, _, loss = b200norm.route.apply(v, 4, True, mask)
         torch.autograd.backward([gates, loss], [torch.full_like(gates, float("inf")), torch.full((), dl, device=DEV)])
         assert (v.grad[~mask] == 0).all()
+
+
+def test_negative_nan_shows():
+    for normalize in (False, True):
+        for E in (8, 16, 64, 300, 1000):
+            x = logits(10, E, torch.float32)
+            x.view(torch.int32)[4, 3] = -1  # a NaN with its sign set
+            g, e, _, loss = b200norm.route.apply(x, 3, normalize)
+            assert g[4].isnan().all() and loss.isnan() and g[[0, 1, 2, 3, 5, 6, 7, 8, 9]].isfinite().all()
+            assert ((e >= 0) & (e < E)).all()

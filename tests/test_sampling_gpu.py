@@ -268,3 +268,13 @@ def test_top_k_of_64_bits_without_a_sign():
         assert torch.equal(b200norm.sample(x, u, top_k=k), b200norm.sample(x, u))
     k = torch.full((6,), 5, dtype=torch.uint64, device=DEV)
     assert torch.equal(b200norm.sample(x, u, top_k=k), b200norm.sample(x, u, top_k=5))
+
+
+def test_a_row_alone_over_eight_ctas_and_in_a_batch_over_two():
+    # 40000 fp32: parts of 20 KB when alone, of 80 KB when 200 rows fill the SMs
+    x, u = make(200, 40000, torch.float32, seed=6)
+    for kw in (dict(), dict(top_k=50), dict(top_k=2000), dict(top_p=0.95), dict(min_p=0.01), dict(top_k=3000, top_p=0.9, min_p=1e-3)):
+        whole = b200norm.sample(x, u, **kw)
+        assert torch.equal(whole, reference(x, u, **kw))
+        for i in range(200):
+            assert torch.equal(b200norm.sample(x[i:i + 1], u[i:i + 1], **kw), whole[i:i + 1])
