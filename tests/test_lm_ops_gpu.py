@@ -456,3 +456,14 @@ def test_the_first_call_of_a_process_may_be_a_captured_one(name):
     root = str(Path(b200norm.__file__).resolve().parent.parent)
     done = subprocess.run([sys.executable, "-c", FIRST_CALL % root, name], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
+
+
+def test_tables_of_sizes_stay_bounded():
+    # a server meets a new number of tokens at almost every step
+    x, w = randn(6000, 16), torch.ones(16, device=DEV)
+    rstd = torch.ones(6000, device=DEV)
+    for T in range(1, 6000):
+        R._route_fwd(x[:T], 2, need_lse=False)
+        A._add_rmsnorm_bwd(x[:T], x[:T], None, w, rstd[:T])
+    for table in (R._workspace_bytes, A._workspace_bytes):
+        assert 0 < table.cache_info().currsize < 5000

@@ -9,6 +9,8 @@ the forward's values.  The reference has neither form; the modules keep RMSNorm'
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -16,7 +18,14 @@ from . import _lib
 from . import functional as Fn
 from .functional import _code, _dual_level, _flat, _on_device, _params, _ptr, _raw_stream, _require_cuda, _unrecorded
 
-_ADD_WS = {}  # (device, M, N, dtype codes) -> workspace bytes; the answer never changes
+
+@lru_cache(maxsize=4096)  # the answer never changes; of as many sizes as a program meets in turn, not of all it ever met
+def _workspace_bytes(index, M, N, io, res):
+    """Bytes of the backward's workspace; `index` is the current device."""
+    n = _lib.load().b200norm_add_rms_bwd_workspace_bytes(M, N, io, res)
+    if n == 0:
+        _lib.check(_lib.ERR_ARG)
+    return n
 
 
 def _check_residual(x, residual):
@@ -80,13 +89,7 @@ def _add_rmsnorm_bwd(h, dy, dh, weight, rstd, *, need_dw=True):
     with _on_device(index):
         ws, ws_bytes = None, 0
         if dw is not None:
-            key = (index, M, N, io, res)
-            ws_bytes = _ADD_WS.get(key)
-            if ws_bytes is None:
-                ws_bytes = lib.b200norm_add_rms_bwd_workspace_bytes(M, N, io, res)
-                if ws_bytes == 0:
-                    _lib.check(_lib.ERR_ARG)
-                _ADD_WS[key] = ws_bytes
+            ws_bytes = _workspace_bytes(index, M, N, io, res)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
         _lib.check(lib.b200norm_add_rms_bwd(
             hr.data_ptr(), hs, dyr.data_ptr(), dys, _ptr(dhr), dhs, _ptr(weight), rstd.data_ptr(), dx.data_ptr(), N, _ptr(dres),

@@ -8,6 +8,7 @@ The gradient reaches the logits through the gates and through P; f is a count.  
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from operator import index as as_int
 
 import torch
@@ -16,7 +17,14 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 from .functional import _code, _flat, _on_device, _ptr, _raw_stream, _require_cuda, _unrecorded
 
-_WS_BYTES = {}  # (device, T, E, k, dtype code) -> workspace bytes; the answer never changes
+
+@lru_cache(maxsize=4096)  # the answer never changes; of as many sizes as a program meets in turn, not of all it ever met
+def _workspace_bytes(index, T, E, k, code):
+    """Bytes of the forward's workspace, 1 for none; `index` is the current device."""
+    n = _lib.load().b200norm_route_workspace_bytes(T, E, k, code)
+    if n == 0:
+        _lib.check(_lib.ERR_ARG)
+    return n
 
 
 def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True, kept=None):
@@ -42,13 +50,7 @@ def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True, kept=None
     lib = _lib.load()
     index = device.index
     with _on_device(index):
-        key = (index, T, E, k, code)
-        ws_bytes = _WS_BYTES.get(key)
-        if ws_bytes is None:
-            ws_bytes = lib.b200norm_route_workspace_bytes(T, E, k, code)
-            if ws_bytes == 0:
-                _lib.check(_lib.ERR_ARG)
-            _WS_BYTES[key] = ws_bytes
+        ws_bytes = _workspace_bytes(index, T, E, k, code)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes > 1 else None
         _lib.check(lib.b200norm_route_fwd_kept(
             x.data_ptr(), xs, _ptr(mask), gates.data_ptr(), experts.data_ptr(), _ptr(lse), counts.data_ptr(), _ptr(kept),
