@@ -27,9 +27,10 @@ def _workspace_bytes(index, T, E, k, code):
     return n
 
 
-def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True, kept=None):
+def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True, keep=False):
     """Returns (gates fp32 (..., k), experts int32 (..., k), counts int32 (E + 1,) whose last is the number of live
-    tokens, loss fp32 scalar, lse fp32 (T,) or None).  `kept`: a second tensor for the counts."""
+    tokens, loss fp32 scalar, lse fp32 (T,) or None).  `keep`: lse is (T + E + 1,), behind the tokens' values the bits of the
+    counts once more, for a backward whose caller gives `counts` away."""
     _require_cuda(logits)
     if logits.dtype == torch.float64:
         raise RuntimeError("b200norm: router logits of dtype torch.float64 are not supported (float32, float16, bfloat16)")
@@ -46,20 +47,22 @@ def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True, kept=None
     experts = torch.empty(*shape, k, dtype=torch.int32, device=device)
     counts = torch.empty(E + 1, dtype=torch.int32, device=device)
     loss = gates.new_empty(())
-    lse = torch.empty(T, dtype=torch.float32, device=device) if need_lse else None
+    lse = torch.empty(T + E + 1 if keep else T, dtype=torch.float32, device=device) if need_lse or keep else None
     lib = _lib.load()
     index = device.index
     with _on_device(index):
         ws_bytes = _workspace_bytes(index, T, E, k, code)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes > 1 else None
         _lib.check(lib.b200norm_route_fwd_kept(
-            x.data_ptr(), xs, _ptr(mask), gates.data_ptr(), experts.data_ptr(), _ptr(lse), counts.data_ptr(), _ptr(kept),
-            loss.data_ptr(), _ptr(ws), ws_bytes, T, E, k, int(bool(normalize)), code, _raw_stream(index)))
+            x.data_ptr(), xs, _ptr(mask), gates.data_ptr(), experts.data_ptr(), _ptr(lse), counts.data_ptr(),
+            lse.data_ptr() + 4 * T if keep else None, loss.data_ptr(), _ptr(ws), ws_bytes, T, E, k, int(bool(normalize)), code,
+            _raw_stream(index)))
     return gates, experts, counts, loss, lse
 
 
 def _route_bwd(logits, gates, experts, counts, lse, dgates, dloss, normalize=True):
-    """Gradients of (gates, loss), either of which may be None, with respect to the logits."""
+    """Gradients of (gates, loss), either of which may be None, with respect to the logits.  counts None: those that
+    _route_fwd kept behind lse."""
     _require_cuda(logits)
     k = experts.shape[-1]
     x, T, E, xs = _flat(logits)
@@ -77,9 +80,9 @@ def _route_bwd(logits, gates, experts, counts, lse, dgates, dloss, normalize=Tru
     index = logits.device.index
     with _on_device(index):
         _lib.check(lib.b200norm_route_bwd(
-            x.data_ptr(), xs, gates.data_ptr(), experts.data_ptr(), lse.data_ptr(), counts.data_ptr(),
-            _ptr(dgates), dgs, _ptr(dloss), dlogits.data_ptr(), T, E, k,
-            int(bool(normalize)), _code(x, "router logits"), _raw_stream(index)))
+            x.data_ptr(), xs, gates.data_ptr(), experts.data_ptr(), lse.data_ptr(),
+            lse.data_ptr() + 4 * T if counts is None else counts.data_ptr(), _ptr(dgates), dgs, _ptr(dloss), dlogits.data_ptr(),
+            T, E, k, int(bool(normalize)), _code(x, "router logits"), _raw_stream(index)))
     return dlogits
 
 
@@ -101,13 +104,12 @@ class route(torch.autograd.Function):
     def forward(ctx, logits, k, normalize=True, mask=None):
         # The backward's counts are its own: those that are returned may be summed over ranks, which no version counter tells.
         wanted = ctx.needs_input_grad[0]
-        kept = torch.empty(logits.shape[-1] + 1, dtype=torch.int32, device=logits.device) if wanted else None
-        gates, experts, counts, loss, lse = _route_fwd(logits, k, normalize, mask, need_lse=wanted, kept=kept)
+        gates, experts, counts, loss, lse = _route_fwd(logits, k, normalize, mask, need_lse=wanted, keep=wanted)
         chosen = counts[:-1]
         ctx.mark_non_differentiable(experts, chosen)
         ctx.set_materialize_grads(False)
         if wanted:
-            ctx.save_for_backward(logits, gates, experts, kept, lse)
+            ctx.save_for_backward(logits, gates, experts, lse)
             ctx.normalize = normalize
         return gates, experts, chosen, loss
 
@@ -116,8 +118,8 @@ class route(torch.autograd.Function):
     def backward(ctx, dgates, _dexperts, _dcounts, dloss):
         if dgates is None and dloss is None:
             return None, None, None, None
-        logits, gates, experts, kept, lse = ctx.saved_tensors
-        return _route_bwd(logits, gates, experts, kept, lse, dgates, dloss, ctx.normalize), None, None, None
+        logits, gates, experts, lse = ctx.saved_tensors
+        return _route_bwd(logits, gates, experts, None, lse, dgates, dloss, ctx.normalize), None, None, None
 
 
 class Router:
