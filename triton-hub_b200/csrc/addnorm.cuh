@@ -5,7 +5,7 @@
 //   backward   xhat = h * rstd;  wdy = w * dy;  c1 = sum(xhat * wdy) / N
 //              d = (wdy - xhat * c1) * rstd + dh;  dx = round_T(d), dr = round_R(d);  dw = sum_rows(dy * xhat)
 //   8 bits     a_g = max |y| over a group of columns;  s_g = max(a_g, 2^-64) / 448 (or the next power of two
-//              up);  q = e4m3(y / s_g), from the unrounded y
+//              up);  q = e4m3(y / s_g), from the unrounded y; of a whole row a_g = rstd max |h w|
 //
 // T is the storage type of x, y, dy and dx; R that of the residual stream (r, h, dh, dr): T or fp32.  h is
 // rounded to R before the statistics are taken, so that y is the norm of the h that is returned and that
@@ -16,14 +16,16 @@
 // enough of them in flight.  A row lives in the registers of TPR threads, LD 16-byte packets each.
 //   16384 x 4096 bf16           forward 84 us, backward 83: 0.98 of the copy bandwidth
 //   6001 x 5120 bf16, fp32 h    forward 63 us (0.90), backward 76 (0.99)
-//   16384 x 5120 bf16 to 8 bits, a scale a row, with residual  93 us (0.96)
-//   8191 x 4104 fp16 to 8 bits, a scale per 32 columns  28 us (0.56), bound by instructions
-//   8182 x 4101 bf16 (rows off the packet boundaries)  forward 45 us (0.91), backward 52 (0.79), to 8 bits per 128 columns 44
-//     (0.36); 3001 x 1001 fp16 7 and 11 us, of which the launches, the first loads and the column reduce are half
+//   16384 x 5120 bf16 to 8 bits, a scale a row, with residual  96 us (0.94)
+//   8191 x 4104 fp16 to 8 bits, a scale per 32 columns  28 us (0.55): 20 instructions an element, the issue slots 67 % busy, the
+//     rest of the time mostly in shared memory's latency and the row's barrier
+//   8182 x 4101 bf16 (rows off the packet boundaries)  forward 45 us (0.91), backward 52 (0.79), to 8 bits per 128 columns 47
+//     (0.33); 3001 x 1001 fp16 7 and 11 us, of which the launches, the first loads and the column reduce are half
 //   229824 x 146 bf16  forward 66 us (0.62), backward 73 (0.56): 18 packets cost the instructions of 32
 // The backward's ring makes 8192 x 8192 bf16 113 -> 86 us and 6001 x 5120 with fp32 h 100 -> 76; 16384 x 1024 is as quick
 // without one.  The forward needs none (it writes as much as it reads), but for the 8-bit form without a residual: 20480 x 4096
-// bf16, a scale per 32 columns, 63 -> 51 us.
+// bf16, a scale per 32 columns, 63 -> 51 us.  (This pair and those at the choices of shapes were measured with quotients of one
+// product; those of two, see Fp8Scale, add 2 to 8 % to 8-bit forms with fp32 scales: 51 -> 53 here.)
 #pragma once
 
 #include "norm_common.cuh"
@@ -287,10 +289,13 @@ __host__ __device__ constexpr int addnorm_threads(int tpr) { return tpr < 160 ? 
 // registers beside the row.
 __host__ __device__ constexpr bool addnorm_wide(int ld, int vec, int tpr) { return ld * vec > 24 || tpr > 768; }
 
-// CTAs per SM that the register allocation leaves room for: as many threads as run without spills, by the elements a
-// thread holds; more (`lean`) where that pays.  Lean makes the forward of 8182 x 4101 bf16 50 -> 45 us, of 4091 x 4101 fp32 61
-// -> 45, the 8-bit form of 8192 x 8192 bf16 58 -> 48, the backward of 335544 x 100 bf16 85 -> 72, and costs 16384 x 2048 bf16
-// forward 2 us of 43.
+// CTAs per SM that the register allocation leaves room for, as so many threads: forward 512 (128 registers) above 16 elements a
+// thread, else 768 (80) or, `lean`, 1024 (64); backward 512 or, lean, 768.  Lean are all forwards but the one through a ring with a
+// scale a row, and backwards of up to 8 elements without a ring.  It makes the forward of 8182 x 4101 bf16 50 -> 45 us, of 4091 x
+// 4101 fp32 61 -> 45, the 8-bit form of 8192 x 8192 bf16 58 -> 48, the backward of 335544 x 100 bf16 85 -> 72, and costs
+// 16384 x 2048 bf16 forward 2 us of 43.  Lean forwards spill a little: 4 to 76 bytes a thread in a dozen kernels of 16-bit rows on
+// 8 to 128 threads, up to 192 in those with an fp32 residual, up to 52 in fp32 ones of four packets; the times are with that.  1024
+// threads have no more than 64 registers: with two packets up to 24 bytes are spilled, with four 12 to 484.
 __host__ __device__ constexpr int addnorm_fwd_ctas(int elements, int tpr, bool lean) {
   const int n = (elements > 16 ? 512 : lean ? 1024 : 768) / addnorm_threads(tpr);
   return n < 1 ? 1 : n;

@@ -14,7 +14,7 @@
 // A warp takes a token; lane i holds the EPL neighbouring experts from i * EPL on, so the lowest of several
 // lanes with one maximum also has the lowest index.  Reading the logits once is all that memory asks for (65536 x 128
 // fp32: 6 us); what bounds the forward is the instructions of the choice, the exponentials and the sums, 475 a token
-// (44 us, 37 of them in route_fwd_kernel), and the backward (16 us for 10 us of traffic) their share of it.  Column sums of p
+// (44 us, 37 of them in route_fwd_kernel), and the backward (17 us for 11 us of traffic; 183 a token) their share of it.  Column sums of p
 // stay in registers over all of a warp's tokens and meet once per CTA, in shared memory; counts are shared-memory integer
 // atomics, whose order cannot show; the CTAs' partial rows are added in one fixed order.
 #pragma once
