@@ -293,3 +293,18 @@ def test_negative_nan_shows():
             g, e, _, loss = b200norm.route.apply(x, 3, normalize)
             assert g[4].isnan().all() and loss.isnan() and g[[0, 1, 2, 3, 5, 6, 7, 8, 9]].isfinite().all()
             assert ((e >= 0) & (e < E)).all()
+
+
+def test_hooks_that_round_saved_numbers():
+    # saved tensors in 16 bits: logits that have no more, gates and log-sums off by 2^-9; the counts are whole numbers
+    x = logits(700, 64, torch.bfloat16).float()
+
+    def grad(loss_weight):
+        v = x.clone().requires_grad_(True)
+        gates, _, _, loss = b200norm.route.apply(v, 4)
+        return torch.autograd.grad(loss_weight * loss + (gates * gates).sum() * 1e-3, v)[0]
+
+    want = grad(100.0)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.bfloat16().float() if t.is_floating_point() else t, lambda t: t):
+        got = grad(100.0)
+    assert (got - want).norm() <= 2.0 ** -6 * want.norm()

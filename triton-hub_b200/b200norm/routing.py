@@ -29,8 +29,8 @@ def _workspace_bytes(index, T, E, k, code):
 
 def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True, keep=False):
     """Returns (gates fp32 (..., k), experts int32 (..., k), counts int32 (E + 1,) whose last is the number of live
-    tokens, loss fp32 scalar, lse fp32 (T,) or None).  `keep`: lse is (T + E + 1,), behind the tokens' values the bits of the
-    counts once more, for a backward whose caller gives `counts` away."""
+    tokens, loss fp32 scalar, lse fp32 (T,) or None).  `keep`: lse is int32 (T + E + 1,), the bits of its values and behind
+    them the counts once more, for a backward whose caller gives `counts` away."""
     _require_cuda(logits)
     if logits.dtype == torch.float64:
         raise RuntimeError("b200norm: router logits of dtype torch.float64 are not supported (float32, float16, bfloat16)")
@@ -47,7 +47,11 @@ def _route_fwd(logits, k, normalize=True, mask=None, *, need_lse=True, keep=Fals
     experts = torch.empty(*shape, k, dtype=torch.int32, device=device)
     counts = torch.empty(E + 1, dtype=torch.int32, device=device)
     loss = gates.new_empty(())
-    lse = torch.empty(T + E + 1 if keep else T, dtype=torch.float32, device=device) if need_lse or keep else None
+    lse = None
+    if keep:  # whole numbers, lest a hook on saved tensors should round them
+        lse = torch.empty(T + E + 1, dtype=torch.int32, device=device)
+    elif need_lse:
+        lse = torch.empty(T, dtype=torch.float32, device=device)
     lib = _lib.load()
     index = device.index
     with _on_device(index):
