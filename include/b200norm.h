@@ -379,7 +379,7 @@ B200NORM_API int b200norm_sample(const void* logits, int64_t row_stride, const f
  * b200norm_route_fwd_kept: the same, with the counts written to `kept` (E + 1), too (NULL: not wanted), for callers that hand
  *   `counts` on to code that may change them (a sum over ranks, say) and give `kept` to the backward.
  * b200norm_route_bwd: gradients dgates (T, k) and dloss (one fp32 value on the device), either NULL, to dlogits (T, E)
- *   contiguous; counts are taken as constants.
+ *   contiguous; counts are taken as constants, experts outside [0, E) as none.
  * workspace: at least b200norm_route_workspace_bytes bytes, 16-byte aligned; where that is 1 none is needed, and
  *   workspace may be NULL.
  */

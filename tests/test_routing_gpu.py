@@ -308,3 +308,18 @@ def test_hooks_that_round_saved_numbers():
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t.bfloat16().float() if t.is_floating_point() else t, lambda t: t):
         got = grad(100.0)
     assert (got - want).norm() <= 2.0 ** -6 * want.norm()
+
+
+def test_experts_that_are_none_get_no_gradient():
+    # the saved choices, changed where no version counter sees it, to others that do not exist
+    x = logits(50, 40, torch.float32)
+    for normalize in (False, True):
+        v = x.clone().requires_grad_(True)
+        gates, experts, _, _ = b200norm.route.apply(v, 4, normalize)
+        o = R._route_fwd(x, 4, normalize)
+        dg = torch.randn(50, 4, device=DEV)
+        none = o[1].clone()
+        none[::2, 1] = -1
+        experts.data[::2, 1] = torch.tensor([40, 64, 2 ** 31 - 1, -2, -2 ** 31], device=DEV, dtype=torch.int32).repeat(5)
+        got, = torch.autograd.grad(gates, v, dg)
+        assert torch.equal(got, R._route_bwd(x, o[0], none, o[2], o[4], dg, None, normalize))

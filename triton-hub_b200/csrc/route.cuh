@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(kRouteBwdThreads) route_bwd_kernel(const Route
       total += x[i];
       s = fmaf(x[i], c[i], s);
     }
-    const bool any = e >= 0;
+    const bool any = static_cast<unsigned>(e) < static_cast<unsigned>(p.E);  // -1: none; and no other place is written to
     float g = any ? gate * dg : 0.f;
     const float inv = rcp_fast(warp_sum(total)), sum_g = warp_sum(g);
     s = warp_sum(s) * inv;
